@@ -213,8 +213,7 @@ def prepare(case, seed):
                     c[n][a:b] = x
                 else:
                     c[n][a:b], c[n + "s"][a:b] = _quantise(x.float())
-        s["longest"] = case["longest"]
-    return s
+        return s
 
 
 # ------------------------------------------------------------------------------------------------ plain forms
@@ -349,8 +348,7 @@ def _own(s):
     if op == "cache":
         ops.kv_store(s["k"], s["v"], cache, s["slots"])
         return ops.kv_load(cache, s["slots"])
-    return ops.paged_attention(s["q"], cache, s["page_table"], s["lens"], window=case["window"],
-                               max_len=s["longest"])
+    return ops.paged_attention(s["q"], cache, s["page_table"], s["lens"], window=case["window"])
 
 
 def run(state):
