@@ -49,7 +49,8 @@ typedef enum vpq_status {
   VPQ_ERR_CUDA = 4,        /* CUDA runtime / driver error, or no sm_100 device    */
   VPQ_ERR_NCCL = 5,        /* NCCL missing or returned an error                   */
   VPQ_ERR_TIMEOUT = 6,     /* a bounded device-side wait gave up                  */
-  VPQ_ERR_NOT_FOUND = 7    /* vpq_function(): unknown (library, entry) pair       */
+  VPQ_ERR_NOT_FOUND = 7,   /* vpq_function(): unknown (library, entry) pair       */
+  VPQ_ERR_INDEX = 8        /* an index in device memory was outside of its table  */
 } vpq_status;
 
 int vpq_version(void);
@@ -432,11 +433,112 @@ int vpq_affine_qmm_grouped_w8g64_bf16(int act, const uint32_t* w, const void* sc
                                       const int* rows_map, int64_t experts, int64_t rows, void* x_sorted,
                                       void* stream);
 
+/* --- the attention block between the q|k|v and the o projection ------------
+ * Norm of queries and keys per head with the position rotation, the paged key-value cache (plain or
+ * 8-bit affine) and the attention of one new token per sequence over it: what a decode step runs
+ * between VPQ_EPILOGUE_QKV and VPQ_EPILOGUE_ADD.
+ *
+ * Indices that live in device memory (pages, slots, positions, lengths) cannot be refused by the
+ * host. A negative slot or position marks a padded row and is skipped. Any other index outside of
+ * its table is skipped too (nothing outside a buffer is read or written) and reported by the next
+ * vpq_device_status as VPQ_ERR_INDEX. */
+
+/* A paged cache. Value i of (page, head, token) lies at page * page_stride + head * head_stride +
+ * token * token_stride + i, in elements, of k and of v alike; the three strides all 0: dense
+ * [num_pages, kv_heads, page_size, head_dim]. bits 16: bf16, k_scales and v_scales null. bits 8: codes
+ * of one byte, and per 64 values a bf16 pair (scale, bias) at page * scale_page_stride + head *
+ * scale_head_stride + token * scale_token_stride + 2 * (i / 64) (all 0: dense
+ * [num_pages, kv_heads, page_size, head_dim / 64, 2]); a code c stands for scale * c + bias.
+ * head_dim 64, 128 or 256; page_size a multiple of 16. k, v, k_scales, v_scales and every stride are
+ * 16-byte multiples, except that scale strides need only be multiples of head_dim / 32 elements.
+ * No two (page, head, token) may share bytes. */
+typedef struct vpq_kv_cache {
+  void* k;
+  void* v;
+  void* k_scales;
+  void* v_scales;
+  int64_t num_pages;
+  int32_t page_size, kv_heads, head_dim, bits;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+} vpq_kv_cache;
+
+/* Rows of queries, keys and values as a projection leaves them: head h of token m at
+ * m * q_stride + h * head_dim (elements; stride 0 = heads * head_dim). Outputs likewise; q_out may be q
+ * and k_out may be k (with the same stride), no other overlap.
+ *   x <- x * rsqrt(mean(x^2) + eps) * norm_w     over the head, if norm_w (bf16 [head_dim]) is given
+ *   (a, b) <- (a cos - b sin, b cos + a sin)     for the rot_dim / 2 pairs of the first rot_dim values:
+ *       pair j is (j, j + rot_dim / 2), or (2j, 2j + 1) with interleaved = 1
+ * in f32, rounded to bf16 once. cos_sin [table_rows, rot_dim] f32 holds cos of every pair, then sin;
+ * token m takes row positions[m] (positions null: row m). rot_dim: a multiple of 16, at most head_dim; 0
+ * (cos_sin null): no rotation. All pointers and row strides 16-byte multiples, positions 4 bytes. */
+typedef struct vpq_qk_desc {
+  const void* q;
+  const void* k;
+  const void* v;             /* vpq_qkv_norm_rope_store_bf16 only */
+  void* q_out;
+  void* k_out;               /* vpq_qk_norm_rope_bf16 only */
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  const void* q_norm_w;      /* bf16 [head_dim] or null */
+  const void* k_norm_w;
+  const float* cos_sin;
+  const int32_t* positions;
+  int64_t M, table_rows;
+  int32_t q_heads, kv_heads, head_dim, rot_dim, interleaved;
+  float eps;
+} vpq_qk_desc;
+
+/* q_out, k_out from q and k. A row whose position is not in the table is left as it was. */
+int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream);
+
+/* The same pass with the keys, and the values as they are, going straight to slot slots[m] of the
+ * cache (slot = page * page_size + place in the page; 8-bit codes are made from the unrounded f32
+ * keys). q_out is written for every row whose position is in the table, slot or not; a negative slot
+ * stores nothing. Two rows must not name the same slot. */
+int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const vpq_kv_cache* cache_host,
+                                 const int64_t* slots, void* stream);
+
+/* Rows k, v [M, kv_heads, head_dim] (row strides in elements, 0 = dense) into and out of the cache.
+ * The 8-bit quantizer, per 64 values: bias = min rounded down to bf16, scale = (max - bias) / 255
+ * rounded up to bf16 (at least 2^-126), code = rint((x - bias) / scale), so no value is clipped and each
+ * reads back within scale / 2 (before load's rounding to bf16). 64 values with a NaN or infinity among them, or farther
+ * apart than the largest float, read back as NaN. vpq_kv_load_bf16 gives zeros for a slot outside. */
+int vpq_kv_store_bf16(const vpq_kv_cache* cache_host, const void* k, const void* v, int64_t k_stride,
+                      int64_t v_stride, const int64_t* slots, int64_t M, void* stream);
+int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, int64_t k_stride,
+                     int64_t v_stride, const int64_t* slots, int64_t M, void* stream);
+
+/* Attention of one new token per sequence: head h of sequence b,
+ *   out[b, h] = sum_t softmax_t(scale * q[b, h] . k[t]) v[t]   over tokens t in [len - window, len)
+ * (window 0: [0, len)), len = seq_lens[b], key / value head h / (q_heads / kv_heads); a sequence of
+ * length 0 (or less) gives zeros. Token t lies in page page_table[b * table_stride + t / page_size];
+ * entries of pages outside the token range are not read. A length above max_pages * page_size is cut to it and
+ * reported, a page outside the cache holds no tokens and is reported. Scores, weights' sums and
+ * products accumulate in f32; the result does not depend on timing.
+ * workspace: device memory of vpq_paged_attention_bytes, 16-byte aligned, scratch of this call (calls
+ * that may overlap on the GPU need one each); it needs no initialisation and holds nothing afterwards.
+ * q and out rows: stride in elements, 0 = q_heads * head_dim, 16-byte multiples. q_heads is a multiple of the
+ * cache's kv_heads. scale 0: 1 / sqrt(head_dim). */
+typedef struct vpq_paged_attention_desc {
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  int64_t table_stride;      /* entries between the rows of page_table; 0 = max_pages */
+  int32_t batch, max_pages, q_heads, window;
+  float scale;
+} vpq_paged_attention_desc;
+size_t vpq_paged_attention_bytes(const vpq_paged_attention_desc* desc_host, const vpq_kv_cache* cache_host);
+int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_host, const vpq_kv_cache* cache_host,
+                             void* workspace, size_t bytes, void* stream);
+
 /* Device-side status of the tensor-core kernels: every wait inside them is
  * bounded; one that gives up records where and the kernel returns. Reads the
  * status word of the current device back to the host (synchronises `stream`),
  * clears it, and returns VPQ_OK or VPQ_ERR_TIMEOUT with *detail set to the
- * recorded code. The analogue of Fence::wait_ok(&reason),
+ * recorded code; or VPQ_ERR_INDEX if the attention block met a page, slot, position or length outside
+ * of its table since the last call (detail 0x40000 | 1 page, 2 slot, 4 position, 8 length). The analogue of Fence::wait_ok(&reason),
  * apple-silicon/metal-compute/command-stream.h:92-99. */
 int vpq_device_status(void* stream, uint32_t* detail);
 

@@ -1,0 +1,199 @@
+"""CPU tests of the attention block's entry points: what they refuse, with which status, before any launch; and how
+the Python front end refuses. Valid calls end at VPQ_ERR_CUDA here (no CPU path)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from vpipe_b200 import _lib
+
+INVALID, ALIGN, UNSUPPORTED, CUDA = 1, 2, 3, 4
+P = 0x7F0000000000  # an address that is never used: every call below ends on the host
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses below are made up: host checks only")
+
+
+def cache(**kw):
+    c = _lib.KvCache()
+    c.k, c.v, c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.bits = P, P + (1 << 30), 64, 32, 8, 128, 16
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def cache8(**kw):
+    return cache(**{**dict(bits=8, k_scales=P + (2 << 30), v_scales=P + (3 << 30)), **kw})
+
+
+def qk(**kw):
+    d = _lib.QkDesc()
+    d.q, d.k, d.v, d.q_out, d.k_out = P, P + 4096, P + 8192, P + 16384, P + 32768
+    d.M, d.q_heads, d.kv_heads, d.head_dim, d.eps = 3, 32, 8, 128, 1e-6
+    d.cos_sin, d.positions, d.table_rows, d.rot_dim = P + 65536, P + 131072, 100, 128
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def attn(**kw):
+    d = _lib.PagedAttentionDesc()
+    d.q, d.out, d.page_table, d.seq_lens = P, P + 4096, P + 8192, P + 16384
+    d.batch, d.max_pages, d.q_heads = 4, 10, 32
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def norm_rope(L, d):
+    return L.vpq_qk_norm_rope_bf16(C.byref(d), None)
+
+
+def store_pass(L, d, c, slots=P):
+    return L.vpq_qkv_norm_rope_store_bf16(C.byref(d), C.byref(c), slots, None)
+
+
+def attend(L, d, c, ws=P, size=1 << 30):
+    return L.vpq_paged_attention_bf16(C.byref(d), C.byref(c), ws, size, None)
+
+
+def test_valid_calls_reach_the_device_check(vpq):
+    L = vpq.lib()
+    assert norm_rope(L, qk()) == CUDA
+    assert norm_rope(L, qk(q_out=P, k_out=P + 4096)) == CUDA
+    assert norm_rope(L, qk(cos_sin=None, positions=None, rot_dim=0, table_rows=0)) == CUDA
+    assert norm_rope(L, qk(positions=None)) == CUDA
+    for c in (cache(), cache8(), cache(page_stride=128 * 8 * 32 * 2, head_stride=128, token_stride=1024)):
+        assert store_pass(L, qk(), c) == CUDA
+        assert L.vpq_kv_store_bf16(C.byref(c), P, P, 0, 0, P, 5, None) == CUDA
+        assert L.vpq_kv_load_bf16(C.byref(c), P, P, 0, 2048, P, 5, None) == CUDA
+        assert attend(L, attn(), c) == CUDA
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(M=0), INVALID), (dict(M=-1), INVALID), (dict(q_heads=0), INVALID), (dict(kv_heads=0), INVALID),
+    (dict(head_dim=96), UNSUPPORTED), (dict(head_dim=0), UNSUPPORTED), (dict(q=None), INVALID), (dict(k=None), INVALID),
+    (dict(q_out=None), INVALID), (dict(k_out=None), INVALID), (dict(q=P + 8), ALIGN), (dict(k=P + 2), ALIGN),
+    (dict(q_out=P + 4), ALIGN), (dict(q_stride=4095), INVALID), (dict(q_stride=4100), ALIGN),
+    (dict(k_stride=1000), INVALID), (dict(k_stride=-1024), INVALID), (dict(q_stride=1 << 62), INVALID),
+    (dict(rot_dim=8), INVALID), (dict(rot_dim=144), INVALID), (dict(rot_dim=0), INVALID), (dict(rot_dim=-16), INVALID),
+    (dict(table_rows=0), INVALID), (dict(positions=None, table_rows=2), INVALID), (dict(positions=P + 2), ALIGN),
+    (dict(cos_sin=P + 4), ALIGN), (dict(cos_sin=None), INVALID), (dict(cos_sin=None, rot_dim=0), INVALID),
+    (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID), (dict(q_norm_w=P + 2), ALIGN),
+    (dict(k_norm_w=P + 8), ALIGN), (dict(q_out=P, q_out_stride=8192), INVALID),
+    (dict(k_out=P + 4096, k_out_stride=2048), INVALID), (dict(q_heads=1 << 20), UNSUPPORTED),
+])
+def test_norm_rope_refuses(vpq, kw, code):
+    assert norm_rope(vpq.lib(), qk(**kw)) == code
+    assert vpq.lib().vpq_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(bits=4), UNSUPPORTED), (dict(bits=8), INVALID), (dict(k=None), INVALID), (dict(v=None), INVALID),
+    (dict(num_pages=0), INVALID), (dict(num_pages=1 << 31), INVALID), (dict(kv_heads=0), INVALID),
+    (dict(head_dim=80), UNSUPPORTED), (dict(page_size=0), UNSUPPORTED), (dict(page_size=24), UNSUPPORTED),
+    (dict(page_size=-16), UNSUPPORTED), (dict(k=P + 8), ALIGN), (dict(v=P + 1), ALIGN), (dict(k_scales=P), INVALID),
+    (dict(token_stride=64, head_stride=4096, page_stride=32768), INVALID),
+    (dict(token_stride=132, head_stride=8192, page_stride=65536), ALIGN),
+    (dict(token_stride=128, head_stride=0, page_stride=32768), INVALID),
+    (dict(token_stride=128, head_stride=4096, page_stride=-32768), INVALID),
+    (dict(token_stride=128, head_stride=4096, page_stride=1 << 60), INVALID),
+])
+def test_a_cache_is_checked(vpq, kw, code):
+    L = vpq.lib()
+    c = cache(**kw)
+    assert L.vpq_kv_store_bf16(C.byref(c), P, P, 0, 0, P, 5, None) == code
+    assert L.vpq_kv_load_bf16(C.byref(c), P, P, 0, 0, P, 5, None) == code
+    heads = 32 if c.kv_heads <= 0 else 4 * c.kv_heads
+    assert attend(L, attn(q_heads=heads), c) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(k_scales=None), INVALID), (dict(v_scales=None), INVALID), (dict(k_scales=P + 4), ALIGN),
+    (dict(scale_token_stride=2, scale_head_stride=128, scale_page_stride=1024), INVALID),
+    (dict(scale_token_stride=6, scale_head_stride=192, scale_page_stride=1536), ALIGN),
+    (dict(token_stride=136, head_stride=8192, page_stride=65536), ALIGN),
+])
+def test_an_8_bit_cache_is_checked(vpq, kw, code):
+    L = vpq.lib()
+    c = cache8(**kw)
+    assert L.vpq_kv_store_bf16(C.byref(c), P, P, 0, 0, P, 5, None) == code
+    assert attend(L, attn(), c) == code
+
+
+def test_store_pass_refuses(vpq):
+    L = vpq.lib()
+    assert store_pass(L, qk(v=None), cache()) == INVALID
+    assert store_pass(L, qk(v=P + 2), cache()) == ALIGN
+    assert store_pass(L, qk(v_stride=100), cache()) == INVALID
+    assert store_pass(L, qk(), cache(kv_heads=4)) == INVALID
+    assert store_pass(L, qk(), cache(head_dim=64)) == INVALID
+    assert store_pass(L, qk(), cache(), None) == INVALID
+    assert store_pass(L, qk(), cache(), P + 4) == ALIGN
+    assert L.vpq_qkv_norm_rope_store_bf16(None, C.byref(cache()), P, None) == INVALID
+    assert L.vpq_qkv_norm_rope_store_bf16(C.byref(qk()), None, P, None) == INVALID
+    assert L.vpq_qk_norm_rope_bf16(None, None) == INVALID
+
+
+def test_store_and_load_refuse(vpq):
+    L = vpq.lib()
+    for f in (L.vpq_kv_store_bf16, L.vpq_kv_load_bf16):
+        c = C.byref(cache())
+        assert f(None, P, P, 0, 0, P, 5, None) == INVALID
+        assert f(c, None, P, 0, 0, P, 5, None) == INVALID
+        assert f(c, P, None, 0, 0, P, 5, None) == INVALID
+        assert f(c, P, P, 0, 0, None, 5, None) == INVALID
+        assert f(c, P, P, 0, 0, P, 0, None) == INVALID
+        assert f(c, P, P, 0, 0, P, -3, None) == INVALID
+        assert f(c, P, P, 512, 0, P, 5, None) == INVALID
+        assert f(c, P, P, 0, 1028, P, 5, None) == ALIGN
+        assert f(c, P + 2, P, 0, 0, P, 5, None) == ALIGN
+        assert f(c, P, P, 0, 0, P + 2, 5, None) == ALIGN
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(q=None), INVALID), (dict(out=None), INVALID), (dict(page_table=None), INVALID), (dict(seq_lens=None), INVALID),
+    (dict(batch=0), INVALID), (dict(batch=-2), INVALID), (dict(max_pages=0), INVALID), (dict(q_heads=0), INVALID),
+    (dict(q_heads=12), INVALID), (dict(q_heads=65544), UNSUPPORTED), (dict(window=-1), INVALID),
+    (dict(scale=-0.5), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
+    (dict(q=P + 2), ALIGN), (dict(out=P + 8), ALIGN), (dict(q_stride=4092), INVALID), (dict(q_stride=4100), ALIGN),
+    (dict(out_stride=100), INVALID), (dict(out_stride=1 << 50), INVALID), (dict(table_stride=9), INVALID),
+    (dict(page_table=P + 2), ALIGN), (dict(seq_lens=P + 1), ALIGN), (dict(max_pages=1 << 27), UNSUPPORTED),
+])
+def test_paged_attention_refuses(vpq, kw, code):
+    assert attend(vpq.lib(), attn(**kw), cache()) == code
+    assert vpq.lib().vpq_last_error()
+
+
+def test_paged_attention_workspace(vpq):
+    L = vpq.lib()
+    need = L.vpq_paged_attention_bytes(C.byref(attn()), C.byref(cache()))
+    assert need > 0
+    assert attend(L, attn(), cache(), P, need) == CUDA
+    assert attend(L, attn(), cache(), P, need - 1) == INVALID
+    assert attend(L, attn(), cache(), None, need) == INVALID
+    assert attend(L, attn(), cache(), P + 8, need) == ALIGN
+    assert L.vpq_paged_attention_bytes(None, C.byref(cache())) == 0
+    assert L.vpq_paged_attention_bytes(C.byref(attn(q_heads=12)), C.byref(cache())) == 0
+    # every batch the call takes has its prefix in there
+    big = L.vpq_paged_attention_bytes(C.byref(attn(batch=1 << 20)), C.byref(cache()))
+    assert big >= need + ((1 << 20) - 4) * 8
+
+
+def test_python_refuses_cpu_tensors_and_wrong_types(vpq):
+    ops = vpq.ops
+    q, k = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.qk_norm_rope(q, k)
+    with pytest.raises(ValueError, match="bfloat16"):
+        ops.qk_norm_rope(q.float(), k)
+    pages = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.PagedKVCache(pages, pages.clone())
+    with pytest.raises(ValueError, match="scales"):
+        ops.PagedKVCache(pages.to(torch.uint8), pages.to(torch.uint8))
+    with pytest.raises(ValueError, match="16 or 8"):
+        ops.PagedKVCache.empty(2, 16, 2, 64, bits=4, device="cpu")
+
+
+def test_status_string_of_a_bad_index(vpq):
+    assert vpq.status_string(8) not in ("ok", "unknown status")

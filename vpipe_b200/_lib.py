@@ -65,6 +65,12 @@ SYMBOLS = [
     ("vpq_qmv_plan_run", _i, [_vp, _vp]),
     ("vpq_qmv_plan_destroy", _i, [_vp]),
     ("vpq_affine_qmm_w4g64_bf16", _i, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    ("vpq_qk_norm_rope_bf16", _i, [_vp, _vp]),
+    ("vpq_qkv_norm_rope_store_bf16", _i, [_vp, _vp, _vp, _vp]),
+    ("vpq_kv_store_bf16", _i, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    ("vpq_kv_load_bf16", _i, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    ("vpq_paged_attention_bytes", C.c_size_t, [_vp, _vp]),
+    ("vpq_paged_attention_bf16", _i, [_vp, _vp, _vp, C.c_size_t, _vp]),
     ("vpq_device_status", _i, [_vp, C.POINTER(C.c_uint32)]),
     ("vpq_wait_probe", _i, [C.c_uint32, C.c_uint32, _vp]),
     ("vpq_peer_barrier_probe", _i, [_vp, _i, _i, C.c_uint32, _vp]),
@@ -102,6 +108,34 @@ class LinearDesc(C.Structure):
                 ("k_rows", C.c_int64), ("norm_w", C.c_void_p), ("expert", C.c_void_p),
                 ("experts", C.c_int64), ("x_div", C.c_int32), ("eps", C.c_float),
                 ("row_map", C.c_void_p), ("row_gather", C.c_int32), ("expert_div", C.c_int32)]
+
+
+class KvCache(C.Structure):
+    """struct vpq_kv_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("num_pages", C.c_int64), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("bits", C.c_int32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("scale_page_stride", C.c_int64), ("scale_head_stride", C.c_int64),
+                ("scale_token_stride", C.c_int64)]
+
+
+class QkDesc(C.Structure):
+    """struct vpq_qk_desc"""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_out", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_out_stride", C.c_int64), ("k_out_stride", C.c_int64), ("q_norm_w", C.c_void_p),
+                ("k_norm_w", C.c_void_p), ("cos_sin", C.c_void_p), ("positions", C.c_void_p), ("M", C.c_int64),
+                ("table_rows", C.c_int64), ("q_heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
+
+
+class PagedAttentionDesc(C.Structure):
+    """struct vpq_paged_attention_desc"""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("table_stride", C.c_int64),
+                ("batch", C.c_int32), ("max_pages", C.c_int32), ("q_heads", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float)]
 
 
 class VpqError(RuntimeError):

@@ -174,6 +174,7 @@ extern "C" const char* vpq_status_string(int status) {
     case VPQ_ERR_NCCL: return "NCCL error";
     case VPQ_ERR_TIMEOUT: return "device-side wait timed out";
     case VPQ_ERR_NOT_FOUND: return "unknown library or entry";
+    case VPQ_ERR_INDEX: return "index in device memory outside of its table";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,566 @@
+// kv_cache.cu -- norm of queries and keys per head with the position rotation, and the paged
+// key-value cache's store (plain, or 8-bit affine) and load. All memory streams: a few dozen
+// instructions per 16 bytes, each row read once and written once.
+#include "vpq_kv.cuh"
+
+#include <climits>
+
+namespace vpq {
+
+__device__ uint32_t g_kv_status = 0;
+
+namespace {
+
+// One head's row is D values, eight (16 bytes) per lane: LPH = D / 8 lanes hold it, and every
+// reduction (the norm's sum, a group's extremes) and the exchange of rotation partners is a shuffle
+// among them. A head is processed in registers from load to store, so q_out = q is safe.
+struct QkArgs {
+  const uint8_t* in[3];  // q, k, v rows; null where there are none
+  uint8_t* out[2];       // q, k rows out
+  int64_t in_stride[3];  // bytes
+  int64_t out_stride[2];
+  const uint16_t* norm_w[2];
+  const float* cos_sin;
+  const int32_t* positions;
+  const int64_t* slots;
+  int64_t M, table_rows, num_slots;
+  int heads[3];
+  int chunks;      // lane groups that share a token's heads
+  int rot, interleaved;
+  float eps, inv_d;
+  KvView kv;
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ void unpack8(const uint4 r, float (&x)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+
+// The 8-bit quantizer over the 64 values of eight lanes. The bias is the minimum rounded DOWN to
+// bf16 and the scale is rounded UP, so min and max both lie inside the code range: with nearest rounding a group
+// whose offset is large against its spread would lose values to clipping (the bias alone is off by
+// up to 2^-9 of the offset). The scale's floor of 2^-126 keeps its reciprocal finite; a group of
+// equal values takes code 0. A NaN or infinity among the 64 (or a spread beyond the largest float) makes the
+// pair NaN, so the group reads back as NaN.
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
+  float mn = x[0], mx = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    mn = min_nan(mn, x[i]);
+    mx = max_nan(mx, x[i]);
+  }
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) {
+    mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  }
+  const __nv_bfloat16 b16 = __float2bfloat16_rd(mn);
+  const float b = __bfloat162float(b16);
+  const float range = __fsub_rn(mx, b);
+  const __nv_bfloat16 s16 = __float2bfloat16_ru(fmaxf(__fdiv_rn(range, 255.0f), 1.17549435e-38f));
+  const float inv = __fdiv_rn(1.0f, __bfloat162float(s16));
+  const bool fine = range <= 3.402823466e38f;  // false for NaN
+  pair = fine ? ((uint32_t)__bfloat16_as_ushort(s16) | ((uint32_t)__bfloat16_as_ushort(b16) << 16)) : 0x7fff7fffu;
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = (uint32_t)__float2int_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], b), inv), 0.0f), 255.0f));
+  }
+  return make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
+}
+
+// MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads a lane
+// group takes, all loaded before the first is used.
+template <int D, int MODE, int HPT>
+__global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
+  constexpr int LPH = D / 8;
+  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  const int l = threadIdx.x % LPH;
+  const int64_t m_raw = id / A.chunks;
+  const int chunk = (int)(id - m_raw * A.chunks);
+  const bool in_range = m_raw < A.M;
+  const int64_t m = in_range ? m_raw : 0;  // lanes past the end keep their warp's shuffles company
+  const int hq = A.heads[0], hqk = hq + A.heads[1];
+  const int total = hqk + (MODE ? A.heads[2] : 0);
+
+  bool turn = in_range;  // whether the rotated parts of this token are written
+  int64_t row = m;
+  if (A.cos_sin && A.positions) {
+    const int p = __ldg(A.positions + m);
+    turn = in_range && p >= 0 && p < A.table_rows;
+    if (in_range && p >= A.table_rows && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
+    row = turn ? p : 0;
+  }
+  bool store = false;
+  int64_t page = 0, at = 0;
+  if (MODE) {
+    const int64_t s = __ldg(A.slots + m);
+    store = in_range && turn && s >= 0 && s < A.num_slots;
+    if (in_range && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+    if (store) {
+      page = s / A.kv.page_size;
+      at = s - page * A.kv.page_size;
+    }
+  }
+
+  uint4 raw[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int h = chunk + i * A.chunks;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (in_range && h < total) {
+      const int part = h < hq ? 0 : (h < hqk ? 1 : 2);
+      const int hh = h - (part == 0 ? 0 : (part == 1 ? hq : hqk));
+      raw[i] = *reinterpret_cast<const uint4*>(A.in[part] + m * A.in_stride[part] + (int64_t)hh * (D * 2) + l * 16);
+    }
+  }
+
+  // this lane's eight values and their place among the pairs
+  const int d0 = l * 8, half = A.rot >> 1;
+  float cs[8], sn[8];
+  int partner = l;
+  bool second = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { cs[i] = 1.0f, sn[i] = 0.0f; }
+  const bool rotated = A.cos_sin && d0 < A.rot;
+  if (rotated) {
+    const float* t = A.cos_sin + row * A.rot;
+    if (A.interleaved) {
+      const float4 c = __ldg(reinterpret_cast<const float4*>(t + (d0 >> 1)));
+      const float4 s = __ldg(reinterpret_cast<const float4*>(t + half + (d0 >> 1)));
+      cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
+      sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
+    } else {
+      second = d0 >= half;
+      const int j = second ? d0 - half : d0;
+      partner = second ? l - (half >> 3) : l + (half >> 3);
+      const float4 c0 = __ldg(reinterpret_cast<const float4*>(t + j)), c1 = __ldg(reinterpret_cast<const float4*>(t + j + 4));
+      const float4 s0 = __ldg(reinterpret_cast<const float4*>(t + half + j));
+      const float4 s1 = __ldg(reinterpret_cast<const float4*>(t + half + j + 4));
+      cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
+      sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w, sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int h = chunk + i * A.chunks;
+    if (__all_sync(0xffffffffu, h >= total)) { break; }
+    const int part = h < hq ? 0 : (h < hqk ? 1 : 2);
+    const int hh = h - (part == 0 ? 0 : (part == 1 ? hq : hqk));
+    float x[8];
+    unpack8(raw[i], x);
+    // lanes of a warp can hold heads of different parts: the shuffles below run for all, the values of v are kept
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
+#pragma unroll
+    for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
+    if (part < 2 && h < total && A.norm_w[part]) {
+      float w[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(A.norm_w[part] + d0)), w);
+      const float r = rsqrtf(__fmaf_rn(ss, A.inv_d, A.eps));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { x[e] = x[e] * r * w[e]; }
+    }
+    if (A.interleaved) {
+      if (part < 2 && rotated) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = x[2 * e], b = x[2 * e + 1];
+          x[2 * e] = a * cs[e] - b * sn[e];
+          x[2 * e + 1] = b * cs[e] + a * sn[e];
+        }
+      }
+    } else if (A.cos_sin) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float o = __shfl_sync(0xffffffffu, x[e], partner, LPH);
+        if (part < 2 && rotated) { x[e] = second ? x[e] * cs[e] + o * sn[e] : x[e] * cs[e] - o * sn[e]; }
+      }
+    }
+    if (MODE == 0 || part == 0) {
+      if (turn && h < total) {
+        uint8_t* o = A.out[part] + m * A.out_stride[part] + (int64_t)hh * (D * 2) + l * 16;
+        *reinterpret_cast<uint4*>(o) = pack8(x);
+      }
+    }
+    if (MODE == 16) {
+      if (store && part > 0 && h < total) {
+        uint8_t* base = part == 1 ? A.kv.k : A.kv.v;
+        const int64_t off = page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes + l * 16;
+        *reinterpret_cast<uint4*>(base + off) = pack8(x);
+      }
+    }
+    if (MODE == 8 && __any_sync(0xffffffffu, part > 0)) {
+      uint32_t pair;
+      const uint2 c = quant8(x, pair);
+      if (store && part > 0 && h < total) {
+        const int64_t off = page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes + l * 8;
+        *reinterpret_cast<uint2*>((part == 1 ? A.kv.k : A.kv.v) + off) = c;
+        if ((l & 7) == 0) {
+          const int64_t so = page * A.kv.spage_bytes + hh * A.kv.shead_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4;
+          *reinterpret_cast<uint32_t*>((part == 1 ? A.kv.ks : A.kv.vs) + so) = pair;
+        }
+      }
+    }
+  }
+}
+
+struct LoadArgs {
+  KvView kv;
+  uint8_t* out[2];
+  int64_t stride[2];  // bytes
+  const int64_t* slots;
+  int64_t M, num_slots;
+};
+
+// Eight values a thread: 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out.
+template <int D, int BITS>
+__global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs A) {
+  constexpr int LPH = D / 8;
+  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  const int l = threadIdx.x % LPH;
+  const int heads = 2 * A.kv.kv_heads;
+  const int64_t m = id / heads;
+  if (m >= A.M) { return; }
+  const int h = (int)(id - m * heads);
+  const bool is_v = h >= A.kv.kv_heads;
+  const int hh = is_v ? h - A.kv.kv_heads : h;
+  const int64_t s = __ldg(A.slots + m);
+  uint4 y = make_uint4(0, 0, 0, 0);
+  if (s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+  if (s >= 0 && s < A.num_slots) {
+    const int64_t page = s / A.kv.page_size, at = s - page * A.kv.page_size;
+    const uint8_t* p = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes;
+    if (BITS == 16) {
+      y = *reinterpret_cast<const uint4*>(p + l * 16);
+    } else {
+      const uint2 c = *reinterpret_cast<const uint2*>(p + l * 8);
+      const uint32_t pair = *reinterpret_cast<const uint32_t*>((is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes +
+                                                              hh * A.kv.shead_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4);
+      const float sc = __uint_as_float(pair << 16), b = __uint_as_float(pair & 0xffff0000u);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = dequant_f32(sc, (c.x >> (8 * i)) & 0xffu, b);
+        x[4 + i] = dequant_f32(sc, (c.y >> (8 * i)) & 0xffu, b);
+      }
+      y = pack8(x);
+    }
+  }
+  *reinterpret_cast<uint4*>(A.out[is_v] + m * A.stride[is_v] + (int64_t)hh * (D * 2) + l * 16) = y;
+}
+
+bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
+
+template <int MODE>
+int launch_norm(const char* who, const QkArgs& a0, int D, cudaStream_t st) {
+  QkArgs a = a0;
+  const int total = a.heads[0] + a.heads[1] + (MODE ? a.heads[2] : 0);
+  const int64_t per_block = 256 / (D / 8);
+  // One head per lane group while the launch is too small to fill the machine (a decode step lives by
+  // latency); four once there is a wave of them, so the table's row and the norm weights are fetched
+  // once per four heads and four loads are in flight.
+  const bool wide = a.M * total > (int64_t)num_sms() * 8 * per_block * 4;
+  const int hpt = wide ? 4 : 1;
+  a.chunks = (total + hpt - 1) / hpt;
+  const int64_t blocks = (a.M * a.chunks + per_block - 1) / per_block;
+  if (blocks > INT_MAX) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)a.M); }
+  const dim3 g((unsigned)blocks);
+#define VPQ_GO(DD)                                                   \
+  if (wide) {                                                        \
+    norm_rope_store_kernel<DD, MODE, 4><<<g, 256, 0, st>>>(a);       \
+  } else {                                                           \
+    norm_rope_store_kernel<DD, MODE, 1><<<g, 256, 0, st>>>(a);       \
+  }
+  if (D == 64) {
+    VPQ_GO(64)
+  } else if (D == 128) {
+    VPQ_GO(128)
+  } else {
+    VPQ_GO(256)
+  }
+#undef VPQ_GO
+  VPQ_LAUNCH_OK(who);
+  return VPQ_OK;
+}
+
+bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
+
+// Fills and checks one row operand; stride 0 = dense.
+int take_rows(const char* who, const char* name, const void* p, int64_t stride, int64_t heads, int D, int64_t M,
+              int64_t* bytes) {
+  if (!p) { return fail(VPQ_ERR_INVALID_ARG, "%s: %s is null", who, name); }
+  if (stride == 0) { stride = heads * D; }
+  if (stride < heads * D) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: %s rows overlap (stride %lld for %lld values)", who, name, (long long)stride,
+                (long long)(heads * D));
+  }
+  if (stride > (INT64_MAX / 2) / M) { return fail(VPQ_ERR_INVALID_ARG, "%s: %s stride out of range", who, name); }
+  if (!aligned16(p) || (stride & 7)) {
+    return fail(VPQ_ERR_ALIGNMENT, "%s: %s and its row stride must be multiples of 16 bytes", who, name);
+  }
+  *bytes = stride * 2;
+  return VPQ_OK;
+}
+
+// The part of a vpq_qk_desc that both entry points share.
+int take_qk(const char* who, const vpq_qk_desc& d, QkArgs* a) {
+  if (d.M <= 0 || d.q_heads <= 0 || d.kv_heads <= 0) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: need M>0, q_heads>0, kv_heads>0 (M=%lld q_heads=%d kv_heads=%d)", who,
+                (long long)d.M, d.q_heads, d.kv_heads);
+  }
+  if (!known_dim(d.head_dim)) {
+    return fail(VPQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256 (got %d)", who, d.head_dim);
+  }
+  if (d.q_heads > 65536 || d.kv_heads > 65536 || d.M > (int64_t)1 << 40) {
+    return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 heads and 2^40 rows", who);
+  }
+  if (d.cos_sin) {
+    if (d.rot_dim <= 0 || d.rot_dim > d.head_dim || (d.rot_dim & 15)) {
+      return fail(VPQ_ERR_INVALID_ARG, "%s: rot_dim must be a multiple of 16 up to head_dim (rot_dim=%d head_dim=%d)", who,
+                  d.rot_dim, d.head_dim);
+    }
+    if (d.table_rows <= 0 || (!d.positions && d.table_rows < d.M)) {
+      return fail(VPQ_ERR_INVALID_ARG, "%s: cos_sin has %lld rows, %lld are needed", who, (long long)d.table_rows,
+                  (long long)(d.positions ? 1 : d.M));
+    }
+    if (!aligned16(d.cos_sin) || (reinterpret_cast<uintptr_t>(d.positions) & 3)) {
+      return fail(VPQ_ERR_ALIGNMENT, "%s: cos_sin must be 16-byte aligned, positions 4-byte", who);
+    }
+  } else if (d.rot_dim != 0 || d.positions) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: rot_dim and positions need cos_sin", who);
+  }
+  if (!(d.eps >= 0.0f)) { return fail(VPQ_ERR_INVALID_ARG, "%s: eps must not be negative", who); }
+  if (!aligned16(d.q_norm_w) || !aligned16(d.k_norm_w)) {
+    return fail(VPQ_ERR_ALIGNMENT, "%s: norm weights must be 16-byte aligned", who);
+  }
+  a->norm_w[0] = static_cast<const uint16_t*>(d.q_norm_w);
+  a->norm_w[1] = static_cast<const uint16_t*>(d.k_norm_w);
+  a->cos_sin = d.cos_sin;
+  a->positions = d.positions;
+  a->M = d.M;
+  a->table_rows = d.table_rows;
+  a->heads[0] = d.q_heads;
+  a->heads[1] = d.kv_heads;
+  a->heads[2] = d.kv_heads;
+  a->rot = d.rot_dim;
+  a->interleaved = d.interleaved != 0;
+  a->eps = d.eps;
+  a->inv_d = 1.0f / (float)d.head_dim;
+  if (int rc = take_rows(who, "q", d.q, d.q_stride, d.q_heads, d.head_dim, d.M, &a->in_stride[0])) { return rc; }
+  if (int rc = take_rows(who, "k", d.k, d.k_stride, d.kv_heads, d.head_dim, d.M, &a->in_stride[1])) { return rc; }
+  if (int rc = take_rows(who, "q_out", d.q_out, d.q_out_stride, d.q_heads, d.head_dim, d.M, &a->out_stride[0])) { return rc; }
+  a->in[0] = static_cast<const uint8_t*>(d.q);
+  a->in[1] = static_cast<const uint8_t*>(d.k);
+  a->out[0] = static_cast<uint8_t*>(d.q_out);
+  if (d.q_out == d.q && a->out_stride[0] != a->in_stride[0]) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: q_out is q with another row stride", who);
+  }
+  return VPQ_OK;
+}
+
+int take_slots(const char* who, const int64_t* slots) {
+  if (!slots) { return fail(VPQ_ERR_INVALID_ARG, "%s: slots is null", who); }
+  if (reinterpret_cast<uintptr_t>(slots) & 7) { return fail(VPQ_ERR_ALIGNMENT, "%s: slots must be 8-byte aligned", who); }
+  return VPQ_OK;
+}
+
+}  // namespace
+
+int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
+  if (!c) { return fail(VPQ_ERR_INVALID_ARG, "%s: null cache", who); }
+  if (c->bits != 8 && c->bits != 16) { return fail(VPQ_ERR_UNSUPPORTED, "%s: a cache has 16 or 8 bits (got %d)", who, c->bits); }
+  if (!known_dim(c->head_dim)) {
+    return fail(VPQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256 (got %d)", who, c->head_dim);
+  }
+  if (c->num_pages <= 0 || c->num_pages > INT_MAX || c->kv_heads <= 0 || c->kv_heads > 65536) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < num_pages < 2^31, 0 < kv_heads <= 65536 (num_pages=%lld kv_heads=%d)", who,
+                (long long)c->num_pages, c->kv_heads);
+  }
+  if (c->page_size <= 0 || (c->page_size & 15) || c->page_size > (1 << 20)) {
+    return fail(VPQ_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16, at most 2^20 (got %d)", who, c->page_size);
+  }
+  const bool q = c->bits == 8;
+  if (!c->k || !c->v || (q && (!c->k_scales || !c->v_scales))) { return fail(VPQ_ERR_INVALID_ARG, "%s: null pages", who); }
+  if (!q && (c->k_scales || c->v_scales)) { return fail(VPQ_ERR_INVALID_ARG, "%s: a 16-bit cache has no scales", who); }
+  if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scales) || !aligned16(c->v_scales)) {
+    return fail(VPQ_ERR_ALIGNMENT, "%s: pages and scales must be 16-byte aligned", who);
+  }
+  const int64_t D = c->head_dim, elt = q ? 1 : 2;
+  int64_t ps = c->page_stride, hs = c->head_stride, ts = c->token_stride;
+  if (!ps && !hs && !ts) { ts = D, hs = ts * c->page_size, ps = hs * c->kv_heads; }
+  const int64_t pairs = D / kKvGroup * 2;
+  int64_t sps = c->scale_page_stride, shs = c->scale_head_stride, sts = c->scale_token_stride;
+  if (!sps && !shs && !sts) { sts = pairs, shs = sts * c->page_size, sps = shs * c->kv_heads; }
+  if (ts < D || (hs < D && c->kv_heads > 1) || (ps < D && c->num_pages > 1) || hs < 0 || ps < 0 ||
+      (q && (sts < pairs || (shs < pairs && c->kv_heads > 1) || (sps < pairs && c->num_pages > 1) || shs < 0 || sps < 0))) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is smaller than a row", who);
+  }
+  const int64_t lim = (int64_t)1 << 46;  // of one term, in elements: no sum of three passes 2^48
+  if (ts > lim / c->page_size || hs > lim / c->kv_heads || ps > lim / c->num_pages || sts > lim / c->page_size ||
+      shs > lim / c->kv_heads || sps > lim / c->num_pages) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is out of range", who);
+  }
+  const int64_t mult = 16 / elt;
+  if (!strides_ok(ts, mult) || !strides_ok(hs, mult) || !strides_ok(ps, mult) ||
+      (q && (!strides_ok(sts, pairs) || !strides_ok(shs, pairs) || !strides_ok(sps, pairs)))) {
+    return fail(VPQ_ERR_ALIGNMENT, "%s: page strides must be multiples of 16 bytes, scale strides of head_dim / 32", who);
+  }
+  view->k = static_cast<uint8_t*>(c->k);
+  view->v = static_cast<uint8_t*>(c->v);
+  view->ks = static_cast<uint8_t*>(c->k_scales);
+  view->vs = static_cast<uint8_t*>(c->v_scales);
+  view->num_pages = c->num_pages;
+  view->page_bytes = ps * elt;
+  view->head_bytes = hs * elt;
+  view->token_bytes = ts * elt;
+  view->spage_bytes = sps * 2;
+  view->shead_bytes = shs * 2;
+  view->stoken_bytes = sts * 2;
+  view->page_size = c->page_size;
+  view->kv_heads = c->kv_heads;
+  return VPQ_OK;
+}
+
+int kv_status_read(cudaStream_t st, uint32_t* out) {
+  uint32_t v = 0;
+  VPQ_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, g_kv_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st));
+  VPQ_CUDA_OK(cudaStreamSynchronize(st));
+  if (v != 0) {
+    const uint32_t zero = 0;
+    VPQ_CUDA_OK(cudaMemcpyToSymbolAsync(g_kv_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
+    VPQ_CUDA_OK(cudaStreamSynchronize(st));
+  }
+  *out = v;
+  return VPQ_OK;
+}
+
+}  // namespace vpq
+
+using namespace vpq;
+
+extern "C" int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream) {
+  const char* who = "qk_norm_rope";
+  clear_error();
+  if (!desc_host) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
+  QkArgs a = {};
+  if (int rc = take_qk(who, *desc_host, &a)) { return rc; }
+  if (int rc = take_rows(who, "k_out", desc_host->k_out, desc_host->k_out_stride, desc_host->kv_heads, desc_host->head_dim,
+                         desc_host->M, &a.out_stride[1])) {
+    return rc;
+  }
+  a.out[1] = static_cast<uint8_t*>(desc_host->k_out);
+  if (desc_host->k_out == desc_host->k && a.out_stride[1] != a.in_stride[1]) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: k_out is k with another row stride", who);
+  }
+  if (int rc = require_sm100()) { return rc; }
+  return launch_norm<0>(who, a, desc_host->head_dim, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const vpq_kv_cache* cache_host,
+                                            const int64_t* slots, void* stream) {
+  const char* who = "qkv_norm_rope_store";
+  clear_error();
+  if (!desc_host) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
+  QkArgs a = {};
+  if (int rc = take_qk(who, *desc_host, &a)) { return rc; }
+  if (int rc = take_rows(who, "v", desc_host->v, desc_host->v_stride, desc_host->kv_heads, desc_host->head_dim,
+                         desc_host->M, &a.in_stride[2])) {
+    return rc;
+  }
+  a.in[2] = static_cast<const uint8_t*>(desc_host->v);
+  if (int rc = kv_check(who, cache_host, &a.kv)) { return rc; }
+  if (cache_host->kv_heads != desc_host->kv_heads || cache_host->head_dim != desc_host->head_dim) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: the cache has %d heads of %d, the rows %d of %d", who, cache_host->kv_heads,
+                cache_host->head_dim, desc_host->kv_heads, desc_host->head_dim);
+  }
+  if (int rc = take_slots(who, slots)) { return rc; }
+  a.slots = slots;
+  a.num_slots = a.kv.num_pages * a.kv.page_size;
+  if (int rc = require_sm100()) { return rc; }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return cache_host->bits == 8 ? launch_norm<8>(who, a, desc_host->head_dim, st)
+                               : launch_norm<16>(who, a, desc_host->head_dim, st);
+}
+
+extern "C" int vpq_kv_store_bf16(const vpq_kv_cache* cache_host, const void* k, const void* v, int64_t k_stride,
+                                 int64_t v_stride, const int64_t* slots, int64_t M, void* stream) {
+  const char* who = "kv_store";
+  clear_error();
+  QkArgs a = {};
+  if (int rc = kv_check(who, cache_host, &a.kv)) { return rc; }
+  if (M <= 0 || M > (int64_t)1 << 40) { return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < M <= 2^40 (M=%lld)", who, (long long)M); }
+  const int D = cache_host->head_dim, H = cache_host->kv_heads;
+  if (int rc = take_rows(who, "k", k, k_stride, H, D, M, &a.in_stride[1])) { return rc; }
+  if (int rc = take_rows(who, "v", v, v_stride, H, D, M, &a.in_stride[2])) { return rc; }
+  if (int rc = take_slots(who, slots)) { return rc; }
+  a.in[1] = static_cast<const uint8_t*>(k);
+  a.in[2] = static_cast<const uint8_t*>(v);
+  a.heads[1] = a.heads[2] = H;
+  a.slots = slots;
+  a.M = M;
+  a.num_slots = a.kv.num_pages * a.kv.page_size;
+  if (int rc = require_sm100()) { return rc; }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return cache_host->bits == 8 ? launch_norm<8>(who, a, D, st) : launch_norm<16>(who, a, D, st);
+}
+
+extern "C" int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, int64_t k_stride,
+                                int64_t v_stride, const int64_t* slots, int64_t M, void* stream) {
+  const char* who = "kv_load";
+  clear_error();
+  LoadArgs a = {};
+  if (int rc = kv_check(who, cache_host, &a.kv)) { return rc; }
+  if (M <= 0 || M > (int64_t)1 << 40) { return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < M <= 2^40 (M=%lld)", who, (long long)M); }
+  const int D = cache_host->head_dim, H = cache_host->kv_heads;
+  if (int rc = take_rows(who, "k_out", k_out, k_stride, H, D, M, &a.stride[0])) { return rc; }
+  if (int rc = take_rows(who, "v_out", v_out, v_stride, H, D, M, &a.stride[1])) { return rc; }
+  if (int rc = take_slots(who, slots)) { return rc; }
+  a.out[0] = static_cast<uint8_t*>(k_out);
+  a.out[1] = static_cast<uint8_t*>(v_out);
+  a.slots = slots;
+  a.M = M;
+  a.num_slots = a.kv.num_pages * a.kv.page_size;
+  if (int rc = require_sm100()) { return rc; }
+  const int64_t per_block = 256 / (D / 8);
+  const int64_t blocks = (M * 2 * H + per_block - 1) / per_block;
+  if (blocks > INT_MAX) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
+  const dim3 g((unsigned)blocks);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define VPQ_GO(DD)                                     \
+  if (cache_host->bits == 8) {                         \
+    kv_load_kernel<DD, 8><<<g, 256, 0, st>>>(a);       \
+  } else {                                             \
+    kv_load_kernel<DD, 16><<<g, 256, 0, st>>>(a);      \
+  }
+  if (D == 64) {
+    VPQ_GO(64)
+  } else if (D == 128) {
+    VPQ_GO(128)
+  } else {
+    VPQ_GO(256)
+  }
+#undef VPQ_GO
+  VPQ_LAUNCH_OK(who);
+  return VPQ_OK;
+}

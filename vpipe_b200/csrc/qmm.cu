@@ -27,6 +27,7 @@
 //
 // No TMA multicast is used anywhere; each CTA issues plain TMA loads and tile
 // reuse between CTAs comes from L2.
+#include "vpq_kv.cuh"
 #include "vpq_sm100.cuh"
 
 #include <algorithm>
@@ -1128,6 +1129,15 @@ extern "C" int vpq_device_status(void* stream, uint32_t* detail) {
     VPQ_CUDA_OK(cudaMemcpyToSymbolAsync(g_qmm_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
     VPQ_CUDA_OK(cudaStreamSynchronize(st));
     return fail(VPQ_ERR_TIMEOUT, "a bounded device-side wait gave up (site %u, role %u)", v >> 8, v & 0xffu);
+  }
+  uint32_t ik = 0, ia = 0;
+  if (int rc = kv_status_read(st, &ik)) { return rc; }
+  if (int rc = attn_status_read(st, &ia)) { return rc; }
+  if ((ik | ia) != 0) {
+    ik |= ia;
+    if (detail) { *detail = ik | 0x40000u; }
+    return fail(VPQ_ERR_INDEX, "the attention block met an index outside of its table:%s%s%s%s", (ik & kBadPage) ? " page" : "",
+                (ik & kBadSlot) ? " slot" : "", (ik & kBadPosition) ? " position" : "", (ik & kBadLength) ? " length" : "");
   }
   return VPQ_OK;
 }

@@ -1,0 +1,32 @@
+// vpq_kv.cuh -- what the kernels of the attention block share: the paged cache's view on the device,
+// its argument checks, and the report of an index outside of its table.
+#pragma once
+
+#include "vpq_common.cuh"
+
+namespace vpq {
+
+// What an index report names (vpq_device_status, detail 0x40000 | bits).
+enum : uint32_t { kBadPage = 1, kBadSlot = 2, kBadPosition = 4, kBadLength = 8 };
+
+constexpr int kKvGroup = 64;  // values that share a scale and a bias of an 8-bit cache
+
+// A vpq_kv_cache with its strides filled in.
+struct KvView {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* ks;
+  uint8_t* vs;
+  int64_t num_pages;
+  int64_t page_bytes, head_bytes, token_bytes;     // k and v
+  int64_t spage_bytes, shead_bytes, stoken_bytes;  // scale pairs
+  int page_size, kv_heads;
+};
+
+// Checks a cache descriptor and fills `view`; kv_cache.cu.
+int kv_check(const char* who, const vpq_kv_cache* c, KvView* view);
+// Reads and clears the index reports of the two sources; kv_cache.cu, paged_attn.cu.
+int kv_status_read(cudaStream_t st, uint32_t* out);
+int attn_status_read(cudaStream_t st, uint32_t* out);
+
+}  // namespace vpq

@@ -450,8 +450,222 @@ def qmm_grouped_down(codes, scales, biases, x_sorted, tile2e, sdst=None, y_rows=
     return out
 
 
+# ---- the attention block between the q | k | v and the o projection
+class _Placed:
+    """Makes `device` (and `stream`, if given) current for a call, so that what the call allocates belongs to the
+    stream that it runs on."""
+    __slots__ = ("ctx",)
+
+    def __init__(self, device, stream):
+        if stream is not None:
+            self.ctx = torch.cuda.stream(stream)
+        else:
+            self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _heads(name, t, device, shape=None):
+    """Pointer and row stride (elements) of rows [M, heads, dim]: strides beyond the row's are the caller's."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3:
+        raise ValueError(f"vpipe_b200.ops: {name} must be bfloat16 [rows, heads, head_dim]")
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"vpipe_b200.ops: {name} must live on {device} (no CPU path)")
+    m, h, d = t.shape
+    if shape is not None and (m, h, d) != shape:
+        raise ValueError(f"vpipe_b200.ops: {name} has shape {tuple(t.shape)}, {shape} is wanted")
+    sm, sh, sd = t.stride()
+    if (d > 1 and sd != 1) or (h > 1 and sh != d):
+        raise ValueError(f"vpipe_b200.ops: the heads of a row of {name} must be contiguous")
+    return t.data_ptr(), sm if m > 1 else 0
+
+
+def _index(name, t, device, dtype, shape):
+    if t.dtype != dtype or not t.is_cuda or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"vpipe_b200.ops: {name} must be a contiguous {dtype} tensor {shape} on {device}")
+    return t.data_ptr()
+
+
+class PagedKVCache:
+    """The pages of a key-value cache: k, v [pages, kv_heads, page_size, head_dim], bfloat16, or uint8 codes with
+    k_scales, v_scales bfloat16 [pages, kv_heads, page_size, head_dim / 64, 2] = (scale, bias). Any strides whose last
+    is dense (k and v alike): [pages, page_size, kv_heads, head_dim] is `.transpose(1, 2)` away. Made once; the
+    tensors are held, not copied (struct vpq_kv_cache)."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        quantised = k_scales is not None
+        want = torch.uint8 if quantised else torch.bfloat16
+        if (v_scales is not None) != quantised or k.dtype != want or v.dtype != want:
+            raise ValueError("PagedKVCache: bfloat16 pages without scales, or uint8 codes with k_scales and v_scales")
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.device != v.device or not k.is_cuda:
+            raise ValueError("PagedKVCache: k and v must be alike, [pages, kv_heads, page_size, head_dim] on a CUDA device")
+        if k.stride(3) != 1:
+            raise ValueError("PagedKVCache: the last dimension must be contiguous")
+        pages, heads, size, dim = k.shape
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.device, self.kv_heads, self.head_dim, self.page_size = k.device, heads, dim, size
+        self.num_pages, self.bits = pages, 8 if quantised else 16
+        d = self.desc = _lib.KvCache()
+        d.k, d.v = k.data_ptr(), v.data_ptr()
+        d.num_pages, d.page_size, d.kv_heads, d.head_dim, d.bits = pages, size, heads, dim, self.bits
+        d.page_stride, d.head_stride, d.token_stride = k.stride()[:3]
+        if quantised:
+            shape = (pages, heads, size, dim // 64, 2)
+            for s in (k_scales, v_scales):
+                if s.dtype != torch.bfloat16 or tuple(s.shape) != shape or s.device != k.device or s.stride() != k_scales.stride():
+                    raise ValueError(f"PagedKVCache: k_scales and v_scales must be bfloat16 {shape}, alike")
+            if k_scales.stride(4) != 1 or (dim > 64 and k_scales.stride(3) != 2):
+                raise ValueError("PagedKVCache: the scale pairs of a row must be contiguous")
+            d.k_scales, d.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
+            d.scale_page_stride, d.scale_head_stride, d.scale_token_stride = k_scales.stride()[:3]
+        self.ref = C.byref(d)
+        self._workspace_bytes = {}
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, head_dim, bits=16, device="cuda"):
+        """Pages that hold nothing yet (the tokens of a sequence are defined by its length, not by the pages)."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        if bits == 16:
+            return cls(*(torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2)))
+        if bits != 8:
+            raise ValueError("PagedKVCache.empty: bits must be 16 or 8")
+        codes = [torch.empty(shape, dtype=torch.uint8, device=device) for _ in range(2)]
+        pairs = [torch.empty(shape[:3] + (head_dim // 64, 2), dtype=torch.bfloat16, device=device) for _ in range(2)]
+        return cls(*codes, *pairs)
+
+
+def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved):
+    dev = q.device
+    d = _lib.QkDesc()
+    d.q, d.q_stride = _heads("q", q, dev)
+    d.k, d.k_stride = _heads("k", k, dev, (q.shape[0], k.shape[1], q.shape[2]))
+    d.M, d.q_heads, d.head_dim = q.shape
+    d.kv_heads, d.eps, d.interleaved = k.shape[1], eps, int(interleaved)
+    for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        if w is not None:
+            setattr(d, name, _index(name, w, dev, torch.bfloat16, (q.shape[2],)))
+    if cos_sin is not None:
+        if cos_sin.dim() != 2:
+            raise ValueError("vpipe_b200.ops: cos_sin must be float32 [rows, rot_dim]")
+        d.cos_sin = _index("cos_sin", cos_sin, dev, torch.float32, tuple(cos_sin.shape))
+        d.table_rows, d.rot_dim = cos_sin.shape
+    if positions is not None:
+        d.positions = _index("positions", positions, dev, torch.int32, (q.shape[0],))
+    return d
+
+
+def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=None, eps=1e-6, interleaved=False,
+                 q_out=None, k_out=None, stream=None):
+    """Norm of queries and keys over each head, then the position rotation, in one pass (vpq_qk_norm_rope_bf16).
+    q [M, q_heads, D], k [M, kv_heads, D] bfloat16, rows with any stride (parts of one q | k | v row are fine);
+    cos_sin float32 [rows, rot_dim] = cos | sin of the pairs' angles; token m takes row positions[m] (int32; None: row
+    m) and is left as it was if that is outside of the table. q_out / k_out may be q / k. Returns (q_out, k_out)."""
+    dev = q.device
+    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved)
+    with _Placed(dev, stream) as st:
+        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if q_out is None else q_out
+        k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if k_out is None else k_out
+        if q.shape[0] == 0:
+            return q_out, k_out
+        d.q_out, d.q_out_stride = _heads("q_out", q_out, dev, tuple(q.shape))
+        d.k_out, d.k_out_stride = _heads("k_out", k_out, dev, tuple(k.shape))
+        check(lib().vpq_qk_norm_rope_bf16(C.byref(d), st))
+    return q_out, k_out
+
+
+def qkv_norm_rope_store(q, k, v, q_norm_w, k_norm_w, cos_sin, positions, cache, slots, eps=1e-6, interleaved=False,
+                        q_out=None, stream=None):
+    """qk_norm_rope with the keys, and the values as they are, going straight into the cache: row m to slot slots[m]
+    (int64; page * page_size + place; negative: nowhere) (vpq_qkv_norm_rope_store_bf16). Returns q_out."""
+    dev = cache.device
+    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved)
+    d.v, d.v_stride = _heads("v", v, dev, tuple(k.shape))
+    s = _index("slots", slots, dev, torch.int64, (q.shape[0],))
+    with _Placed(dev, stream) as st:
+        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if q_out is None else q_out
+        if q.shape[0] == 0:
+            return q_out
+        d.q_out, d.q_out_stride = _heads("q_out", q_out, dev, tuple(q.shape))
+        check(lib().vpq_qkv_norm_rope_store_bf16(C.byref(d), cache.ref, s, st))
+    return q_out
+
+
+def kv_store(k, v, cache, slots, stream=None):
+    """Rows k, v [M, kv_heads, head_dim] into slots [M] of the cache, quantised if it is (vpq_kv_store_bf16)."""
+    dev = cache.device
+    shape = (k.shape[0], cache.kv_heads, cache.head_dim)
+    pk, sk = _heads("k", k, dev, shape)
+    pv, sv = _heads("v", v, dev, shape)
+    s = _index("slots", slots, dev, torch.int64, shape[:1])
+    if shape[0] == 0:
+        return
+    with _Placed(dev, stream) as st:
+        check(lib().vpq_kv_store_bf16(cache.ref, pk, pv, sk, sv, s, shape[0], st))
+
+
+def kv_load(cache, slots, k_out=None, v_out=None, stream=None):
+    """The values of slots [M]: (k, v) bfloat16 [M, kv_heads, head_dim], zeros for a slot outside of the cache
+    (vpq_kv_load_bf16)."""
+    dev = cache.device
+    s = _index("slots", slots, dev, torch.int64, (slots.numel(),))
+    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
+    with _Placed(dev, stream) as st:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if k_out is None else k_out
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_out is None else v_out
+        if shape[0] == 0:
+            return k_out, v_out
+        pk, sk = _heads("k_out", k_out, dev, shape)
+        pv, sv = _heads("v_out", v_out, dev, shape)
+        check(lib().vpq_kv_load_bf16(cache.ref, pk, pv, sk, sv, s, shape[0], st))
+    return k_out, v_out
+
+
+def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=None, stream=None):
+    """Attention of one new token per sequence over the cache (vpq_paged_attention_bf16): q [B, q_heads, head_dim],
+    page_table int32 [B, max_pages], seq_lens int32 [B] (the new token's own key included), window 0 = all tokens.
+    Lengths are read on the device, so a captured call serves any. The workspace is allocated per call on the stream
+    that the call runs on."""
+    dev = cache.device
+    shape = tuple(q.shape)
+    d = _lib.PagedAttentionDesc()
+    d.q, d.q_stride = _heads("q", q, dev)
+    if shape[2] != cache.head_dim:
+        raise ValueError(f"vpipe_b200.ops: q has head_dim {shape[2]}, the cache {cache.head_dim}")
+    if page_table.dim() != 2:
+        raise ValueError("vpipe_b200.ops: page_table must be int32 [batch, max_pages]")
+    d.page_table = _index("page_table", page_table, dev, torch.int32, (shape[0], page_table.shape[1]))
+    d.seq_lens = _index("seq_lens", seq_lens, dev, torch.int32, shape[:1])
+    d.batch, d.q_heads = shape[:2]
+    d.max_pages = page_table.shape[1]
+    d.window = window
+    if scale is not None:
+        if not scale > 0:
+            raise ValueError("vpipe_b200.ops: scale must be positive")
+        d.scale = scale
+    with _Placed(dev, stream) as st:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if out is None else out
+        if shape[0] == 0:
+            return out
+        d.out, d.out_stride = _heads("out", out, dev, shape)
+        ref = C.byref(d)
+        need = cache._workspace_bytes.get(shape)
+        if need is None:
+            need = cache._workspace_bytes[shape] = int(lib().vpq_paged_attention_bytes(ref, cache.ref))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        check(lib().vpq_paged_attention_bf16(ref, cache.ref, ws.data_ptr(), need, st))
+    return out
+
+
 def device_status(stream=None) -> int:
-    """Raises VpqError(TIMEOUT) if a bounded device-side wait gave up; else 0."""
+    """Raises VpqError: TIMEOUT if a bounded device-side wait gave up, INDEX if the attention block met an index
+    outside of its table; else 0."""
     detail = C.c_uint32(0)
     check(lib().vpq_device_status(_stream(stream), C.byref(detail)))
     return int(detail.value)
