@@ -26,6 +26,8 @@ struct QkArgs {
   int64_t M, table_rows, num_slots;
   int heads[3];
   int chunks;      // lane groups that share a token's heads
+  int per_block;   // of them in a block, and the blocks of a token
+  int token_blocks;
   int rot, interleaved;
   float eps, inv_d;
   KvView kv;
@@ -79,12 +81,20 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
   const float inv = __fdiv_rn(1.0f, __bfloat162float(s16));
   const bool fine = range <= 3.402823466e38f;  // false for NaN
   pair = fine ? ((uint32_t)__bfloat16_as_ushort(s16) | ((uint32_t)__bfloat16_as_ushort(b16) << 16)) : 0x7fff7fffu;
+  // Adding 2^23 rounds to an integer, ties to even, and leaves it in the low byte: b <= x and the rounded-up
+  // scale keep the quotient in [0, 255.0001], so there is nothing to clamp.
   uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = (uint32_t)__float2int_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], b), inv), 0.0f), 255.0f));
-  }
-  return make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
+  for (int i = 0; i < 8; ++i) { c[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[i], b), inv), 8388608.0f)); }
+  auto four = [](uint32_t a, uint32_t b2, uint32_t c2, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b2, 0x0040), __byte_perm(c2, d, 0x0040), 0x5410);
+  };
+  return make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
+}
+
+__device__ __forceinline__ int64_t slot_page(int64_t slot, int page_size) {
+  // a 64-bit division costs five times as much
+  return (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
 }
 
 // MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads a lane
@@ -92,12 +102,14 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
 template <int D, int MODE, int HPT>
 __global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
   constexpr int LPH = D / 8;
-  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int l = threadIdx.x % LPH;
-  const int64_t m_raw = id / A.chunks;
-  const int chunk = (int)(id - m_raw * A.chunks);
-  const bool in_range = m_raw < A.M;
-  const int64_t m = in_range ? m_raw : 0;  // lanes past the end keep their warp's shuffles company
+  const uint32_t tok = blockIdx.x / (uint32_t)A.token_blocks;
+  const int slice = (int)(blockIdx.x - tok * (uint32_t)A.token_blocks) * A.per_block + (int)threadIdx.x / LPH;
+  const int64_t m = tok;
+  const bool in_range = (int)threadIdx.x / LPH < A.per_block && slice < A.chunks;  // the rest keeps its warp's shuffles company
+  const int chunk = in_range ? slice : 0;
   const int hq = A.heads[0], hqk = hq + A.heads[1];
   const int total = hqk + (MODE ? A.heads[2] : 0);
 
@@ -116,7 +128,7 @@ __global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
     store = in_range && turn && s >= 0 && s < A.num_slots;
     if (in_range && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
     if (store) {
-      page = s / A.kv.page_size;
+      page = slot_page(s, A.kv.page_size);
       at = s - page * A.kv.page_size;
     }
   }
@@ -170,10 +182,12 @@ __global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
     unpack8(raw[i], x);
     // lanes of a warp can hold heads of different parts: the shuffles below run for all, the values of v are kept
     float ss = 0.0f;
+    if (A.norm_w[0] || A.norm_w[1]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
+      for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
 #pragma unroll
-    for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
+      for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
+    }
     if (part < 2 && h < total && A.norm_w[part]) {
       float w[8];
       unpack8(__ldg(reinterpret_cast<const uint4*>(A.norm_w[part] + d0)), w);
@@ -231,77 +245,138 @@ struct LoadArgs {
   int64_t stride[2];  // bytes
   const int64_t* slots;
   int64_t M, num_slots;
+  int chunks, per_block, token_blocks;
 };
 
-// Eight values a thread: 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out.
-template <int D, int BITS>
+// Eight values a lane and head: 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out. A lane
+// group takes HPT heads of its token, all requested before the first is used.
+template <int D, int BITS, int HPT>
 __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs A) {
   constexpr int LPH = D / 8;
-  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int l = threadIdx.x % LPH;
+  const uint32_t tok = blockIdx.x / (uint32_t)A.token_blocks;
+  const int chunk = (int)(blockIdx.x - tok * (uint32_t)A.token_blocks) * A.per_block + (int)threadIdx.x / LPH;
+  if ((int)threadIdx.x / LPH >= A.per_block || chunk >= A.chunks) { return; }
+  const int64_t m = tok;
   const int heads = 2 * A.kv.kv_heads;
-  const int64_t m = id / heads;
-  if (m >= A.M) { return; }
-  const int h = (int)(id - m * heads);
-  const bool is_v = h >= A.kv.kv_heads;
-  const int hh = is_v ? h - A.kv.kv_heads : h;
   const int64_t s = __ldg(A.slots + m);
-  uint4 y = make_uint4(0, 0, 0, 0);
   if (s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-  if (s >= 0 && s < A.num_slots) {
-    const int64_t page = s / A.kv.page_size, at = s - page * A.kv.page_size;
-    const uint8_t* p = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes;
-    if (BITS == 16) {
-      y = *reinterpret_cast<const uint4*>(p + l * 16);
-    } else {
-      const uint2 c = *reinterpret_cast<const uint2*>(p + l * 8);
-      const uint32_t pair = *reinterpret_cast<const uint32_t*>((is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes +
-                                                              hh * A.kv.shead_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4);
-      const float sc = __uint_as_float(pair << 16), b = __uint_as_float(pair & 0xffff0000u);
-      float x[8];
+  const bool live = s >= 0 && s < A.num_slots;
+  const int64_t page = live ? slot_page(s, A.kv.page_size) : 0, at = live ? s - page * A.kv.page_size : 0;
+  const int64_t off = page * A.kv.page_bytes + at * A.kv.token_bytes + l * (BITS == 16 ? 16 : 8);
+  const int64_t soff = page * A.kv.spage_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4;
+  uint4 y[HPT];
+  uint32_t pair[HPT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = dequant_f32(sc, (c.x >> (8 * i)) & 0xffu, b);
-        x[4 + i] = dequant_f32(sc, (c.y >> (8 * i)) & 0xffu, b);
+  for (int i = 0; i < HPT; ++i) {
+    const int h = chunk + i * A.chunks;
+    const bool is_v = h >= A.kv.kv_heads;
+    const int hh = is_v ? h - A.kv.kv_heads : h;
+    y[i] = make_uint4(0, 0, 0, 0);
+    pair[i] = 0;
+    if (live && h < heads) {
+      const uint8_t* p = (is_v ? A.kv.v : A.kv.k) + off + hh * A.kv.head_bytes;
+      if (BITS == 16) {
+        y[i] = *reinterpret_cast<const uint4*>(p);
+      } else {
+        const uint2 c = *reinterpret_cast<const uint2*>(p);
+        y[i].x = c.x, y[i].y = c.y;
+        pair[i] = *reinterpret_cast<const uint32_t*>((is_v ? A.kv.vs : A.kv.ks) + soff + hh * A.kv.shead_bytes);
       }
-      y = pack8(x);
     }
   }
-  *reinterpret_cast<uint4*>(A.out[is_v] + m * A.stride[is_v] + (int64_t)hh * (D * 2) + l * 16) = y;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int h = chunk + i * A.chunks;
+    if (h >= heads) { break; }
+    const bool is_v = h >= A.kv.kv_heads;
+    const int hh = is_v ? h - A.kv.kv_heads : h;
+    if (BITS == 8) {
+      const float sc = __uint_as_float(pair[i] << 16), b = __uint_as_float(pair[i] & 0xffff0000u);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = dequant_f32(sc, (y[i].x >> (8 * e)) & 0xffu, b);
+        x[4 + e] = dequant_f32(sc, (y[i].y >> (8 * e)) & 0xffu, b);
+      }
+      y[i] = pack8(x);
+    }
+    *reinterpret_cast<uint4*>(A.out[is_v] + m * A.stride[is_v] + (int64_t)hh * (D * 2) + l * 16) = y[i];
+  }
 }
 
 bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
 
+// How a token's heads are dealt: `chunks` lane groups take HPT heads each, evenly over blocks of at most
+// 256 threads that belong to one token (no division by the thread, and a token's table row is fetched by few
+// blocks). One head per lane group while the launch is too small to fill the machine (a decode step lives by
+// latency); four once there are waves of them.
+struct Deal {
+  bool wide;
+  int chunks, per_block, token_blocks;
+  dim3 grid, block;
+};
+int deal(const char* who, int64_t M, int heads, int D, Deal* d) {
+  const int groups = 256 / (D / 8);
+  d->wide = M * heads > (int64_t)num_sms() * 8 * groups * 2;
+  const int hpt = d->wide ? 4 : 1;
+  d->chunks = (heads + hpt - 1) / hpt;
+  d->token_blocks = (d->chunks + groups - 1) / groups;
+  d->per_block = (d->chunks + d->token_blocks - 1) / d->token_blocks;
+  if (M > INT_MAX / d->token_blocks) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
+  d->grid = dim3((unsigned)(M * d->token_blocks));
+  d->block = dim3((unsigned)((d->per_block * (D / 8) + 31) & ~31));
+  return VPQ_OK;
+}
+
+template <typename K, typename A>
+int launch_with_pdl(K kern, const Deal& d, cudaStream_t st, const A& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = d.grid;
+  cfg.blockDim = d.block;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VPQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a));
+  return VPQ_OK;
+}
+
 template <int MODE>
 int launch_norm(const char* who, const QkArgs& a0, int D, cudaStream_t st) {
   QkArgs a = a0;
-  const int total = a.heads[0] + a.heads[1] + (MODE ? a.heads[2] : 0);
-  const int64_t per_block = 256 / (D / 8);
-  // One head per lane group while the launch is too small to fill the machine (a decode step lives by
-  // latency); four once there is a wave of them, so the table's row and the norm weights are fetched
-  // once per four heads and four loads are in flight.
-  const bool wide = a.M * total > (int64_t)num_sms() * 8 * per_block * 4;
-  const int hpt = wide ? 4 : 1;
-  a.chunks = (total + hpt - 1) / hpt;
-  const int64_t blocks = (a.M * a.chunks + per_block - 1) / per_block;
-  if (blocks > INT_MAX) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)a.M); }
-  const dim3 g((unsigned)blocks);
-#define VPQ_GO(DD)                                                   \
-  if (wide) {                                                        \
-    norm_rope_store_kernel<DD, MODE, 4><<<g, 256, 0, st>>>(a);       \
-  } else {                                                           \
-    norm_rope_store_kernel<DD, MODE, 1><<<g, 256, 0, st>>>(a);       \
-  }
+  Deal d;
+  if (int rc = deal(who, a.M, a.heads[0] + a.heads[1] + (MODE ? a.heads[2] : 0), D, &d)) { return rc; }
+  a.chunks = d.chunks, a.per_block = d.per_block, a.token_blocks = d.token_blocks;
   if (D == 64) {
-    VPQ_GO(64)
-  } else if (D == 128) {
-    VPQ_GO(128)
-  } else {
-    VPQ_GO(256)
+    return d.wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, d, st, a)
+                  : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, d, st, a);
   }
-#undef VPQ_GO
-  VPQ_LAUNCH_OK(who);
-  return VPQ_OK;
+  if (D == 128) {
+    return d.wide ? launch_with_pdl(norm_rope_store_kernel<128, MODE, 4>, d, st, a)
+                  : launch_with_pdl(norm_rope_store_kernel<128, MODE, 1>, d, st, a);
+  }
+  return d.wide ? launch_with_pdl(norm_rope_store_kernel<256, MODE, 4>, d, st, a)
+                : launch_with_pdl(norm_rope_store_kernel<256, MODE, 1>, d, st, a);
+}
+
+template <int BITS>
+int launch_load(const char* who, const LoadArgs& a0, int D, cudaStream_t st) {
+  LoadArgs a = a0;
+  Deal d;
+  if (int rc = deal(who, a.M, 2 * a.kv.kv_heads, D, &d)) { return rc; }
+  a.chunks = d.chunks, a.per_block = d.per_block, a.token_blocks = d.token_blocks;
+  if (D == 64) {
+    return d.wide ? launch_with_pdl(kv_load_kernel<64, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<64, BITS, 1>, d, st, a);
+  }
+  if (D == 128) {
+    return d.wide ? launch_with_pdl(kv_load_kernel<128, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<128, BITS, 1>, d, st, a);
+  }
+  return d.wide ? launch_with_pdl(kv_load_kernel<256, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<256, BITS, 1>, d, st, a);
 }
 
 bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
@@ -542,25 +617,6 @@ extern "C" int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, voi
   a.M = M;
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
-  const int64_t per_block = 256 / (D / 8);
-  const int64_t blocks = (M * 2 * H + per_block - 1) / per_block;
-  if (blocks > INT_MAX) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
-  const dim3 g((unsigned)blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define VPQ_GO(DD)                                     \
-  if (cache_host->bits == 8) {                         \
-    kv_load_kernel<DD, 8><<<g, 256, 0, st>>>(a);       \
-  } else {                                             \
-    kv_load_kernel<DD, 16><<<g, 256, 0, st>>>(a);      \
-  }
-  if (D == 64) {
-    VPQ_GO(64)
-  } else if (D == 128) {
-    VPQ_GO(128)
-  } else {
-    VPQ_GO(256)
-  }
-#undef VPQ_GO
-  VPQ_LAUNCH_OK(who);
-  return VPQ_OK;
+  return cache_host->bits == 8 ? launch_load<8>(who, a, D, st) : launch_load<16>(who, a, D, st);
 }

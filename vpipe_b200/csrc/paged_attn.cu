@@ -5,7 +5,7 @@
 // Bound: HBM. Every key and value is read once and used by the q_heads / kv_heads queries that share
 // it; per 16 tokens of one head that is 8 KB (bf16, head_dim 128) against 16 small matrix products.
 //
-// Work split. The unit is 16 tokens of one (sequence, key head). All units of a call, in the order
+// Work split. The unit is 16 or 32 tokens of one (sequence, key head). All units of a call, in the order
 // (sequence, head, tokens), form one line that is cut into equal runs, one per CTA, and a CTA's run into one per
 // warp: no SM waits for a long sequence, whatever the lengths, and the lengths are read on the device, so a
 // captured graph serves any of them. Each warp streams its run through its own ring in shared memory
@@ -18,13 +18,15 @@
 // and need twice the accumulators). S^T = K Q^T comes out with tokens in rows; P enters the second product,
 // O^T = V^T P^T, as its B operand, which wants the 8 x 8 blocks transposed: one movmatrix each.
 //
-// 8-bit caches multiply the codes, not the values: c - 128 is exact in fp16, so with k = s c + b
-//   q . k = sum_g s_g (q . (c - 128))_g + (b_g + 128 s_g) sum_g q            (g: groups of 64)
-//   o     = sum_t (p_t s_tg) (c - 128) + sum_t p_t (b_tg + 128 s_tg)
-// and scales and biases act on 16 x 8 scores instead of 16 x head_dim values. Centred codes matter: with
-// 0..255 the rounding of p s would be amplified by the codes' mean. q is scaled by a power of two per head to
-// fill fp16's range (exact up to 2^-39 of the head's largest value); p s is taken relative to a running
-// power of two above every scale, times 2^15, which keeps its rounding at 2^-11 relative down to 2^-29.
+// 8-bit caches multiply the codes, not the values. A byte c with a zero byte above it IS the fp16 number
+// c 2^-24 (a subnormal), so a pair of operands costs one byte permute. With k = s c + b, g: groups of 64,
+//   q . k = sum_g s_g (q . c)_g + b_g sum_g q
+//   o     = sum_t p'_tg c - 128 sum_t p'_tg + sum_t p_t (b_tg + 128 s_tg),   p'_tg = p_t s_tg rounded to fp16
+// and scales and biases act on 16 x 8 scores instead of 16 x head_dim values. The middle term of o (one
+// product with a constant operand per group) takes the codes' mean out of the rounding of p', which it
+// would amplify by about three. q is scaled by a power of two per head to fill fp16's range (exact up to 2^-39 of
+// the head's largest value); p s is taken relative to a running power of two above every scale, times 2^15,
+// which keeps its rounding at 2^-11 relative down to 2^-29.
 // In a bf16 cache p is rounded to bf16 (2^-8) and the sum of weights adds the rounded p, so the
 // weights still sum to one.
 #include "vpq_kv.cuh"
@@ -38,8 +40,13 @@ __device__ uint32_t g_attn_status = 0;
 
 namespace {
 
-constexpr int kUnit = 16;    // tokens of a unit
 constexpr float kNegInf = -__builtin_huge_valf();
+
+// What the joining kernel has to know of a CTA: the (sequence, head) that begins in its run and goes on in
+// the next CTA's, where its partial result is (0: the run's first, 1), and the last CTA that has a part.
+struct CtaHead {
+  int b, h, slot, last;  // last -1: none
+};
 
 struct AttnArgs {
   KvView kv;
@@ -49,16 +56,17 @@ struct AttnArgs {
   const int32_t* page_table;
   const int32_t* seq_lens;
   int64_t table_stride;
-  int64_t* prefix;   // workspace: units (of one head) before each sequence, then units per CTA
-  float* ml;         // [CTA][2][heads per column block][2]: maximum and sum of a partial result
-  float* part;       // [CTA][2][heads per column block][D]
+  CtaHead* heads;    // workspace: one per CTA
+  float* ml;         // [CTA][2][cols][2]: maximum and sum of a partial result
+  float* part;       // [CTA][2][cols][D]
+  float* scratch;    // [CTA][warp][cols][D]: a warp's first partial result, if another run follows it
   int batch, max_pages, window;
   int group;         // query heads of a key head
   int cols;          // query heads a unit serves (a column block): min(group, 8 NT)
   int blocks;        // column blocks of a key head
   int hk;            // kv_heads * blocks
   float scale_log2;
-  int stage_bytes, ring_bytes, entry_bytes;  // shared memory: a stage, a warp's ring, a partial result
+  int stage_bytes, ring_bytes;  // shared memory: a stage, a warp's ring
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -131,13 +139,33 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-// Bytes 0, 1 of w (HI: 2, 3) as fp16 pairs of c - 128: 0x6400 | c is 1024 + c exactly.
+// Bytes 0, 1 of w (HI: 2, 3), each with a zero byte above: the fp16 numbers c 2^-24.
 template <bool HI>
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));  // 1152
-  return r;
+__device__ __forceinline__ uint32_t codes(uint32_t w) {
+  return __byte_perm(w, 0u, HI ? 0x4342 : 0x4140);
+}
+// Quotients of numbers that nearly always fit 32 bits (a 64-bit division costs five times as much).
+__device__ __forceinline__ int64_t div_u(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The scale pairs of a row.
+template <int G>
+__device__ __forceinline__ void lds_pairs(uint32_t (&p)[G], uint32_t a) {
+  if (G == 1) {
+    p[0] = lds32(a);
+  } else if (G == 2) {
+    const uint2 w = lds64(a);
+    p[0] = w.x, p[G > 1 ? 1 : 0] = w.y;
+  } else {
+    const uint4 w = lds128(a);
+    p[0] = w.x, p[G > 1 ? 1 : 0] = w.y, p[G > 2 ? 2 : 0] = w.z, p[G > 3 ? 3 : 0] = w.w;
+  }
+}
+// The factor that takes a partial result (maximum m, sum l) to the joint maximum; one without a live token
+// counts nothing, unless it holds a NaN.
+__device__ __forceinline__ float weight_of(float m, float l, float joint) {
+  return m == kNegInf ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - joint);
 }
 
 // Tokens of sequence b that count: [start, len), len cut to what the table can name.
@@ -148,7 +176,10 @@ __device__ __forceinline__ void token_range(const AttnArgs& A, int b, int& start
   len = n > 0 ? n : 0;
   start = (A.window > 0 && len > A.window) ? len - A.window : 0;
 }
-__device__ __forceinline__ int units_of(int start, int len) { return len > start ? (len + kUnit - 1) / kUnit - start / kUnit : 0; }
+template <int U>
+__device__ __forceinline__ int units_of(int start, int len) {
+  return len > start ? (len + U - 1) / U - start / U : 0;
+}
 
 // Where 16-byte chunk c of row `row` lies in a K or V tile. 16 bits: the eight rows that an ldmatrix
 // reads fall into eight bank groups. 8 bits: see the loads in the loop.
@@ -164,26 +195,28 @@ __device__ __forceinline__ int swz_v(int row, int c) {
 // What a unit in flight is: written by lane 0 with its copies, read when its turn comes.
 struct alignas(16) UnitMeta {
   int b, h;       // sequence; key head * blocks + column block
-  int lo_hi;      // live rows [lo, hi) of the 16
-  int flags;
+  int bits;       // live rows [lo, hi): lo | hi << 8, flags << 16
+  int rest;       // units of this (sequence, head) behind this one
 };
-enum : int { kFirst = 1, kLast = 2, kSegBegin = 4, kSegEnd = 8 };
+enum : int { kFirst = 1 << 16, kLast = 2 << 16, kSegBegin = 4 << 16 };
 
-// A partial result of a warp, in shared memory: header here, D values of each column in the entry.
+// A partial result of a warp: its numbers are at `data` (the warp's ring, or its scratch in the workspace).
 struct EntryHead {
-  int seg;      // b * hk + h, -1: none
-  int flags;    // kSegBegin, kSegEnd
-  int b, h;
+  const float* data;
+  int b, h;     // b -1: none
+  int begins;   // from the first token on
+  int rest;     // as UnitMeta, of its last unit
   float m[16], l[16];
 };
 
-template <int D, int BITS, int NT, int kWarps, int STAGES>
+template <int D, int BITS, int NT, int TM, int kWarps, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnArgs A) {
+  constexpr int kUnit = 16 * TM;
   constexpr int kRow = D * BITS / 8;
   constexpr int kTile = kUnit * kRow;
-  constexpr int kPair = BITS == 8 ? D / kKvGroup * 4 : 0;  // scale pairs of a row
-  constexpr int kPairs = kUnit * kPair;
   constexpr int G = D / kKvGroup;
+  constexpr int kPair = BITS == 8 ? G * 4 : 0;  // scale pairs of a row
+  constexpr int kPairs = kUnit * kPair;
   constexpr int MT = D / 16;  // 16-row blocks of O^T
 
   extern __shared__ __align__(128) uint8_t smem[];
@@ -205,7 +238,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   for (int b = b_lo; b < b_hi; ++b) {
     int s, n;
     token_range(A, b, s, n);
-    mine += units_of(s, n);
+    mine += units_of<kUnit>(s, n);
+    if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > n) { atomicOr(&g_attn_status, kBadLength); }
   }
   int64_t incl = mine;
 #pragma unroll
@@ -214,7 +248,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     if (lane >= d) { incl += o; }
   }
   if (lane == 31) { s_wsum[warp] = incl; }
-  if (tid < kWarps * 2) { s_entry[tid].seg = -1; }
+  if (tid < kWarps * 2) { s_entry[tid].b = -1; }
+  if (tid == 0) { A.heads[blockIdx.x].last = -1; }
   __syncthreads();
   int64_t base = 0, total = 0;
 #pragma unroll
@@ -222,39 +257,41 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     if (w < warp) { base += s_wsum[w]; }
     total += s_wsum[w];
   }
-  const int64_t excl = base + incl - mine;
-  s_excl[tid] = excl;
-  const int64_t units = total * A.hk;
-  int64_t per_cta = (units + gridDim.x - 1) / gridDim.x;
-  per_cta = per_cta > kWarps ? per_cta : kWarps;
-  if (blockIdx.x == 0) {  // what the joining kernel needs of this
-    int64_t at = excl;
-    for (int b = b_lo; b < b_hi; ++b) {
-      int s, n;
-      token_range(A, b, s, n);
-      A.prefix[b] = at;
-      at += units_of(s, n);
-      if (__ldg(A.seq_lens + b) > n) { atomicOr(&g_attn_status, kBadLength); }
-    }
-    if (tid == 0) {
-      A.prefix[A.batch] = total;
-      A.prefix[A.batch + 1] = per_cta;
-    }
-  }
+  s_excl[tid] = base + incl - mine;
   __syncthreads();
+  const int64_t units = total * A.hk;
+  int64_t per_cta = div_u(units + gridDim.x - 1, gridDim.x);
+  per_cta = per_cta > kWarps ? per_cta : kWarps;
   const int64_t cta0 = (int64_t)blockIdx.x * per_cta;
   if (cta0 >= units) { return; }  // the whole CTA
   const int64_t cta1 = cta0 + per_cta < units ? cta0 + per_cta : units;
   const int64_t per_warp = (cta1 - cta0 + kWarps - 1) / kWarps;
   const int64_t u0 = cta0 + warp * per_warp;
-  int64_t u1 = u0 + per_warp < cta1 ? u0 + per_warp : cta1;
+  const int64_t u1 = u0 + per_warp < cta1 ? u0 + per_warp : cta1;
   int left = u0 < u1 ? (int)(u1 - u0) : 0;  // units this warp has yet to request
   int todo = left;                          // and to compute
 
   // ---- the loader's place in the line
-  int lb = 0, lh = 0, ltile = 0, ltile0 = 0, ltile_end = 0, lstart = 0, llen = 0;
+  int lb = 0, lh = 0, lkv = 0, lblk = 0, ltile = 0, ltile0 = 0, ltile_end = 0, lstart = 0, llen = 0;
   int pg = 0, off = 0;     // page-table column and token offset in the page
   bool fresh = true;       // the next unit begins a (sequence, head) for this warp
+  int page[TM];            // page numbers of the next unit, fetched one unit ahead; -1: none
+  auto enter = [&]() {     // to the first token of unit ltile
+    const int64_t at = (int64_t)ltile * kUnit;
+    pg = (int)((uint32_t)at / (uint32_t)A.kv.page_size);
+    off = (int)((uint32_t)at % (uint32_t)A.kv.page_size);
+  };
+  auto fetch_pages = [&]() {
+    int c = pg, o = off;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int first = ltile * kUnit + 16 * i;
+      // entries of pages without a live token are not read
+      page[i] = (first < llen && first + 16 > lstart) ? __ldg(A.page_table + (int64_t)lb * A.table_stride + c) : -1;
+      o += 16;
+      if (o == A.kv.page_size) { o = 0, ++c; }
+    }
+  };
   if (left > 0) {
     int lo = 0, hi = kWarps * 32 - 1;
     while (lo < hi) {  // the last thread whose sequences begin at or before u0
@@ -268,84 +305,111 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     int64_t at = s_excl[lo];
     for (lb = lo * cpt;; ++lb) {
       token_range(A, lb, lstart, llen);
-      const int n = units_of(lstart, llen);
+      const int n = units_of<kUnit>(lstart, llen);
       if ((at + n) * A.hk > u0) { break; }
       at += n;
     }
     ltile0 = lstart / kUnit;
-    ltile_end = ltile0 + units_of(lstart, llen);
+    ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
     const int64_t in_seq = u0 - at * A.hk;
-    lh = (int)(in_seq / (ltile_end - ltile0));
-    ltile = ltile0 + (int)(in_seq % (ltile_end - ltile0));
-    pg = (int)((int64_t)ltile * kUnit / A.kv.page_size);
-    off = (int)((int64_t)ltile * kUnit - (int64_t)pg * A.kv.page_size);
+    lh = (int)div_u(in_seq, ltile_end - ltile0);
+    ltile = ltile0 + (int)(in_seq - (int64_t)lh * (ltile_end - ltile0));
+    lkv = lh / A.blocks;
+    lblk = lh - lkv * A.blocks;
+    enter();
+    fetch_pages();
   }
 
   uint8_t* ring = smem + warp * A.ring_bytes;
   const uint32_t ring_s = smem_u32(ring);
-  uint8_t* entry0 = smem + kWarps * A.ring_bytes + warp * A.entry_bytes;
+  constexpr int CH = kRow / 16;                      // 16-byte chunks of a row
+  constexpr int kRowsPer = CH < 32 ? 32 / CH : 1;    // rows that one round of the warp's copies covers
+  constexpr int kRounds = 16 * CH / 32;
+  const int crow = CH < 32 ? lane / CH : 0, cch = lane % CH;
+  const int64_t lane_off = crow * A.kv.token_bytes + cch * 16;
 
   // Requests the next unit into stage `st`; commits a group in any case.
   auto request = [&](int st) {
     if (left > 0) {
-      const int page = __ldg(A.page_table + (int64_t)lb * A.table_stride + pg);
-      const bool ok = (uint32_t)page < (uint32_t)A.kv.num_pages;
-      if (!ok && lane == 0) { atomicOr(&g_attn_status, kBadPage); }
       int lo = lstart - ltile * kUnit;
       lo = lo > 0 ? lo : 0;
       int hi = llen - ltile * kUnit;
       hi = hi < kUnit ? hi : kUnit;
-      if (!ok) { lo = hi = 0; }
-      const int64_t pp = ok ? page : 0;
-      const int kvh = lh / A.blocks;
-      const int64_t o = pp * A.kv.page_bytes + kvh * A.kv.head_bytes + (int64_t)off * A.kv.token_bytes;
       const uint32_t dst = ring_s + st * A.stage_bytes;
-      constexpr int CH = kRow / 16;
+      int bad = 0;
 #pragma unroll
-      for (int j = 0; j < CH / 2; ++j) {
-        const int id = lane + 32 * j, row = id / CH, c = id % CH;
-        const bool live = row >= lo && row < hi;  // dead rows become zeros: whatever they hold, 0 p adds 0
-        const int64_t so = o + row * A.kv.token_bytes + c * 16;
-        cp_async16(dst + row * kRow + swz_k<D, BITS>(row, c) * 16, A.kv.k + so, live);
-        cp_async16(dst + kTile + row * kRow + swz_v<D, BITS>(row, c) * 16, A.kv.v + so, live);
+      for (int i = 0; i < TM; ++i) {
+        const bool ok = (uint32_t)page[i] < (uint32_t)A.kv.num_pages;
+        // A page without live tokens, or none: rows of zeros. Dead rows of a page become zeros too: whatever
+        // they hold, their weight 0 has to add 0.
+        const int rlo = ok ? lo - 16 * i : 16, rhi = ok ? hi - 16 * i : 0;
+        if (!ok && lo < 16 * i + 16 && hi > 16 * i) { bad |= 1 << i; }
+        const int64_t pp = ok ? page[i] : 0;
+        const int64_t o = pp * A.kv.page_bytes + lkv * A.kv.head_bytes + (int64_t)off * A.kv.token_bytes + lane_off;
+        const uint8_t* kp = A.kv.k + o;
+        const uint8_t* vp = A.kv.v + o;
+#pragma unroll
+        for (int j = 0; j < kRounds; ++j) {
+          const int row = CH <= 32 ? crow + j * kRowsPer : 0;
+          const bool live = row >= rlo && row < rhi;
+          const int64_t so = (int64_t)(j * kRowsPer) * A.kv.token_bytes;
+          cp_async16(dst + (16 * i + row) * kRow + swz_k<D, BITS>(row, cch) * 16, kp + so, live);
+          cp_async16(dst + kTile + (16 * i + row) * kRow + swz_v<D, BITS>(row, cch) * 16, vp + so, live);
+        }
+        if (BITS == 8) {
+          const int row = lane & 15;
+          const bool live = row >= rlo && row < rhi;
+          const uint8_t* sp = (lane < 16 ? A.kv.ks : A.kv.vs) + pp * A.kv.spage_bytes + lkv * A.kv.shead_bytes +
+                              (int64_t)(off + row) * A.kv.stoken_bytes;
+          cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + (16 * i + row) * kPair, sp, live);
+        }
+        off += 16;
+        if (off == A.kv.page_size) { off = 0, ++pg; }
       }
-      if (BITS == 8) {
-        const int row = lane & 15;
-        const bool live = row >= lo && row < hi;
-        const uint8_t* sp = (lane < 16 ? A.kv.ks : A.kv.vs) + pp * A.kv.spage_bytes + kvh * A.kv.shead_bytes +
-                            (int64_t)(off + row) * A.kv.stoken_bytes;
-        cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + row * kPair, sp, live);
+      if (bad) {  // a page outside the cache holds no tokens: the live rows shrink to what is left
+        if (lane == 0) { atomicOr(&g_attn_status, kBadPage); }
+        if (TM == 1 || bad == 3) {
+          lo = hi = 0;
+        } else if (bad == 1) {
+          lo = min(max(lo, 16), hi);
+        } else {
+          hi = max(min(hi, 16), lo);
+        }
       }
       if (fresh) {
-        const int h0 = kvh * A.group + (lh % A.blocks) * A.cols;
-        const int n = min(A.cols, A.group - (lh % A.blocks) * A.cols);
+        const int h0 = lkv * A.group + lblk * A.cols;
+        const int n = min(A.cols, A.group - lblk * A.cols);
         const uint8_t* qp = A.q + (int64_t)lb * A.q_stride + (int64_t)h0 * (D * 2);
         for (int i = lane; i < n * (D / 8); i += 32) { cp_async16(dst + 2 * kTile + 2 * kPairs + i * 16, qp + i * 16, true); }
       }
-      const bool last = left == 1 || ltile + 1 == ltile_end;
+      const int rest = ltile_end - 1 - ltile;
       if (lane == 0) {
-        s_meta[warp][st] = {lb, lh, lo | (hi << 8),
-                            (fresh ? kFirst : 0) | (last ? kLast : 0) | (ltile == ltile0 ? kSegBegin : 0) |
-                                (ltile + 1 == ltile_end ? kSegEnd : 0)};
+        s_meta[warp][st] = {lb, lh,
+                            lo | (hi << 8) | (fresh ? kFirst : 0) | ((left == 1 || rest == 0) ? kLast : 0) |
+                                (ltile == ltile0 ? kSegBegin : 0),
+                            rest};
       }
       --left;
       fresh = false;
-      off += kUnit;
-      if (off == A.kv.page_size) { off = 0, ++pg; }
-      if (++ltile == ltile_end && left > 0) {
-        fresh = true;
-        if (++lh == A.hk) {
-          lh = 0;
-          do {
-            ++lb;
-            token_range(A, lb, lstart, llen);
-          } while (units_of(lstart, llen) == 0);
-          ltile0 = lstart / kUnit;
-          ltile_end = ltile0 + units_of(lstart, llen);
+      ++ltile;
+      if (left > 0) {
+        if (rest == 0) {
+          fresh = true;
+          ++lh;
+          if (++lblk == A.blocks) { lblk = 0, ++lkv; }
+          if (lh == A.hk) {
+            lh = lkv = lblk = 0;
+            do {
+              ++lb;
+              token_range(A, lb, lstart, llen);
+            } while (units_of<kUnit>(lstart, llen) == 0);
+            ltile0 = lstart / kUnit;
+            ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
+          }
+          ltile = ltile0;
+          enter();
         }
-        ltile = ltile0;
-        pg = (int)((int64_t)ltile * kUnit / A.kv.page_size);
-        off = (int)((int64_t)ltile * kUnit - (int64_t)pg * A.kv.page_size);
+        fetch_pages();
       }
     }
     cp_commit();
@@ -353,7 +417,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 
   float o_acc[NT][MT][4];
   float m_run[NT][2], l_run[NT][2];
-  float o_bias[NT][G][2], q_sum[NT][G][2], q_mul[NT][2];  // 8 bits
+  float o_mean[NT][G][4], o_bias[NT][G][2], q_sum[NT][G][2], q_mul[NT][2];  // 8 bits
   uint32_t qf[NT][D / 16][2];
   int sigma = -100;      // 8 bits: exponent of the power of two above every value scale so far
   bool run_begins = false, first_run = true;
@@ -368,10 +432,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     request(st == 0 ? STAGES - 1 : st - 1);
     const uint32_t kt = ring_s + st * A.stage_bytes, vt = kt + kTile, ksc = vt + kTile, vsc = ksc + kPairs,
                    qt = vsc + kPairs;
-    const int ncol = min(A.cols, A.group - (U.h % A.blocks) * A.cols);
 
-    if (U.flags & kFirst) {
-      run_begins = (U.flags & kSegBegin) != 0;
+    if (U.bits & kFirst) {
+      const int blk = U.h % A.blocks;
+      const int ncol = min(A.cols, A.group - blk * A.cols);
+      run_begins = (U.bits & kSegBegin) != 0;
       sigma = -100;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -421,87 +486,111 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {  // the same for the columns of this lane's scores
-            q_mul[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+            q_mul[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * (A.scale_log2 * 16777216.0f);  // codes' 2^24
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              q_sum[n][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * t + c) * 4);
-              o_bias[n][g][c] = 0.0f;
+              q_sum[n][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * t + c) * 4) * A.scale_log2;
+              o_bias[n][g][c] = o_mean[n][g][c] = o_mean[n][g][2 + c] = 0.0f;
             }
           }
         }
       }
     }
 
-    // ---- scores: rows r, r + 8 of the unit, columns 2t, 2t + 1
-    float s[NT][4];
+    // ---- scores times log2(e) scale: rows 16 i + r, 16 i + r + 8 of the unit, columns 2t, 2t + 1
+    float s[TM][NT][4];
     if (BITS == 16) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f; }
       const int row = (lane & 7) + (lane & 8), ch = lane >> 4;
 #pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f; }
+      }
+#pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        uint32_t a[4];
-        ldsm4(a, kt + row * kRow + swz_k<D, BITS>(row, 2 * k + ch) * 16);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) { mma<false>(s[n], a, qf[n][k][0], qf[n][k][1]); }
-      }
+        for (int i = 0; i < TM; ++i) {
+          uint32_t a[4];
+          ldsm4(a, kt + (16 * i + row) * kRow + swz_k<D, BITS>(row, 2 * k + ch) * 16);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { s[n][i] *= A.scale_log2; }
-      }
-    } else {
-      float bias[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { s[n][i] = bias[n][i] = 0.0f; }
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        // a lane's 16 codes feed four k steps: the k order is permuted the same way in q
-        const uint4 x = lds128(kt + r * kRow + swz_k<D, BITS>(r, 4 * g + t) * 16);
-        const uint4 y = lds128(kt + (r + 8) * kRow + swz_k<D, BITS>(r + 8, 4 * g + t) * 16);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-        float c[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) { c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f; }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t a[4] = {centred<false>(xs[u]), centred<false>(ys[u]), centred<true>(xs[u]), centred<true>(ys[u])};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) { mma<true>(c[n], a, qf[n][g * 4 + u][0], qf[n][g * 4 + u][1]); }
+          for (int n = 0; n < NT; ++n) { mma<false>(s[i][n], a, qf[n][k][0], qf[n][k][1]); }
         }
-        const uint32_t p0 = lds32(ksc + r * kPair + g * 4), p1 = lds32(ksc + (r + 8) * kPair + g * 4);
-        const float s0 = lo16(p0), s1 = lo16(p1);
-        const float b0 = __fmaf_rn(128.0f, s0, hi16(p0)), b1 = __fmaf_rn(128.0f, s1, hi16(p1));
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[n][i] = __fmaf_rn(c[n][i], i < 2 ? s0 : s1, s[n][i]);
-            bias[n][i] = __fmaf_rn(i < 2 ? b0 : b1, q_sum[n][g][i & 1], bias[n][i]);
+          for (int e = 0; e < 4; ++e) { s[i][n][e] *= A.scale_log2; }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        uint32_t p0[G], p1[G];
+        lds_pairs<G>(p0, ksc + (16 * i + r) * kPair);
+        lds_pairs<G>(p1, ksc + (16 * i + r + 8) * kPair);
+        float bias[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { s[i][n][e] = bias[n][e] = 0.0f; }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          // a lane's 16 codes feed four k steps: the k order is permuted the same way in q
+          const uint4 x = lds128(kt + (16 * i + r) * kRow + swz_k<D, BITS>(r, 4 * g + t) * 16);
+          const uint4 y = lds128(kt + (16 * i + r + 8) * kRow + swz_k<D, BITS>(r + 8, 4 * g + t) * 16);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          float c[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) { c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f; }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t a[4] = {codes<false>(xs[u]), codes<false>(ys[u]), codes<true>(xs[u]), codes<true>(ys[u])};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { mma<true>(c[n], a, qf[n][g * 4 + u][0], qf[n][g * 4 + u][1]); }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t p = e < 2 ? p0[g] : p1[g];
+              s[i][n][e] = __fmaf_rn(c[n][e], lo16(p), s[i][n][e]);
+              bias[n][e] = __fmaf_rn(hi16(p), q_sum[n][g][e & 1], bias[n][e]);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { s[i][n][e] = __fmaf_rn(s[i][n][e], q_mul[n][e & 1], bias[n][e]); }
+        }
+      }
+    }
+    const int lo = U.bits & 0xff, hi = (U.bits >> 8) & 0xff;
+    if (lo > 0 || hi < kUnit) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = 16 * i + r + (e < 2 ? 0 : 8);
+            s[i][n][e] = row >= lo && row < hi ? s[i][n][e] : kNegInf;
           }
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { s[n][i] = __fmaf_rn(s[n][i], q_mul[n][i & 1], bias[n][i]) * A.scale_log2; }
-      }
     }
-    const int lo = U.lo_hi & 0xff, hi = U.lo_hi >> 8;
-    const bool live0 = r >= lo && r < hi, live1 = r + 8 >= lo && r + 8 < hi;
-    float p[NT][4];
     bool grows = false;
     float m_new[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { s[n][i] = (i < 2 ? live0 : live1) ? s[n][i] : kNegInf; }
-#pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float x = fmaxf(s[n][c], s[n][2 + c]);
+        float x = fmaxf(s[0][n][c], s[0][n][2 + c]);
+#pragma unroll
+        for (int i = 1; i < TM; ++i) { x = fmaxf(x, fmaxf(s[i][n][c], s[i][n][2 + c])); }
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -509,20 +598,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         grows |= m_new[n][c] > m_run[n][c];
       }
     }
-    // 8 bits: this lane's value scales and centred biases
-    float vs[2][G], vb[2][G], rescale = 1.0f, up = 1.0f;
+    // 8 bits: this lane's value pairs, and the power of two above their scales
+    uint32_t vp[TM][2][G];
+    float rescale = 1.0f, up = 1.0f;
     if (BITS == 8) {
       uint32_t top = 0;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint32_t p0 = lds32(vsc + r * kPair + g * 4), p1 = lds32(vsc + (r + 8) * kPair + g * 4);
-        vs[0][g] = lo16(p0), vs[1][g] = lo16(p1);
-        vb[0][g] = __fmaf_rn(128.0f, vs[0][g], hi16(p0));
-        vb[1][g] = __fmaf_rn(128.0f, vs[1][g], hi16(p1));
-        top = max(top, max((p0 << 16) & 0x7fffffffu, (p1 << 16) & 0x7fffffffu));
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          lds_pairs<G>(vp[i][h], vsc + (16 * i + r + 8 * h) * kPair);
+#pragma unroll
+          for (int g = 0; g < G; ++g) { top = max(top, vp[i][h][g] & 0x7fffu); }
+        }
       }
       top = __reduce_max_sync(0xffffffffu, top);
-      const int e = (int)(top >> 23) - 126;  // top < 2^e
+      const int e = (int)(top >> 7) - 126;  // every scale is below 2^e
       if (e > sigma) {
         grows = true;
         rescale = ex2((float)(sigma - e));
@@ -546,7 +637,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
           if (BITS == 8) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) { o_bias[n][g][c] *= f; }
+            for (int g = 0; g < G; ++g) {
+              o_bias[n][g][c] *= f;
+              o_mean[n][g][c] *= fo;
+            }
           }
         }
       }
@@ -554,82 +648,92 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float m = m_run[n][i & 1];
-        p[n][i] = ex2(s[n][i] - (m == kNegInf ? 0.0f : m));  // no live token yet: 2^-inf, not NaN
+      for (int c = 0; c < 2; ++c) {
+        const float m = m_run[n][c] == kNegInf ? 0.0f : m_run[n][c];  // no live token yet: 2^-inf, not NaN
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          s[i][n][c] = ex2(s[i][n][c] - m);
+          s[i][n][2 + c] = ex2(s[i][n][2 + c] - m);
+        }
       }
     }
 
     // ---- O^T += V^T P^T
-    if (BITS == 16) {
-      uint32_t b[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w = pack_bf16x2(p[n][2 * h], p[n][2 * h + 1]);
-          l_run[n][0] += lo16(w);
-          l_run[n][1] += hi16(w);
-          b[n][h] = movm(w);
-        }
-      }
-      const int row = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        uint32_t a[4];
-        ldsm4t(a, vt + row * kRow + swz_v<D, BITS>(row, 2 * i + ch) * 16);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) { mma<false>(o_acc[n][i], a, b[n][0], b[n][1]); }
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { l_run[n][i & 1] += p[n][i]; }
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
+    for (int i = 0; i < TM; ++i) {
+      if (BITS == 16) {
         uint32_t b[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float f = vs[h][g] * up;
-            b[n][h] = movm(pack_f16x2(p[n][2 * h] * f, p[n][2 * h + 1] * f));
-            o_bias[n][g][0] = __fmaf_rn(p[n][2 * h], vb[h][g], o_bias[n][g][0]);
-            o_bias[n][g][1] = __fmaf_rn(p[n][2 * h + 1], vb[h][g], o_bias[n][g][1]);
+            const uint32_t w = pack_bf16x2(s[i][n][2 * h], s[i][n][2 * h + 1]);
+            l_run[n][0] += lo16(w);
+            l_run[n][1] += hi16(w);
+            b[n][h] = movm(w);
           }
         }
-        // codes 64 g + 8 r + 0..7 of tokens 2t, 2t + 1, 2t + 8, 2t + 9. A row's eight lanes of equal t read 64
-        // bytes; the swizzle puts the four token pairs of a half warp into different banks.
-        uint2 w[4];
+        const int row = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = 2 * t + (j & 1) + (j >> 1) * 8;
-          w[j] = lds64(vt + row * kRow + swz_v<D, BITS>(row, 4 * g + (r >> 1)) * 16 + (r & 1) * 8);
+        for (int k = 0; k < MT; ++k) {
+          uint32_t a[4];
+          ldsm4t(a, vt + (16 * i + row) * kRow + swz_v<D, BITS>(row, 2 * k + ch) * 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) { mma<false>(o_acc[n][k], a, b[n][0], b[n][1]); }
         }
-        uint32_t x[2][4];  // per token pair: values 0|1, 2|3, 4|5, 6|7 as bytes (even token, odd token, ...)
+      } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          x[h][0] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x5140);
-          x[h][1] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x7362);
-          x[h][2] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x5140);
-          x[h][3] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x7362);
+        for (int n = 0; n < NT; ++n) {
+          l_run[n][0] += s[i][n][0] + s[i][n][2];
+          l_run[n][1] += s[i][n][1] + s[i][n][3];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // rows r, r + 8 of this block: values 64 g + 8 r + 2 i, + 1
-          const uint32_t a[4] = {centred<false>(x[0][i]), centred<true>(x[0][i]), centred<false>(x[1][i]),
-                                 centred<true>(x[1][i])};
+        for (int g = 0; g < G; ++g) {
+          uint32_t b[NT][2];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) { mma<true>(o_acc[n][g * 4 + i], a, b[n][0], b[n][1]); }
+          for (int h = 0; h < 2; ++h) {
+            const float sc = lo16(vp[i][h][g]), f = sc * up, bb = __fmaf_rn(128.0f, sc, hi16(vp[i][h][g]));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              b[n][h] = movm(pack_f16x2(s[i][n][2 * h] * f, s[i][n][2 * h + 1] * f));
+              o_bias[n][g][0] = __fmaf_rn(s[i][n][2 * h], bb, o_bias[n][g][0]);
+              o_bias[n][g][1] = __fmaf_rn(s[i][n][2 * h + 1], bb, o_bias[n][g][1]);
+            }
+          }
+          const uint32_t mean[4] = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // the code 128
+#pragma unroll
+          for (int n = 0; n < NT; ++n) { mma<true>(o_mean[n][g], mean, b[n][0], b[n][1]); }
+          // codes 64 g + 8 r + 0..7 of tokens 2t, 2t + 1, 2t + 8, 2t + 9. A row's eight lanes of equal t read 64
+          // bytes; the swizzle puts the four token pairs of a half warp into different banks.
+          uint2 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = 2 * t + (j & 1) + (j >> 1) * 8;
+            w[j] = lds64(vt + (16 * i + row) * kRow + swz_v<D, BITS>(row, 4 * g + (r >> 1)) * 16 + (r & 1) * 8);
+          }
+          uint32_t x[2][4];  // per token pair: values 0|1, 2|3, 4|5, 6|7 as bytes (even token, odd token, ...)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            x[h][0] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x5140);
+            x[h][1] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x7362);
+            x[h][2] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x5140);
+            x[h][3] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x7362);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // rows r, r + 8 of this block: values 64 g + 8 r + 2 k, + 1
+            const uint32_t a[4] = {codes<false>(x[0][k]), codes<true>(x[0][k]), codes<false>(x[1][k]), codes<true>(x[1][k])};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { mma<true>(o_acc[n][g * 4 + k], a, b[n][0], b[n][1]); }
+          }
         }
       }
     }
 
     // ---- the warp's part of a (sequence, head) is complete
-    if (U.flags & kLast) {
-      const bool run_ends = (U.flags & kSegEnd) != 0;
-      const float o_mul = BITS == 8 ? __uint_as_float((uint32_t)(max(sigma - 15, -126) + 127) << 23) : 1.0f;
+    if (U.bits & kLast) {
+      const int blk = U.h % A.blocks, kvh = U.h / A.blocks;
+      const int ncol = min(A.cols, A.group - blk * A.cols);
+      const float o_mul = BITS == 8 ? __uint_as_float((uint32_t)(sigma - 15 + 127) << 23) : 1.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -647,13 +751,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { o_acc[n][i][e] = __fmaf_rn(o_acc[n][i][e], o_mul, o_bias[n][i / 4][e & 1]); }
+            for (int e = 0; e < 4; ++e) {
+              o_acc[n][i][e] = __fmaf_rn((o_acc[n][i][e] - o_mean[n][i / 4][e & 1]) * 16777216.0f, o_mul, o_bias[n][i / 4][e & 1]);
+            }
           }
         }
       }
-      if (run_begins && run_ends) {
-        const int h0 = (U.h / A.blocks) * A.group + (U.h % A.blocks) * A.cols;
-        uint8_t* op = A.out + (int64_t)U.b * A.out_stride + (int64_t)h0 * (D * 2);
+      if (run_begins && U.rest == 0) {
+        uint8_t* op = A.out + (int64_t)U.b * A.out_stride + (int64_t)(kvh * A.group + blk * A.cols) * (D * 2);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // a sum of 0: no live token (a NaN stays one)
@@ -688,20 +793,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
         }
       } else {
-        // at most two per warp: the first part of its run, kept apart, and the last, over the ring that
-        // nothing is in flight to any more
-        const int e = first_run ? 0 : 1;
-        float* to = reinterpret_cast<float*>(first_run ? entry0 : ring);
-        if (!first_run) {
+        // At most two per warp: the first part of its run and the last. When nothing more is requested the
+        // ring is free for it; a first part that is followed by other runs goes to the workspace.
+        const bool done = todo == 1;
+        EntryHead& H = s_entry[warp * 2 + (first_run ? 0 : 1)];
+        float* to = done ? reinterpret_cast<float*>(ring)
+                         : A.scratch + ((int64_t)blockIdx.x * kWarps + warp) * (A.cols * D);
+        if (done) {
           cp_wait<0>();
           __syncwarp();
         }
-        EntryHead& H = s_entry[warp * 2 + e];
         if (lane == 0) {
-          H.seg = U.b * A.hk + U.h;
-          H.flags = (run_begins ? kSegBegin : 0) | (run_ends ? kSegEnd : 0);
+          H.data = to;
           H.b = U.b;
           H.h = U.h;
+          H.begins = run_begins;
+          H.rest = U.rest;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -736,41 +843,41 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   for (int item = warp; item < kWarps * 2 * A.cols; item += kWarps) {
     const int n = item / A.cols, col = item % A.cols;
     const EntryHead& H = s_entry[n];
-    if (H.seg < 0 || col >= min(A.cols, A.group - (H.h % A.blocks) * A.cols)) { continue; }
+    if (H.b < 0) { continue; }
+    const int blk = H.h % A.blocks;
+    if (col >= min(A.cols, A.group - blk * A.cols)) { continue; }
+    auto same = [&](const EntryHead& x) { return x.b == H.b && x.h == H.h; };
     int prev = n - 1;
-    while (prev >= 0 && s_entry[prev].seg < 0) { --prev; }
-    if (prev >= 0 && s_entry[prev].seg == H.seg) { continue; }  // another item joins it
-    int end = n, flags = 0;
+    while (prev >= 0 && s_entry[prev].b < 0) { --prev; }
+    if (prev >= 0 && same(s_entry[prev])) { continue; }  // another item joins it
+    int end = n;
     float m = kNegInf;
     for (int j = n; j < kWarps * 2; ++j) {
-      if (s_entry[j].seg < 0) { continue; }
-      if (s_entry[j].seg != H.seg) { break; }
+      if (s_entry[j].b < 0) { continue; }
+      if (!same(s_entry[j])) { break; }
       end = j;
-      flags = s_entry[j].flags;
       m = fmaxf(m, s_entry[j].m[col]);
     }
-    const bool whole = (H.flags & kSegBegin) && (flags & kSegEnd);
     float l = 0.0f, acc[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
     for (int j = n; j <= end; ++j) {
-      if (s_entry[j].seg < 0) { continue; }
-      const float mj = s_entry[j].m[col];
-      const float f = mj == kNegInf ? (s_entry[j].l[col] == 0.0f ? 0.0f : 1.0f) : ex2(mj - m);
+      if (s_entry[j].b < 0) { continue; }
+      const float f = weight_of(s_entry[j].m[col], s_entry[j].l[col], m);
       l = __fmaf_rn(f, s_entry[j].l[col], l);
-      const float* from = reinterpret_cast<const float*>((j & 1) ? smem + (j >> 1) * A.ring_bytes
-                                                                 : smem + kWarps * A.ring_bytes + (j >> 1) * A.entry_bytes);
+      const float* from = s_entry[j].data + col * D + lane;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f, from[col * D + i * 32 + lane], acc[i]); }
+      for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f, from[i * 32], acc[i]); }
     }
-    if (whole) {
+    const int rest = s_entry[end].rest;
+    if (H.begins && rest == 0) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int head = (H.h / A.blocks) * A.group + (H.h % A.blocks) * A.cols + col;
+      const int head = (H.h / A.blocks) * A.group + blk * A.cols + col;
       __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head * D;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) { op[i * 32 + lane] = __float2bfloat16_rn(acc[i] * inv); }
     } else {
-      // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: the one it ends in
+      // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: another, which it ends in
       const int64_t slot = (int64_t)blockIdx.x * 2 + (n == 0 ? 0 : 1);
       float* pp = A.part + (slot * A.cols + col) * D;
 #pragma unroll
@@ -778,57 +885,80 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       if (lane == 0) {
         A.ml[(slot * A.cols + col) * 2] = m;
         A.ml[(slot * A.cols + col) * 2 + 1] = l;
+        if (H.begins && col == 0) {
+          A.heads[blockIdx.x] = {H.b, H.h, n == 0 ? 0 : 1, (int)div_u(cta1 + rest - 1, per_cta)};
+        }
       }
     }
   }
 }
 
-// Joins what several CTAs have of a (sequence, head): one warp per query head. Sequences without a
-// token get their zeros here.
-template <int D>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs A, int q_heads) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int b = (int)(id / q_heads), head = (int)(id % q_heads);
-  if (b >= A.batch) { return; }
-  const int kvh = head / A.group, blk = (head % A.group) / A.cols, col = (head % A.group) % A.cols;
-  const int64_t p0 = A.prefix[b], n = A.prefix[b + 1] - p0, per_cta = A.prefix[A.batch + 1];
-  __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)b * A.out_stride) + (int64_t)head * D;
-  float acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
-  float l = 0.0f;
-  if (n > 0) {
-    const int64_t u0 = p0 * A.hk + (kvh * A.blocks + blk) * n, u1 = u0 + n;
-    const int64_t c0 = u0 / per_cta, c1 = (u1 - 1) / per_cta;
-    if (c0 == c1) { return; }  // one CTA had it all and has written it
-    auto slot_of = [&](int64_t c) { return (c * 2 + (c * per_cta < u0 ? 1 : 0)) * A.cols + col; };
-    float m = kNegInf;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) { m = fmaxf(m, A.ml[slot_of(c) * 2]); }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d)); }
-#pragma unroll 4
-    for (int64_t c = c0; c <= c1; ++c) {
-      const int64_t sl = slot_of(c);
-      const float mj = A.ml[sl * 2], lj = A.ml[sl * 2 + 1];
-      const float f = mj == kNegInf ? (lj == 0.0f ? 0.0f : 1.0f) : ex2(mj - m);
-      l = __fmaf_rn(f, lj, l);
-      const float* pp = A.part + sl * D;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f, pp[i * 32 + lane], acc[i]); }
+// Joins what several CTAs have of a (sequence, head): block (c, col) serves column col of the one that
+// begins in CTA c's run, its eight warps take every eighth part. Rows of sequences without a token get
+// their zeros here, while the first kernel still runs.
+constexpr int kJoinWarps = 8;
+template <int D, int U>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const AttnArgs A, int q_heads) {
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_acc[kJoinWarps][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x, col = blockIdx.y;
+  if (col == 0) {
+    // the first kernel has let this one start after what was before it had finished: lengths may be read
+    for (int b = c0; b < A.batch; b += gridDim.x) {
+      int s, n;
+      token_range(A, b, s, n);
+      if (n > s) { continue; }
+      uint4* row = reinterpret_cast<uint4*>(A.out + (int64_t)b * A.out_stride);
+      for (int i = threadIdx.x; i < q_heads * (D / 8); i += kJoinWarps * 32) { row[i] = make_uint4(0, 0, 0, 0); }
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const CtaHead H = A.heads[c0];
+  if (H.last < 0) { return; }
+  const int blk = H.h % A.blocks;
+  if (col >= min(A.cols, A.group - blk * A.cols)) { return; }
+  float m = kNegInf, l = 0.0f, acc[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) { op[i * 32 + lane] = __float2bfloat16_rn(acc[i] * inv); }
+  for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
+  for (int c = c0 + warp; c <= H.last; c += kJoinWarps) {
+    const int64_t slot = ((int64_t)c * 2 + (c == c0 ? H.slot : 0)) * A.cols + col;
+    const float mj = A.ml[slot * 2], lj = A.ml[slot * 2 + 1];
+    const float* pp = A.part + slot * D + lane;
+    float x[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) { x[i] = pp[i * 32]; }
+    const float m2 = fmaxf(m, mj);
+    const float f0 = weight_of(m, l, m2), f1 = weight_of(mj, lj, m2);
+    m = m2;
+    l = __fmaf_rn(f1, lj, f0 * l);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f1, x[i], f0 * acc[i]); }
+  }
+  if (lane == 0) { s_m[warp] = m, s_l[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) { s_acc[warp][i * 32 + lane] = acc[i]; }
+  __syncthreads();
+  if (threadIdx.x >= D) { return; }
+  float top = kNegInf, sum = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) { top = fmaxf(top, s_m[w]); }
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float f = weight_of(s_m[w], s_l[w], top);
+    sum = __fmaf_rn(f, s_l[w], sum);
+    o = __fmaf_rn(f, s_acc[w][threadIdx.x], o);
+  }
+  const int head = (H.h / A.blocks) * A.group + blk * A.cols + col;
+  __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head * D;
+  op[threadIdx.x] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : o / sum);
 }
 
 // ---------------------------------------------------------------- host side
 struct Shape {
   int group, cols, nt, blocks, ctas;
-  size_t prefix, ml, part, total;  // byte offsets in the workspace, and its size
+  size_t heads, ml, part, scratch, total;  // byte offsets in the workspace, and its size
 };
+constexpr int kMaxWarps = 10;  // of any instantiation: the scratch has room for them
 
 int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_cache* c, Shape* s) {
   if (!d || !c) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
@@ -839,9 +969,7 @@ int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_ca
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) {
     return fail(VPQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256 (got %d)", who, c->head_dim);
   }
-  if (d->q_heads > 65536 || (int64_t)d->batch * d->q_heads > INT_MAX / 2) {
-    return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 query heads and 2^30 of them in a batch", who);
-  }
+  if (d->q_heads > 65536) { return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 query heads", who); }
   s->group = d->q_heads / c->kv_heads;
   // Two column blocks of eight share a read of the cache where the accumulators leave room (head_dim
   // 256 has 64 of them per block); wider groups read it again, from L2 for the most part.
@@ -850,26 +978,27 @@ int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_ca
   s->blocks = (s->group + s->cols - 1) / s->cols;
   s->ctas = num_sms();
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  s->prefix = 0;
-  s->ml = up((size_t)(d->batch + 2) * 8);
+  const size_t row = (size_t)s->cols * c->head_dim * 4;
+  s->heads = 0;
+  s->ml = up((size_t)s->ctas * sizeof(CtaHead));
   s->part = s->ml + up((size_t)s->ctas * 2 * s->cols * 8);
-  s->total = s->part + up((size_t)s->ctas * 2 * s->cols * c->head_dim * 4);
+  s->scratch = s->part + up((size_t)s->ctas * 2 * row);
+  s->total = s->scratch + up((size_t)s->ctas * kMaxWarps * row);
   return VPQ_OK;
 }
 
-template <int D, int BITS, int NT, int kWarps, int STAGES>
-int launch_main(const AttnArgs& a0, const Shape& s, cudaStream_t st) {
+template <int D, int BITS, int NT, int TM, int kWarps, int STAGES>
+int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
+  static_assert(kWarps <= kMaxWarps, "the workspace is sized for kMaxWarps");
+  static_assert(NT * 8 * D * 4 <= STAGES * 2 * 16 * TM * (D * BITS / 8), "a warp's partial result fits its ring");
+  constexpr int kStage = 2 * 16 * TM * (D * BITS / 8) + (BITS == 8 ? 2 * 16 * TM * (D / kKvGroup) * 4 : 0);
+  static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= 220 * 1024, "rings fit beside the static shared memory");
   AttnArgs a = a0;
-  constexpr int kRow = D * BITS / 8;
-  constexpr int kPairs = BITS == 8 ? kUnit * (D / kKvGroup) * 4 : 0;
-  a.stage_bytes = 2 * kUnit * kRow + 2 * kPairs + ((s.cols * D * 2 + 127) & ~127);
-  a.entry_bytes = s.cols * D * 4;
+  a.stage_bytes = kStage + ((s.cols * D * 2 + 127) & ~127);
   a.ring_bytes = a.stage_bytes * STAGES;
-  if (a.ring_bytes < a.entry_bytes) { a.ring_bytes = a.entry_bytes; }
-  a.ring_bytes = (a.ring_bytes + 127) & ~127;
-  const size_t smem = (size_t)kWarps * (a.ring_bytes + a.entry_bytes);
   static int granted[64] = {};
-  auto kern = paged_attn_kernel<D, BITS, NT, kWarps, STAGES>;
+  auto kern = paged_attn_kernel<D, BITS, NT, TM, kWarps, STAGES>;
+  const size_t smem = (size_t)kWarps * a.ring_bytes;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), granted, smem)) { return rc; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)s.ctas, 1, 1);
@@ -882,22 +1011,10 @@ int launch_main(const AttnArgs& a0, const Shape& s, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   VPQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a));
-  return VPQ_OK;
-}
-
-template <int D>
-int launch_join(const AttnArgs& a, int q_heads, cudaStream_t st) {
-  const int64_t warps = (int64_t)a.batch * q_heads;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((warps + 7) / 8), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  VPQ_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, a, q_heads));
+  cfg.gridDim = dim3((unsigned)s.ctas, (unsigned)s.cols, 1);
+  cfg.blockDim = dim3(kJoinWarps * 32, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  VPQ_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, 16 * TM>, a, q_heads));
   return VPQ_OK;
 }
 
@@ -946,7 +1063,7 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
     return fail(VPQ_ERR_INVALID_ARG, "%s: a row stride is smaller than a row or out of range", who);
   }
   if (d.window < 0) { return fail(VPQ_ERR_INVALID_ARG, "%s: window must not be negative", who); }
-  if ((int64_t)d.max_pages * cache_host->page_size > INT_MAX - kUnit) {
+  if ((int64_t)d.max_pages * cache_host->page_size > INT_MAX - 64) {
     return fail(VPQ_ERR_UNSUPPORTED, "%s: max_pages * page_size must stay below 2^31", who);
   }
   if (!(d.scale >= 0.0f) || d.scale > 3.4e38f) { return fail(VPQ_ERR_INVALID_ARG, "%s: scale must be finite and not negative", who); }
@@ -966,9 +1083,10 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   a.page_table = d.page_table;
   a.seq_lens = d.seq_lens;
   a.table_stride = ts;
-  a.prefix = reinterpret_cast<int64_t*>(ws + s.prefix);
+  a.heads = reinterpret_cast<CtaHead*>(ws + s.heads);
   a.ml = reinterpret_cast<float*>(ws + s.ml);
   a.part = reinterpret_cast<float*>(ws + s.part);
+  a.scratch = reinterpret_cast<float*>(ws + s.scratch);
   a.batch = d.batch;
   a.max_pages = d.max_pages;
   a.window = d.window;
@@ -980,23 +1098,17 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool q8 = cache_host->bits == 8, two = s.nt == 2;
-  int rc = VPQ_OK;
-  // Warps and stages by what fits 227 KB: eight warps, or four where a stage or the partial results are large.
+  const int qh = d.q_heads;
+  // Tokens of a unit, warps and stages. A stage holds 8 to 16 KB, so that a warp's copies in flight cover the
+  // latency; the warps' rings fill the shared memory.
   switch (cache_host->head_dim) {
     case 64:
-      rc = q8 ? (two ? launch_main<64, 8, 2, 8, 4>(a, s, st) : launch_main<64, 8, 1, 8, 4>(a, s, st))
-              : (two ? launch_main<64, 16, 2, 8, 3>(a, s, st) : launch_main<64, 16, 1, 8, 4>(a, s, st));
-      if (rc == VPQ_OK) { rc = launch_join<64>(a, d.q_heads, st); }
-      break;
+      if (q8) { return two ? launch<64, 8, 2, 2, 8, 3>(a, s, qh, st) : launch<64, 8, 1, 2, 8, 4>(a, s, qh, st); }
+      return two ? launch<64, 16, 2, 1, 8, 3>(a, s, qh, st) : launch<64, 16, 1, 1, 8, 4>(a, s, qh, st);
     case 128:
-      rc = q8 ? (two ? launch_main<128, 8, 2, 8, 2>(a, s, st) : launch_main<128, 8, 1, 8, 3>(a, s, st))
-              : (two ? launch_main<128, 16, 2, 4, 3>(a, s, st) : launch_main<128, 16, 1, 8, 2>(a, s, st));
-      if (rc == VPQ_OK) { rc = launch_join<128>(a, d.q_heads, st); }
-      break;
+      if (q8) { return two ? launch<128, 8, 2, 2, 8, 2>(a, s, qh, st) : launch<128, 8, 1, 2, 8, 2>(a, s, qh, st); }
+      return two ? launch<128, 16, 2, 1, 8, 2>(a, s, qh, st) : launch<128, 16, 1, 1, 8, 2>(a, s, qh, st);
     default:
-      rc = q8 ? launch_main<256, 8, 1, 4, 3>(a, s, st) : launch_main<256, 16, 1, 4, 2>(a, s, st);
-      if (rc == VPQ_OK) { rc = launch_join<256>(a, d.q_heads, st); }
-      break;
+      return q8 ? launch<256, 8, 1, 1, 8, 2>(a, s, qh, st) : launch<256, 16, 1, 1, 5, 2>(a, s, qh, st);
   }
-  return rc;
 }
