@@ -11,6 +11,29 @@ __device__ uint32_t g_kv_status = 0;
 
 namespace {
 
+// How a token's heads are dealt: every part (q, k, v) is cut into chunks of HPT neighbouring heads, and one
+// lane group takes a chunk. A block holds the chunks of `tokens` whole tokens, or one token's chunks are spread
+// evenly over `token_blocks` blocks.
+struct Deal {
+  int qc, kc;        // chunks of q, and of k (of v as many)
+  int chunks;        // of a token
+  int per_block;     // of a token in a block
+  int tokens, token_blocks;
+  uint32_t rcp;      // 2^16 / per_block, rounded up: (g * rcp) >> 16 = g / per_block for g < 256
+};
+// The calling lane group's token and chunk; false past the end (such lanes keep their warp's shuffles company).
+template <int LPH>
+__device__ __forceinline__ bool dealt(const Deal& d, int64_t M, int64_t& m, int& chunk) {
+  const uint32_t g = threadIdx.x / LPH;
+  const uint32_t tl = (g * d.rcp) >> 16;
+  const uint32_t tb = blockIdx.x / (uint32_t)d.token_blocks;
+  m = (int64_t)tb * d.tokens + tl;
+  chunk = (int)((blockIdx.x - tb * (uint32_t)d.token_blocks) * (uint32_t)d.per_block + (g - tl * d.per_block));
+  const bool in = (int)tl < d.tokens && m < M && chunk < d.chunks;
+  if (!in) { m = 0, chunk = 0; }
+  return in;
+}
+
 // One head's row is D values, eight (16 bytes) per lane: LPH = D / 8 lanes hold it, and every
 // reduction (the norm's sum, a group's extremes) and the exchange of rotation partners is a shuffle
 // among them. A head is processed in registers from load to store, so q_out = q is safe.
@@ -25,9 +48,7 @@ struct QkArgs {
   const int64_t* slots;
   int64_t M, table_rows, num_slots;
   int heads[3];
-  int chunks;      // lane groups that share a token's heads
-  int per_block;   // of them in a block, and the blocks of a token
-  int token_blocks;
+  Deal deal;
   int rot, interleaved;
   float eps, inv_d;
   KvView kv;
@@ -78,7 +99,7 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
   const float b = __bfloat162float(b16);
   const float range = __fsub_rn(mx, b);
   const __nv_bfloat16 s16 = __float2bfloat16_ru(fmaxf(__fdiv_rn(range, 255.0f), 1.17549435e-38f));
-  const float inv = __fdiv_rn(1.0f, __bfloat162float(s16));
+  const float inv = __frcp_rn(__bfloat162float(s16));
   const bool fine = range <= 3.402823466e38f;  // false for NaN
   pair = fine ? ((uint32_t)__bfloat16_as_ushort(s16) | ((uint32_t)__bfloat16_as_ushort(b16) << 16)) : 0x7fff7fffu;
   // Adding 2^23 rounds to an integer, ties to even, and leaves it in the low byte: b <= x and the rounded-up
@@ -97,23 +118,32 @@ __device__ __forceinline__ int64_t slot_page(int64_t slot, int page_size) {
   return (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
 }
 
-// MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads a lane
-// group takes, all loaded before the first is used.
+// MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads of a chunk, all
+// requested before the first is used; their table row, norm weights and addresses are fetched once.
 template <int D, int MODE, int HPT>
-__global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
+__global__ void __launch_bounds__(256) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
   constexpr int LPH = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int l = threadIdx.x % LPH;
-  const uint32_t tok = blockIdx.x / (uint32_t)A.token_blocks;
-  const int slice = (int)(blockIdx.x - tok * (uint32_t)A.token_blocks) * A.per_block + (int)threadIdx.x / LPH;
-  const int64_t m = tok;
-  const bool in_range = (int)threadIdx.x / LPH < A.per_block && slice < A.chunks;  // the rest keeps its warp's shuffles company
-  const int chunk = in_range ? slice : 0;
-  const int hq = A.heads[0], hqk = hq + A.heads[1];
-  const int total = hqk + (MODE ? A.heads[2] : 0);
+  const int l = threadIdx.x % LPH, d0 = l * 8;
+  int64_t m;
+  int chunk;
+  const bool in_range = dealt<LPH>(A.deal, A.M, m, chunk);
+  const int part = chunk < A.deal.qc ? 0 : (MODE == 0 || chunk < A.deal.qc + A.deal.kc ? 1 : 2);
+  const int h0 = HPT * (chunk - (part == 0 ? 0 : (part == 1 ? A.deal.qc : A.deal.qc + A.deal.kc)));
+  const int n = min(HPT, (part == 0 ? A.heads[0] : A.heads[1]) - h0);  // heads of this chunk
 
-  bool turn = in_range;  // whether the rotated parts of this token are written
+  const uint8_t* in = (part == 0 ? A.in[0] : (part == 1 ? A.in[1] : A.in[2])) +
+                      m * (part == 0 ? A.in_stride[0] : (part == 1 ? A.in_stride[1] : A.in_stride[2])) +
+                      (int64_t)h0 * (D * 2) + l * 16;
+  uint4 raw[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (in_range && i < n) { raw[i] = *reinterpret_cast<const uint4*>(in + i * (D * 2)); }
+  }
+
+  bool turn = in_range;  // whether this token is written at all
   int64_t row = m;
   if (A.cos_sin && A.positions) {
     const int p = __ldg(A.positions + m);
@@ -121,178 +151,209 @@ __global__ void __launch_bounds__(256) norm_rope_store_kernel(const QkArgs A) {
     if (in_range && p >= A.table_rows && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
     row = turn ? p : 0;
   }
-  bool store = false;
-  int64_t page = 0, at = 0;
-  if (MODE) {
+  uint8_t* out;                    // where head h0 of this token goes
+  int64_t out_step = D * 2;        // and from a head to the next
+  uint8_t* pairs = nullptr;
+  if (MODE == 0 || part == 0) {
+    out = (part == 0 ? A.out[0] : A.out[1]) + m * (part == 0 ? A.out_stride[0] : A.out_stride[1]) +
+          (int64_t)h0 * (D * 2) + l * 16;
+  } else {
     const int64_t s = __ldg(A.slots + m);
-    store = in_range && turn && s >= 0 && s < A.num_slots;
+    turn = turn && s >= 0 && s < A.num_slots;
     if (in_range && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-    if (store) {
-      page = slot_page(s, A.kv.page_size);
-      at = s - page * A.kv.page_size;
+    const int64_t page = turn ? slot_page(s, A.kv.page_size) : 0, at = turn ? s - page * A.kv.page_size : 0;
+    out = (part == 1 ? A.kv.k : A.kv.v) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
+          l * (MODE == 8 ? 8 : 16);
+    out_step = A.kv.head_bytes;
+    if (MODE == 8) {
+      pairs = (part == 1 ? A.kv.ks : A.kv.vs) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes +
+              at * A.kv.stoken_bytes + (l >> 3) * 4;
     }
   }
 
-  uint4 raw[HPT];
+  // This lane's eight values among the pairs: y = r (x cw + o sw), o the partner's values (in lane `partner`, or
+  // the neighbours). The norm weights are folded into cos and sin, so that a head costs one product and one sum a
+  // value, and the exchange does not wait for the norm.
+  const int half = A.rot >> 1;
+  const bool rotated = A.cos_sin && d0 < A.rot && part < 2;
+  const bool swap = A.cos_sin && !A.interleaved;
+  const bool any_norm = A.norm_w[0] || A.norm_w[1];
+  const uint16_t* nw = part == 0 ? A.norm_w[0] : (part == 1 ? A.norm_w[1] : nullptr);
+  float cw[8], sw[8];
+  if (nw) {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(nw + d0)), cw);
+  } else {
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int h = chunk + i * A.chunks;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (in_range && h < total) {
-      const int part = h < hq ? 0 : (h < hqk ? 1 : 2);
-      const int hh = h - (part == 0 ? 0 : (part == 1 ? hq : hqk));
-      raw[i] = *reinterpret_cast<const uint4*>(A.in[part] + m * A.in_stride[part] + (int64_t)hh * (D * 2) + l * 16);
-    }
+    for (int e = 0; e < 8; ++e) { cw[e] = 1.0f; }
   }
-
-  // this lane's eight values and their place among the pairs
-  const int d0 = l * 8, half = A.rot >> 1;
-  float cs[8], sn[8];
   int partner = l;
-  bool second = false;
+  if (swap) {
+    const bool second = d0 >= half;
+    if (rotated) { partner = second ? l - (half >> 3) : l + (half >> 3); }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { cs[i] = 1.0f, sn[i] = 0.0f; }
-  const bool rotated = A.cos_sin && d0 < A.rot;
-  if (rotated) {
-    const float* t = A.cos_sin + row * A.rot;
-    if (A.interleaved) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(t + (d0 >> 1)));
-      const float4 s = __ldg(reinterpret_cast<const float4*>(t + half + (d0 >> 1)));
-      cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
-      sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
-    } else {
-      second = d0 >= half;
-      const int j = second ? d0 - half : d0;
-      partner = second ? l - (half >> 3) : l + (half >> 3);
-      const float4 c0 = __ldg(reinterpret_cast<const float4*>(t + j)), c1 = __ldg(reinterpret_cast<const float4*>(t + j + 4));
-      const float4 s0 = __ldg(reinterpret_cast<const float4*>(t + half + j));
-      const float4 s1 = __ldg(reinterpret_cast<const float4*>(t + half + j + 4));
-      cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
-      sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w, sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
+    for (int e = 0; e < 8; ++e) { sw[e] = __shfl_sync(0xffffffffu, cw[e], partner, LPH); }
+    if (rotated) {
+      const float* tab = A.cos_sin + row * A.rot + (second ? d0 - half : d0);
+      const float sg = second ? 1.0f : -1.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 c = __ldg(reinterpret_cast<const float4*>(tab + e)), s = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+        cw[e] *= c.x, cw[e + 1] *= c.y, cw[e + 2] *= c.z, cw[e + 3] *= c.w;
+        sw[e] *= sg * s.x, sw[e + 1] *= sg * s.y, sw[e + 2] *= sg * s.z, sw[e + 3] *= sg * s.w;
+      }
+    }
+  } else if (rotated) {
+    const float* tab = A.cos_sin + row * A.rot + (d0 >> 1);
+    const float4 c4 = __ldg(reinterpret_cast<const float4*>(tab)), s4 = __ldg(reinterpret_cast<const float4*>(tab + half));
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float wa = cw[2 * e], wb = cw[2 * e + 1];
+      cw[2 * e] = wa * c[e], sw[2 * e] = -wb * s[e];
+      cw[2 * e + 1] = wb * c[e], sw[2 * e + 1] = wa * s[e];
     }
   }
 
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
-    const int h = chunk + i * A.chunks;
-    if (__all_sync(0xffffffffu, h >= total)) { break; }
-    const int part = h < hq ? 0 : (h < hqk ? 1 : 2);
-    const int hh = h - (part == 0 ? 0 : (part == 1 ? hq : hqk));
+    if (__all_sync(0xffffffffu, i >= n)) { break; }
     float x[8];
     unpack8(raw[i], x);
-    // lanes of a warp can hold heads of different parts: the shuffles below run for all, the values of v are kept
-    float ss = 0.0f;
-    if (A.norm_w[0] || A.norm_w[1]) {
+    // lanes of a warp can hold heads of different parts: the shuffles run for all, the values of v stay as they are
+    float r = 1.0f;
+    if (any_norm) {
+      float ss = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
 #pragma unroll
       for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
+      if (nw) { r = rsqrtf(__fmaf_rn(ss, A.inv_d, A.eps)); }
     }
-    if (part < 2 && h < total && A.norm_w[part]) {
-      float w[8];
-      unpack8(__ldg(reinterpret_cast<const uint4*>(A.norm_w[part] + d0)), w);
-      const float r = rsqrtf(__fmaf_rn(ss, A.inv_d, A.eps));
+    float o[8];
+    if (swap) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { x[e] = x[e] * r * w[e]; }
-    }
-    if (A.interleaved) {
-      if (part < 2 && rotated) {
+      for (int e = 0; e < 8; ++e) { o[e] = __shfl_sync(0xffffffffu, x[e], partner, LPH); }
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = x[2 * e], b = x[2 * e + 1];
-          x[2 * e] = a * cs[e] - b * sn[e];
-          x[2 * e + 1] = b * cs[e] + a * sn[e];
-        }
-      }
-    } else if (A.cos_sin) {
+      for (int e = 0; e < 8; ++e) { o[e] = x[e ^ 1]; }
+    }
+    if (part < 2) {
+      if (rotated) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float o = __shfl_sync(0xffffffffu, x[e], partner, LPH);
-        if (part < 2 && rotated) { x[e] = second ? x[e] * cs[e] + o * sn[e] : x[e] * cs[e] - o * sn[e]; }
-      }
-    }
-    if (MODE == 0 || part == 0) {
-      if (turn && h < total) {
-        uint8_t* o = A.out[part] + m * A.out_stride[part] + (int64_t)hh * (D * 2) + l * 16;
-        *reinterpret_cast<uint4*>(o) = pack8(x);
-      }
-    }
-    if (MODE == 16) {
-      if (store && part > 0 && h < total) {
-        uint8_t* base = part == 1 ? A.kv.k : A.kv.v;
-        const int64_t off = page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes + l * 16;
-        *reinterpret_cast<uint4*>(base + off) = pack8(x);
+        for (int e = 0; e < 8; ++e) { x[e] = __fmaf_rn(o[e], sw[e], x[e] * cw[e]) * r; }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { x[e] = x[e] * cw[e] * r; }
       }
     }
     if (MODE == 8 && __any_sync(0xffffffffu, part > 0)) {
       uint32_t pair;
       const uint2 c = quant8(x, pair);
-      if (store && part > 0 && h < total) {
-        const int64_t off = page * A.kv.page_bytes + hh * A.kv.head_bytes + at * A.kv.token_bytes + l * 8;
-        *reinterpret_cast<uint2*>((part == 1 ? A.kv.k : A.kv.v) + off) = c;
-        if ((l & 7) == 0) {
-          const int64_t so = page * A.kv.spage_bytes + hh * A.kv.shead_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4;
-          *reinterpret_cast<uint32_t*>((part == 1 ? A.kv.ks : A.kv.vs) + so) = pair;
-        }
+      if (part > 0 && turn && i < n) {
+        *reinterpret_cast<uint2*>(out + i * out_step) = c;
+        if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
+      }
+    }
+    if ((MODE != 8 || part == 0) && turn && i < n) { *reinterpret_cast<uint4*>(out + i * out_step) = pack8(x); }
+  }
+}
+
+struct CopyArgs {
+  KvView kv;
+  uint8_t* rows[2];   // k, v: read by the store, written by the load
+  int64_t stride[2];  // bytes
+  const int64_t* slots;
+  int64_t M, num_slots;
+  Deal deal;
+};
+
+// Rows into the cache.
+template <int D, int BITS, int HPT>
+__global__ void __launch_bounds__(256) kv_store_kernel(const __grid_constant__ CopyArgs A) {
+  constexpr int LPH = D / 8;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int l = threadIdx.x % LPH;
+  int64_t m;
+  int chunk;
+  const bool in_range = dealt<LPH>(A.deal, A.M, m, chunk);
+  const bool is_v = chunk >= A.deal.kc;
+  const int h0 = HPT * (is_v ? chunk - A.deal.kc : chunk);
+  const int n = in_range ? min(HPT, A.kv.kv_heads - h0) : 0;
+  const uint8_t* in = (is_v ? A.rows[1] : A.rows[0]) + m * (is_v ? A.stride[1] : A.stride[0]) + (int64_t)h0 * (D * 2) + l * 16;
+  uint4 raw[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (i < n) { raw[i] = ldg_stream_v4(in + i * (D * 2)); }
+  }
+  const int64_t s = __ldg(A.slots + m);
+  if (n > 0 && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+  const bool live = s >= 0 && s < A.num_slots;
+  const int64_t page = live ? slot_page(s, A.kv.page_size) : 0, at = live ? s - page * A.kv.page_size : 0;
+  uint8_t* out = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
+                 l * (BITS == 16 ? 16 : 8);
+  uint8_t* pairs = (is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes + at * A.kv.stoken_bytes +
+                   (l >> 3) * 4;
+  const int writes = live ? n : 0;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    if (BITS == 16) {
+      if (i < writes) { *reinterpret_cast<uint4*>(out + i * A.kv.head_bytes) = raw[i]; }
+    } else {
+      float x[8];
+      unpack8(raw[i], x);
+      uint32_t pair;
+      const uint2 c = quant8(x, pair);
+      if (i < writes) {
+        *reinterpret_cast<uint2*>(out + i * A.kv.head_bytes) = c;
+        if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
       }
     }
   }
 }
 
-struct LoadArgs {
-  KvView kv;
-  uint8_t* out[2];
-  int64_t stride[2];  // bytes
-  const int64_t* slots;
-  int64_t M, num_slots;
-  int chunks, per_block, token_blocks;
-};
-
-// Eight values a lane and head: 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out. A lane
-// group takes HPT heads of its token, all requested before the first is used.
+// Rows out of it: eight values a lane and head, 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out.
 template <int D, int BITS, int HPT>
-__global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs A) {
+__global__ void __launch_bounds__(256) kv_load_kernel(const __grid_constant__ CopyArgs A) {
   constexpr int LPH = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int l = threadIdx.x % LPH;
-  const uint32_t tok = blockIdx.x / (uint32_t)A.token_blocks;
-  const int chunk = (int)(blockIdx.x - tok * (uint32_t)A.token_blocks) * A.per_block + (int)threadIdx.x / LPH;
-  if ((int)threadIdx.x / LPH >= A.per_block || chunk >= A.chunks) { return; }
-  const int64_t m = tok;
-  const int heads = 2 * A.kv.kv_heads;
+  int64_t m;
+  int chunk;
+  if (!dealt<LPH>(A.deal, A.M, m, chunk)) { return; }
+  const bool is_v = chunk >= A.deal.kc;
+  const int h0 = HPT * (is_v ? chunk - A.deal.kc : chunk);
+  const int n = min(HPT, A.kv.kv_heads - h0);
   const int64_t s = __ldg(A.slots + m);
   if (s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
   const bool live = s >= 0 && s < A.num_slots;
   const int64_t page = live ? slot_page(s, A.kv.page_size) : 0, at = live ? s - page * A.kv.page_size : 0;
-  const int64_t off = page * A.kv.page_bytes + at * A.kv.token_bytes + l * (BITS == 16 ? 16 : 8);
-  const int64_t soff = page * A.kv.spage_bytes + at * A.kv.stoken_bytes + (l >> 3) * 4;
+  const uint8_t* in = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
+                      l * (BITS == 16 ? 16 : 8);
+  const uint8_t* pairs = (is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes +
+                         at * A.kv.stoken_bytes + (l >> 3) * 4;
   uint4 y[HPT];
   uint32_t pair[HPT];
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
-    const int h = chunk + i * A.chunks;
-    const bool is_v = h >= A.kv.kv_heads;
-    const int hh = is_v ? h - A.kv.kv_heads : h;
     y[i] = make_uint4(0, 0, 0, 0);
     pair[i] = 0;
-    if (live && h < heads) {
-      const uint8_t* p = (is_v ? A.kv.v : A.kv.k) + off + hh * A.kv.head_bytes;
+    if (live && i < n) {
       if (BITS == 16) {
-        y[i] = *reinterpret_cast<const uint4*>(p);
+        y[i] = *reinterpret_cast<const uint4*>(in + i * A.kv.head_bytes);
       } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(p);
+        const uint2 c = *reinterpret_cast<const uint2*>(in + i * A.kv.head_bytes);
         y[i].x = c.x, y[i].y = c.y;
-        pair[i] = *reinterpret_cast<const uint32_t*>((is_v ? A.kv.vs : A.kv.ks) + soff + hh * A.kv.shead_bytes);
+        pair[i] = *reinterpret_cast<const uint32_t*>(pairs + i * A.kv.shead_bytes);
       }
     }
   }
+  uint8_t* out = (is_v ? A.rows[1] : A.rows[0]) + m * (is_v ? A.stride[1] : A.stride[0]) + (int64_t)h0 * (D * 2) + l * 16;
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
-    const int h = chunk + i * A.chunks;
-    if (h >= heads) { break; }
-    const bool is_v = h >= A.kv.kv_heads;
-    const int hh = is_v ? h - A.kv.kv_heads : h;
+    if (i >= n) { break; }
     if (BITS == 8) {
       const float sc = __uint_as_float(pair[i] << 16), b = __uint_as_float(pair[i] & 0xffff0000u);
       float x[8];
@@ -303,36 +364,38 @@ __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs A) {
       }
       y[i] = pack8(x);
     }
-    *reinterpret_cast<uint4*>(A.out[is_v] + m * A.stride[is_v] + (int64_t)hh * (D * 2) + l * 16) = y[i];
+    *reinterpret_cast<uint4*>(out + i * (D * 2)) = y[i];
   }
 }
 
 bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
 
-// How a token's heads are dealt: `chunks` lane groups take HPT heads each, evenly over blocks of at most
-// 256 threads that belong to one token (no division by the thread, and a token's table row is fetched by few
-// blocks). One head per lane group while the launch is too small to fill the machine (a decode step lives by
-// latency); four once there are waves of them.
-struct Deal {
-  bool wide;
-  int chunks, per_block, token_blocks;
+// One head per lane group while the launch is too small to fill the machine (a decode step lives by
+// latency), four once there are waves of them.
+bool is_wide(int64_t M, int heads, int D) { return M * heads > (int64_t)num_sms() * 8 * (256 / (D / 8)) * 2; }
+
+struct Launch {
   dim3 grid, block;
 };
-int deal(const char* who, int64_t M, int heads, int D, Deal* d) {
+int deal(const char* who, int64_t M, int q_heads, int kv_heads, bool with_v, int hpt, int D, Deal* d, Launch* l) {
   const int groups = 256 / (D / 8);
-  d->wide = M * heads > (int64_t)num_sms() * 8 * groups * 2;
-  const int hpt = d->wide ? 4 : 1;
-  d->chunks = (heads + hpt - 1) / hpt;
+  d->qc = (q_heads + hpt - 1) / hpt;
+  d->kc = (kv_heads + hpt - 1) / hpt;
+  d->chunks = d->qc + (with_v ? 2 : 1) * d->kc;
   d->token_blocks = (d->chunks + groups - 1) / groups;
   d->per_block = (d->chunks + d->token_blocks - 1) / d->token_blocks;
-  if (M > INT_MAX / d->token_blocks) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
-  d->grid = dim3((unsigned)(M * d->token_blocks));
-  d->block = dim3((unsigned)((d->per_block * (D / 8) + 31) & ~31));
+  d->tokens = groups / d->per_block;
+  if (d->token_blocks > 1 || M < num_sms()) { d->tokens = 1; }
+  d->rcp = (65536u + d->per_block - 1) / d->per_block;
+  const int64_t blocks = (M + d->tokens - 1) / d->tokens;
+  if (blocks > INT_MAX / d->token_blocks) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
+  l->grid = dim3((unsigned)(blocks * d->token_blocks));
+  l->block = dim3((unsigned)((d->tokens * d->per_block * (D / 8) + 31) & ~31));
   return VPQ_OK;
 }
 
 template <typename K, typename A>
-int launch_with_pdl(K kern, const Deal& d, cudaStream_t st, const A& a) {
+int launch_with_pdl(K kern, const Launch& d, cudaStream_t st, const A& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = d.grid;
   cfg.blockDim = d.block;
@@ -349,34 +412,38 @@ int launch_with_pdl(K kern, const Deal& d, cudaStream_t st, const A& a) {
 template <int MODE>
 int launch_norm(const char* who, const QkArgs& a0, int D, cudaStream_t st) {
   QkArgs a = a0;
-  Deal d;
-  if (int rc = deal(who, a.M, a.heads[0] + a.heads[1] + (MODE ? a.heads[2] : 0), D, &d)) { return rc; }
-  a.chunks = d.chunks, a.per_block = d.per_block, a.token_blocks = d.token_blocks;
+  Launch l;
+  const bool wide = is_wide(a.M, a.heads[0] + (MODE ? 2 : 1) * a.heads[1], D);
+  if (int rc = deal(who, a.M, a.heads[0], a.heads[1], MODE != 0, wide ? 4 : 1, D, &a.deal, &l)) { return rc; }
   if (D == 64) {
-    return d.wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, d, st, a)
-                  : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, d, st, a);
+    return wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, l, st, a)
+                : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, l, st, a);
   }
   if (D == 128) {
-    return d.wide ? launch_with_pdl(norm_rope_store_kernel<128, MODE, 4>, d, st, a)
-                  : launch_with_pdl(norm_rope_store_kernel<128, MODE, 1>, d, st, a);
+    return wide ? launch_with_pdl(norm_rope_store_kernel<128, MODE, 4>, l, st, a)
+                : launch_with_pdl(norm_rope_store_kernel<128, MODE, 1>, l, st, a);
   }
-  return d.wide ? launch_with_pdl(norm_rope_store_kernel<256, MODE, 4>, d, st, a)
-                : launch_with_pdl(norm_rope_store_kernel<256, MODE, 1>, d, st, a);
+  return wide ? launch_with_pdl(norm_rope_store_kernel<256, MODE, 4>, l, st, a)
+              : launch_with_pdl(norm_rope_store_kernel<256, MODE, 1>, l, st, a);
 }
 
-template <int BITS>
-int launch_load(const char* who, const LoadArgs& a0, int D, cudaStream_t st) {
-  LoadArgs a = a0;
-  Deal d;
-  if (int rc = deal(who, a.M, 2 * a.kv.kv_heads, D, &d)) { return rc; }
-  a.chunks = d.chunks, a.per_block = d.per_block, a.token_blocks = d.token_blocks;
-  if (D == 64) {
-    return d.wide ? launch_with_pdl(kv_load_kernel<64, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<64, BITS, 1>, d, st, a);
+template <int BITS, bool STORE, int D>
+int launch_copy_d(bool wide, const Launch& l, cudaStream_t st, const CopyArgs& a) {
+  if (STORE) {
+    return wide ? launch_with_pdl(kv_store_kernel<D, BITS, 4>, l, st, a) : launch_with_pdl(kv_store_kernel<D, BITS, 1>, l, st, a);
   }
-  if (D == 128) {
-    return d.wide ? launch_with_pdl(kv_load_kernel<128, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<128, BITS, 1>, d, st, a);
-  }
-  return d.wide ? launch_with_pdl(kv_load_kernel<256, BITS, 4>, d, st, a) : launch_with_pdl(kv_load_kernel<256, BITS, 1>, d, st, a);
+  return wide ? launch_with_pdl(kv_load_kernel<D, BITS, 4>, l, st, a) : launch_with_pdl(kv_load_kernel<D, BITS, 1>, l, st, a);
+}
+
+template <int BITS, bool STORE>
+int launch_copy(const char* who, const CopyArgs& a0, int D, cudaStream_t st) {
+  CopyArgs a = a0;
+  Launch l;
+  const bool wide = is_wide(a.M, 2 * a.kv.kv_heads, D);
+  if (int rc = deal(who, a.M, 0, a.kv.kv_heads, true, wide ? 4 : 1, D, &a.deal, &l)) { return rc; }
+  if (D == 64) { return launch_copy_d<BITS, STORE, 64>(wide, l, st, a); }
+  if (D == 128) { return launch_copy_d<BITS, STORE, 128>(wide, l, st, a); }
+  return launch_copy_d<BITS, STORE, 256>(wide, l, st, a);
 }
 
 bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
@@ -578,45 +645,35 @@ extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const 
                                : launch_norm<16>(who, a, desc_host->head_dim, st);
 }
 
-extern "C" int vpq_kv_store_bf16(const vpq_kv_cache* cache_host, const void* k, const void* v, int64_t k_stride,
-                                 int64_t v_stride, const int64_t* slots, int64_t M, void* stream) {
-  const char* who = "kv_store";
+namespace {
+template <bool STORE>
+int copy_rows(const char* who, const vpq_kv_cache* c, const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+              const int64_t* slots, int64_t M, void* stream) {
   clear_error();
-  QkArgs a = {};
-  if (int rc = kv_check(who, cache_host, &a.kv)) { return rc; }
+  CopyArgs a = {};
+  if (int rc = kv_check(who, c, &a.kv)) { return rc; }
   if (M <= 0 || M > (int64_t)1 << 40) { return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < M <= 2^40 (M=%lld)", who, (long long)M); }
-  const int D = cache_host->head_dim, H = cache_host->kv_heads;
-  if (int rc = take_rows(who, "k", k, k_stride, H, D, M, &a.in_stride[1])) { return rc; }
-  if (int rc = take_rows(who, "v", v, v_stride, H, D, M, &a.in_stride[2])) { return rc; }
+  const int D = c->head_dim, H = c->kv_heads;
+  if (int rc = take_rows(who, STORE ? "k" : "k_out", k, k_stride, H, D, M, &a.stride[0])) { return rc; }
+  if (int rc = take_rows(who, STORE ? "v" : "v_out", v, v_stride, H, D, M, &a.stride[1])) { return rc; }
   if (int rc = take_slots(who, slots)) { return rc; }
-  a.in[1] = static_cast<const uint8_t*>(k);
-  a.in[2] = static_cast<const uint8_t*>(v);
-  a.heads[1] = a.heads[2] = H;
+  a.rows[0] = static_cast<uint8_t*>(const_cast<void*>(k));
+  a.rows[1] = static_cast<uint8_t*>(const_cast<void*>(v));
   a.slots = slots;
   a.M = M;
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache_host->bits == 8 ? launch_norm<8>(who, a, D, st) : launch_norm<16>(who, a, D, st);
+  return c->bits == 8 ? launch_copy<8, STORE>(who, a, D, st) : launch_copy<16, STORE>(who, a, D, st);
+}
+}  // namespace
+
+extern "C" int vpq_kv_store_bf16(const vpq_kv_cache* cache_host, const void* k, const void* v, int64_t k_stride,
+                                 int64_t v_stride, const int64_t* slots, int64_t M, void* stream) {
+  return copy_rows<true>("kv_store", cache_host, k, v, k_stride, v_stride, slots, M, stream);
 }
 
 extern "C" int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, int64_t k_stride,
                                 int64_t v_stride, const int64_t* slots, int64_t M, void* stream) {
-  const char* who = "kv_load";
-  clear_error();
-  LoadArgs a = {};
-  if (int rc = kv_check(who, cache_host, &a.kv)) { return rc; }
-  if (M <= 0 || M > (int64_t)1 << 40) { return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < M <= 2^40 (M=%lld)", who, (long long)M); }
-  const int D = cache_host->head_dim, H = cache_host->kv_heads;
-  if (int rc = take_rows(who, "k_out", k_out, k_stride, H, D, M, &a.stride[0])) { return rc; }
-  if (int rc = take_rows(who, "v_out", v_out, v_stride, H, D, M, &a.stride[1])) { return rc; }
-  if (int rc = take_slots(who, slots)) { return rc; }
-  a.out[0] = static_cast<uint8_t*>(k_out);
-  a.out[1] = static_cast<uint8_t*>(v_out);
-  a.slots = slots;
-  a.M = M;
-  a.num_slots = a.kv.num_pages * a.kv.page_size;
-  if (int rc = require_sm100()) { return rc; }
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache_host->bits == 8 ? launch_load<8>(who, a, D, st) : launch_load<16>(who, a, D, st);
+  return copy_rows<false>("kv_load", cache_host, k_out, v_out, k_stride, v_stride, slots, M, stream);
 }

@@ -59,12 +59,14 @@ struct AttnArgs {
   CtaHead* heads;    // workspace: one per CTA
   float* ml;         // [CTA][2][cols][2]: maximum and sum of a partial result
   float* part;       // [CTA][2][cols][D]
-  float* scratch;    // [CTA][warp][cols][D]: a warp's first partial result, if another run follows it
+  float* scratch;    // [CTA][warp][cols][D]: a warp's first partial result, if another run follows it; null: in
+                     // shared memory behind the rings
   int batch, max_pages, window;
   int group;         // query heads of a key head
   int cols;          // query heads a unit serves (a column block): min(group, 8 NT)
   int blocks;        // column blocks of a key head
   int hk;            // kv_heads * blocks
+  bool few;          // at most 32 sequences, and few enough units for 32-bit sums
   float scale_log2;
   int stage_bytes, ring_bytes;  // shared memory: a stage, a warp's ring
 };
@@ -162,6 +164,12 @@ __device__ __forceinline__ void lds_pairs(uint32_t (&p)[G], uint32_t a) {
     p[0] = w.x, p[G > 1 ? 1 : 0] = w.y, p[G > 2 ? 2 : 0] = w.z, p[G > 3 ? 3 : 0] = w.w;
   }
 }
+// Where value d of column col lies in its row of a warp's partial result: the 32 lanes that store
+// together fall into 32 banks.
+template <int BITS>
+__device__ __forceinline__ int entry_at(int col, int d) {
+  return BITS == 16 ? d ^ ((col & 6) << 2) : d ^ ((col >> 1) & 3) ^ ((d >> 3) & 4);
+}
 // The factor that takes a partial result (maximum m, sum l) to the joint maximum; one without a live token
 // counts nothing, unless it holds a NaN.
 __device__ __forceinline__ float weight_of(float m, float l, float joint) {
@@ -200,12 +208,13 @@ struct alignas(16) UnitMeta {
 };
 enum : int { kFirst = 1 << 16, kLast = 2 << 16, kSegBegin = 4 << 16 };
 
-// A partial result of a warp: its numbers are at `data` (the warp's ring, or its scratch in the workspace).
+// A partial result of a warp. It has room for two: of its first run, if others follow, in the workspace,
+// and of its last run, over its ring.
 struct EntryHead {
-  const float* data;
   int b, h;     // b -1: none
   int begins;   // from the first token on
   int rest;     // as UnitMeta, of its last unit
+  int leads;    // the first of the CTA's line
   float m[16], l[16];
 };
 
@@ -221,9 +230,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_excl[kWarps * 32];
+  __shared__ int2 s_range[kWarps * 32];
   __shared__ int64_t s_wsum[kWarps];
   __shared__ UnitMeta s_meta[kWarps][STAGES];
   __shared__ EntryHead s_entry[kWarps * 2];
+  __shared__ float s_f[kWarps * 2][16], s_fl[kWarps * 2][16];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -231,34 +242,50 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this CTA's run of the line of units
-  const int cpt = (A.batch + kWarps * 32 - 1) / (kWarps * 32);
-  const int b_lo = min(tid * cpt, A.batch), b_hi = min(b_lo + cpt, A.batch);
-  int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) {
-    int s, n;
-    token_range(A, b, s, n);
-    mine += units_of<kUnit>(s, n);
-    if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > n) { atomicOr(&g_attn_status, kBadLength); }
-  }
-  int64_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) { incl += o; }
-  }
-  if (lane == 31) { s_wsum[warp] = incl; }
-  if (tid < kWarps * 2) { s_entry[tid].b = -1; }
+  // ---- this CTA's run of the line of units. Up to 32 sequences: every warp looks at all of them; more: a
+  // thread at a few neighbouring ones each.
+  if (lane < 2) { s_entry[warp * 2 + lane].b = -1; }
   if (tid == 0) { A.heads[blockIdx.x].last = -1; }
-  __syncthreads();
-  int64_t base = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) { base += s_wsum[w]; }
-    total += s_wsum[w];
+  const int cpt = A.few ? 1 : (A.batch + kWarps * 32 - 1) / (kWarps * 32);
+  const int me = A.few ? lane : tid;
+  const int b_lo = min(me * cpt, A.batch), b_hi = min(b_lo + cpt, A.batch);
+  int64_t mine = 0;
+  int2 seen = make_int2(0, 0);  // token range of the last of them
+  for (int b = b_lo; b < b_hi; ++b) {
+    token_range(A, b, seen.x, seen.y);
+    mine += units_of<kUnit>(seen.x, seen.y);
+    if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(&g_attn_status, kBadLength); }
   }
-  s_excl[tid] = base + incl - mine;
-  __syncthreads();
+  int64_t excl, total;  // units (of one head) before the first of them, and of all
+  if (A.few) {
+    int incl = (int)mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) { incl += o; }
+    }
+    excl = incl - (int)mine;
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    int64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) { incl += o; }
+    }
+    if (lane == 31) { s_wsum[warp] = incl; }
+    __syncthreads();
+    excl = incl - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) { excl += s_wsum[w]; }
+      total += s_wsum[w];
+    }
+    s_excl[tid] = excl;
+    s_range[tid] = seen;
+    __syncthreads();
+  }
   const int64_t units = total * A.hk;
   int64_t per_cta = div_u(units + gridDim.x - 1, gridDim.x);
   per_cta = per_cta > kWarps ? per_cta : kWarps;
@@ -293,21 +320,34 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     }
   };
   if (left > 0) {
-    int lo = 0, hi = kWarps * 32 - 1;
-    while (lo < hi) {  // the last thread whose sequences begin at or before u0
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_excl[mid] * A.hk <= u0) {
-        lo = mid;
-      } else {
-        hi = mid - 1;
+    // who looked at u0's sequence: the last whose sequences begin at or before it
+    int64_t at;
+    if (A.few) {
+      lb = 31 - __clz(__ballot_sync(0xffffffffu, excl * A.hk <= u0));
+      at = __shfl_sync(0xffffffffu, excl, lb);
+      lstart = __shfl_sync(0xffffffffu, seen.x, lb), llen = __shfl_sync(0xffffffffu, seen.y, lb);
+    } else {
+      int64_t upto = 0;
+      int tw = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (upto * A.hk <= u0) { tw = w; }
+        upto += s_wsum[w];
       }
-    }
-    int64_t at = s_excl[lo];
-    for (lb = lo * cpt;; ++lb) {
-      token_range(A, lb, lstart, llen);
-      const int n = units_of<kUnit>(lstart, llen);
-      if ((at + n) * A.hk > u0) { break; }
-      at += n;
+      const int64_t ex = s_excl[tw * 32 + lane];
+      const int tl = 31 - __clz(__ballot_sync(0xffffffffu, ex * A.hk <= u0));
+      at = __shfl_sync(0xffffffffu, ex, tl);
+      lb = (tw * 32 + tl) * cpt;
+      if (cpt == 1) {
+        lstart = s_range[tw * 32 + tl].x, llen = s_range[tw * 32 + tl].y;
+      } else {
+        for (;; ++lb) {
+          token_range(A, lb, lstart, llen);
+          const int n = units_of<kUnit>(lstart, llen);
+          if ((at + n) * A.hk > u0) { break; }
+          at += n;
+        }
+      }
     }
     ltile0 = lstart / kUnit;
     ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
@@ -321,6 +361,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   }
 
   uint8_t* ring = smem + warp * A.ring_bytes;
+  float* scratch0 = A.scratch ? A.scratch + (int64_t)blockIdx.x * kWarps * (A.cols * D)
+                              : reinterpret_cast<float*>(smem + kWarps * A.ring_bytes);
   const uint32_t ring_s = smem_u32(ring);
   constexpr int CH = kRow / 16;                      // 16-byte chunks of a row
   constexpr int kRowsPer = CH < 32 ? 32 / CH : 1;    // rows that one round of the warp's copies covers
@@ -793,22 +835,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
         }
       } else {
-        // At most two per warp: the first part of its run and the last. When nothing more is requested the
-        // ring is free for it; a first part that is followed by other runs goes to the workspace.
         const bool done = todo == 1;
-        EntryHead& H = s_entry[warp * 2 + (first_run ? 0 : 1)];
-        float* to = done ? reinterpret_cast<float*>(ring)
-                         : A.scratch + ((int64_t)blockIdx.x * kWarps + warp) * (A.cols * D);
+        EntryHead& H = s_entry[warp * 2 + done];
+        float* to = done ? reinterpret_cast<float*>(ring) : scratch0 + warp * (A.cols * D);
         if (done) {
           cp_wait<0>();
           __syncwarp();
         }
         if (lane == 0) {
-          H.data = to;
           H.b = U.b;
           H.h = U.h;
           H.begins = run_begins;
           H.rest = U.rest;
+          H.leads = warp == 0 && first_run;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -825,7 +864,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const int d = BITS == 16 ? 16 * i + 8 * h + r : 64 * (i / 4) + 8 * r + 2 * (i % 4) + h;
-                  to[col * D + d] = o_acc[n][i][2 * h + c];
+                  to[col * D + entry_at<BITS>(col, d)] = o_acc[n][i][2 * h + c];
                 }
               }
             }
@@ -837,58 +876,95 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     st = st + 1 == STAGES ? 0 : st + 1;
   }
 
-  // ---- join the warps' partial results, in the line's order
+  // ---- join the warps' partial results, in the line's order. A warp takes a column: lane j holds entry j's
+  // maximum and sum, the lanes of one (sequence, head) find their joint maximum together.
   cp_wait<0>();
   __syncthreads();
-  for (int item = warp; item < kWarps * 2 * A.cols; item += kWarps) {
-    const int n = item / A.cols, col = item % A.cols;
+  const int my_b = lane < kWarps * 2 ? s_entry[lane].b : -1, my_h = lane < kWarps * 2 ? s_entry[lane].h : 0;
+  const uint32_t valid = __ballot_sync(0xffffffffu, my_b >= 0);
+  const uint32_t run = __match_any_sync(0xffffffffu, ((uint64_t)(uint32_t)my_b << 32) | (uint32_t)my_h) & valid;
+  const uint32_t leaders = __ballot_sync(0xffffffffu, my_b >= 0 && (run & ((1u << lane) - 1)) == 0);
+  for (int col = warp; col < A.cols; col += kWarps) {
+    if (my_b >= 0) {
+      const float mj = s_entry[lane].m[col], lj = s_entry[lane].l[col];
+      int key = __float_as_int(mj);  // an order of integers that is the numbers' order
+      key = key < 0 ? key ^ 0x7fffffff : key;
+      key = __reduce_max_sync(run, key);
+      const float joint = __int_as_float(key < 0 ? key ^ 0x7fffffff : key);
+      const float f = weight_of(mj, lj, joint);
+      s_f[lane][col] = f;
+      s_fl[lane][col] = f * lj;
+      s_entry[lane].m[col] = joint;
+    }
+  }
+  __syncthreads();
+  // The leaders' sums are dealt over groups of warps.
+  const int count = __popc(leaders);
+  const int share = count > 0 && count < kWarps ? kWarps / count : 1;  // warps of a leader
+  const int gt = (warp % share) * 32 + lane;
+  for (int li = warp / share; li < count; li += kWarps / share) {
+    uint32_t later = leaders;
+    for (int k = 0; k < li; ++k) { later &= later - 1; }
+    const int n = __ffs(later) - 1;
+    const uint32_t members = __shfl_sync(0xffffffffu, run, n);
     const EntryHead& H = s_entry[n];
-    if (H.b < 0) { continue; }
-    const int blk = H.h % A.blocks;
-    if (col >= min(A.cols, A.group - blk * A.cols)) { continue; }
-    auto same = [&](const EntryHead& x) { return x.b == H.b && x.h == H.h; };
-    int prev = n - 1;
-    while (prev >= 0 && s_entry[prev].b < 0) { --prev; }
-    if (prev >= 0 && same(s_entry[prev])) { continue; }  // another item joins it
-    int end = n;
-    float m = kNegInf;
-    for (int j = n; j < kWarps * 2; ++j) {
-      if (s_entry[j].b < 0) { continue; }
-      if (!same(s_entry[j])) { break; }
-      end = j;
-      m = fmaxf(m, s_entry[j].m[col]);
-    }
-    float l = 0.0f, acc[D / 32];
+    const int rest = s_entry[31 - __clz(members)].rest;
+    const int kvh = H.h / A.blocks, blk = H.h - kvh * A.blocks;
+    const int ncol = min(A.cols, A.group - blk * A.cols);
+    const bool whole = H.begins && rest == 0;
+    const int head0 = kvh * A.group + blk * A.cols;
+    __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head0 * D;
+    // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: another, which it ends in
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (H.leads ? 0 : 1);
+    for (int i = gt; i < ncol * (D / 4); i += share * 32) {  // four values of a column
+      const int col = i / (D / 4), d = (i % (D / 4)) * 4;
+      const int at = col * (D / 4) + (entry_at<BITS>(col, d) >> 2);
+      auto of = [&](int j) {
+        return reinterpret_cast<const float4*>((j & 1) ? reinterpret_cast<const float*>(smem + (j >> 1) * A.ring_bytes)
+                                                       : scratch0 + (j >> 1) * (A.cols * D))[at];
+      };
+      float l = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      auto add = [&](float f, float fl, const float4& x) {
+        l += fl;
+        acc.x = __fmaf_rn(f, x.x, acc.x), acc.y = __fmaf_rn(f, x.y, acc.y);
+        acc.z = __fmaf_rn(f, x.z, acc.z), acc.w = __fmaf_rn(f, x.w, acc.w);
+      };
+      uint32_t k = members;
+      for (; __popc(k) >= 4;) {  // four loads in flight
+        int j[4];
+        float4 x[4];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
-    for (int j = n; j <= end; ++j) {
-      if (s_entry[j].b < 0) { continue; }
-      const float f = weight_of(s_entry[j].m[col], s_entry[j].l[col], m);
-      l = __fmaf_rn(f, s_entry[j].l[col], l);
-      const float* from = s_entry[j].data + col * D + lane;
+        for (int e = 0; e < 4; ++e) {
+          j[e] = __ffs(k) - 1;
+          k &= k - 1;
+          x[e] = of(j[e]);
+        }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f, from[i * 32], acc[i]); }
-    }
-    const int rest = s_entry[end].rest;
-    if (H.begins && rest == 0) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int head = (H.h / A.blocks) * A.group + blk * A.cols + col;
-      __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head * D;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) { op[i * 32 + lane] = __float2bfloat16_rn(acc[i] * inv); }
-    } else {
-      // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: another, which it ends in
-      const int64_t slot = (int64_t)blockIdx.x * 2 + (n == 0 ? 0 : 1);
-      float* pp = A.part + (slot * A.cols + col) * D;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) { pp[i * 32 + lane] = acc[i]; }
-      if (lane == 0) {
-        A.ml[(slot * A.cols + col) * 2] = m;
-        A.ml[(slot * A.cols + col) * 2 + 1] = l;
-        if (H.begins && col == 0) {
-          A.heads[blockIdx.x] = {H.b, H.h, n == 0 ? 0 : 1, (int)div_u(cta1 + rest - 1, per_cta)};
+        for (int e = 0; e < 4; ++e) { add(s_f[j[e]][col], s_fl[j[e]][col], x[e]); }
+      }
+      for (; k != 0; k &= k - 1) {
+        const int j = __ffs(k) - 1;
+        add(s_f[j][col], s_fl[j][col], of(j));
+      }
+      if (BITS == 8) {  // entry_at exchanges values within the four
+        if (col & 2) { acc = make_float4(acc.y, acc.x, acc.w, acc.z); }
+        if (col & 4) { acc = make_float4(acc.z, acc.w, acc.x, acc.y); }
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint2*>(op + i * 4) =
+            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(A.part + slot * A.cols * D + i * 4) = acc;
+        if (d == 0) {
+          A.ml[(slot * A.cols + col) * 2] = H.m[col];
+          A.ml[(slot * A.cols + col) * 2 + 1] = l;
         }
       }
+    }
+    if (!whole && H.begins && gt == 0) {
+      A.heads[blockIdx.x] = {H.b, H.h, H.leads ? 0 : 1, (int)div_u(cta1 + rest - 1, per_cta)};
     }
   }
 }
@@ -913,20 +989,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // A warp's first part is fetched together with the record that says whether there is one (whatever lies
+  // there is inside the workspace); the record's own CTA may have it in slot 1.
+  float m1, l1, x[D / 32];
+  auto fetch = [&](int64_t slot) {
+    m1 = A.ml[slot * 2];
+    l1 = A.ml[slot * 2 + 1];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) { x[i] = A.part[slot * D + i * 32 + lane]; }
+  };
+  fetch((int64_t)min(c0 + warp, (int)gridDim.x - 1) * 2 * A.cols + col);
   const CtaHead H = A.heads[c0];
   if (H.last < 0) { return; }
   const int blk = H.h % A.blocks;
   if (col >= min(A.cols, A.group - blk * A.cols)) { return; }
+  if (warp == 0 && H.slot == 1) { fetch(((int64_t)c0 * 2 + 1) * A.cols + col); }
   float m = kNegInf, l = 0.0f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
   for (int c = c0 + warp; c <= H.last; c += kJoinWarps) {
-    const int64_t slot = ((int64_t)c * 2 + (c == c0 ? H.slot : 0)) * A.cols + col;
-    const float mj = A.ml[slot * 2], lj = A.ml[slot * 2 + 1];
-    const float* pp = A.part + slot * D + lane;
-    float x[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) { x[i] = pp[i * 32]; }
+    if (c != c0 + warp) { fetch((int64_t)c * 2 * A.cols + col); }
+    const float mj = m1, lj = l1;
     const float m2 = fmaxf(m, mj);
     const float f0 = weight_of(m, l, m2), f1 = weight_of(mj, lj, m2);
     m = m2;
@@ -992,13 +1075,18 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   static_assert(kWarps <= kMaxWarps, "the workspace is sized for kMaxWarps");
   static_assert(NT * 8 * D * 4 <= STAGES * 2 * 16 * TM * (D * BITS / 8), "a warp's partial result fits its ring");
   constexpr int kStage = 2 * 16 * TM * (D * BITS / 8) + (BITS == 8 ? 2 * 16 * TM * (D / kKvGroup) * 4 : 0);
-  static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= 220 * 1024, "rings fit beside the static shared memory");
+  static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= 216 * 1024, "rings fit beside the static shared memory");
   AttnArgs a = a0;
   a.stage_bytes = kStage + ((s.cols * D * 2 + 127) & ~127);
   a.ring_bytes = a.stage_bytes * STAGES;
   static int granted[64] = {};
   auto kern = paged_attn_kernel<D, BITS, NT, TM, kWarps, STAGES>;
-  const size_t smem = (size_t)kWarps * a.ring_bytes;
+  size_t smem = (size_t)kWarps * a.ring_bytes;
+  const size_t first = (size_t)kWarps * s.cols * D * 4;
+  if (smem + first <= 216 * 1024) {
+    smem += first;
+    a.scratch = nullptr;
+  }
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), granted, smem)) { return rc; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)s.ctas, 1, 1);
@@ -1094,6 +1182,7 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   a.cols = s.cols;
   a.blocks = s.blocks;
   a.hk = cache_host->kv_heads * s.blocks;
+  a.few = d.batch <= 32 && (int64_t)d.max_pages * cache_host->page_size <= INT_MAX / 4;
   const float scale = d.scale != 0.0f ? d.scale : 1.0f / sqrtf((float)cache_host->head_dim);
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
