@@ -7,7 +7,7 @@
 //
 // Work split. The unit is 16 or 32 tokens of one (sequence, key head). All units of a call, in the order
 // (sequence, head, tokens), form one line that is cut into equal runs, one per CTA, and a CTA's run into one per
-// warp: no SM waits for a long sequence, whatever the lengths, and the lengths are read on the device, so a
+// warp (every (sequence, head) counts one unit more than it has, for its start and its end): no SM waits for a long sequence, whatever the lengths, and the lengths are read on the device, so a
 // captured graph serves any of them. Each warp streams its run through its own ring in shared memory
 // (cp.async, no barrier in the loop). What a warp has of a (sequence, head) that it shares with others is
 // joined within the CTA through shared memory, and across CTAs by a second small kernel over partial
@@ -43,9 +43,10 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // What the joining kernel has to know of a CTA: the (sequence, head) that begins in its run and goes on in
-// the next CTA's, where its partial result is (0: the run's first, 1), and the last CTA that has a part.
+// the next CTA's (its first query head, and how many), where its partial result is (0: the run's first, 1), and
+// the last CTA that has a part.
 struct CtaHead {
-  int b, h, slot, last;  // last -1: none
+  int b, h, ncol_slot, last;  // ncol << 1 | slot; last -1: none
 };
 
 struct AttnArgs {
@@ -188,6 +189,12 @@ template <int U>
 __device__ __forceinline__ int units_of(int start, int len) {
   return len > start ? (len + U - 1) / U - start / U : 0;
 }
+// Its length on the line, per head: one place for the start and the end of a (sequence, head), then its units.
+template <int U>
+__device__ __forceinline__ int span_of(int start, int len) {
+  const int n = units_of<U>(start, len);
+  return n > 0 ? n + 1 : 0;
+}
 
 // Where 16-byte chunk c of row `row` lies in a K or V tile. 16 bits: the eight rows that an ldmatrix
 // reads fall into eight bank groups. 8 bits: see the loads in the loop.
@@ -202,8 +209,8 @@ __device__ __forceinline__ int swz_v(int row, int c) {
 
 // What a unit in flight is: written by lane 0 with its copies, read when its turn comes.
 struct alignas(16) UnitMeta {
-  int b, h;       // sequence; key head * blocks + column block
-  int bits;       // live rows [lo, hi): lo | hi << 8, flags << 16
+  int b, h;       // sequence; first query head of the column block
+  int bits;       // live rows [lo, hi): lo | hi << 8, flags << 16, columns << 24
   int rest;       // units of this (sequence, head) behind this one
 };
 enum : int { kFirst = 1 << 16, kLast = 2 << 16, kSegBegin = 4 << 16 };
@@ -215,6 +222,7 @@ struct EntryHead {
   int begins;   // from the first token on
   int rest;     // as UnitMeta, of its last unit
   int leads;    // the first of the CTA's line
+  int ncol;
   float m[16], l[16];
 };
 
@@ -253,10 +261,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   int2 seen = make_int2(0, 0);  // token range of the last of them
   for (int b = b_lo; b < b_hi; ++b) {
     token_range(A, b, seen.x, seen.y);
-    mine += units_of<kUnit>(seen.x, seen.y);
+    mine += span_of<kUnit>(seen.x, seen.y);
     if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(&g_attn_status, kBadLength); }
   }
-  int64_t excl, total;  // units (of one head) before the first of them, and of all
+  int64_t excl, total;  // places (of one head) before the first of them, and of all
   if (A.few) {
     int incl = (int)mine;
 #pragma unroll
@@ -286,17 +294,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     s_range[tid] = seen;
     __syncthreads();
   }
-  const int64_t units = total * A.hk;
-  int64_t per_cta = div_u(units + gridDim.x - 1, gridDim.x);
+  const int64_t places = total * A.hk;
+  int64_t per_cta = div_u(places + gridDim.x - 1, gridDim.x);
   per_cta = per_cta > kWarps ? per_cta : kWarps;
   const int64_t cta0 = (int64_t)blockIdx.x * per_cta;
-  if (cta0 >= units) { return; }  // the whole CTA
-  const int64_t cta1 = cta0 + per_cta < units ? cta0 + per_cta : units;
+  if (cta0 >= places) { return; }  // the whole CTA
+  const int64_t cta1 = cta0 + per_cta < places ? cta0 + per_cta : places;
   const int64_t per_warp = (cta1 - cta0 + kWarps - 1) / kWarps;
   const int64_t u0 = cta0 + warp * per_warp;
   const int64_t u1 = u0 + per_warp < cta1 ? u0 + per_warp : cta1;
-  int left = u0 < u1 ? (int)(u1 - u0) : 0;  // units this warp has yet to request
-  int todo = left;                          // and to compute
+  int left = u0 < u1 ? (int)(u1 - u0) : 0;  // places of the line that this warp has yet to request
+  int todo = 0;                             // units requested and not yet computed
 
   // ---- the loader's place in the line
   int lb = 0, lh = 0, lkv = 0, lblk = 0, ltile = 0, ltile0 = 0, ltile_end = 0, lstart = 0, llen = 0;
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       } else {
         for (;; ++lb) {
           token_range(A, lb, lstart, llen);
-          const int n = units_of<kUnit>(lstart, llen);
+          const int n = span_of<kUnit>(lstart, llen);
           if ((at + n) * A.hk > u0) { break; }
           at += n;
         }
@@ -352,12 +360,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     ltile0 = lstart / kUnit;
     ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
     const int64_t in_seq = u0 - at * A.hk;
-    lh = (int)div_u(in_seq, ltile_end - ltile0);
-    ltile = ltile0 + (int)(in_seq - (int64_t)lh * (ltile_end - ltile0));
+    const int span = ltile_end - ltile0 + 1;
+    lh = (int)div_u(in_seq, span);
+    const int place = (int)(in_seq - (int64_t)lh * span);
+    ltile = ltile0 + (place > 0 ? place - 1 : 0);
+    if (place == 0) { --left; }
     lkv = lh / A.blocks;
     lblk = lh - lkv * A.blocks;
-    enter();
-    fetch_pages();
+    if (left > 0) {
+      enter();
+      fetch_pages();
+    }
   }
 
   uint8_t* ring = smem + warp * A.ring_bytes;
@@ -418,22 +431,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           hi = max(min(hi, 16), lo);
         }
       }
+      const int h0 = lkv * A.group + lblk * A.cols;
+      const int ncol = min(A.cols, A.group - lblk * A.cols);
       if (fresh) {
-        const int h0 = lkv * A.group + lblk * A.cols;
-        const int n = min(A.cols, A.group - lblk * A.cols);
         const uint8_t* qp = A.q + (int64_t)lb * A.q_stride + (int64_t)h0 * (D * 2);
-        for (int i = lane; i < n * (D / 8); i += 32) { cp_async16(dst + 2 * kTile + 2 * kPairs + i * 16, qp + i * 16, true); }
+        for (int i = lane; i < ncol * (D / 8); i += 32) { cp_async16(dst + 2 * kTile + 2 * kPairs + i * 16, qp + i * 16, true); }
       }
       const int rest = ltile_end - 1 - ltile;
       if (lane == 0) {
-        s_meta[warp][st] = {lb, lh,
-                            lo | (hi << 8) | (fresh ? kFirst : 0) | ((left == 1 || rest == 0) ? kLast : 0) |
+        s_meta[warp][st] = {lb, h0,
+                            lo | (hi << 8) | (ncol << 24) | (fresh ? kFirst : 0) | ((left == 1 || rest == 0) ? kLast : 0) |
                                 (ltile == ltile0 ? kSegBegin : 0),
                             rest};
       }
+      ++todo;
       --left;
       fresh = false;
       ++ltile;
+      if (left > 0 && rest == 0) { --left; }
       if (left > 0) {
         if (rest == 0) {
           fresh = true;
@@ -476,8 +491,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
                    qt = vsc + kPairs;
 
     if (U.bits & kFirst) {
-      const int blk = U.h % A.blocks;
-      const int ncol = min(A.cols, A.group - blk * A.cols);
+      const int ncol = U.bits >> 24;
       run_begins = (U.bits & kSegBegin) != 0;
       sigma = -100;
 #pragma unroll
@@ -773,8 +787,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 
     // ---- the warp's part of a (sequence, head) is complete
     if (U.bits & kLast) {
-      const int blk = U.h % A.blocks, kvh = U.h / A.blocks;
-      const int ncol = min(A.cols, A.group - blk * A.cols);
+      const int ncol = U.bits >> 24;
       const float o_mul = BITS == 8 ? __uint_as_float((uint32_t)(sigma - 15 + 127) << 23) : 1.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -800,7 +813,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         }
       }
       if (run_begins && U.rest == 0) {
-        uint8_t* op = A.out + (int64_t)U.b * A.out_stride + (int64_t)(kvh * A.group + blk * A.cols) * (D * 2);
+        uint8_t* op = A.out + (int64_t)U.b * A.out_stride + (int64_t)U.h * (D * 2);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // a sum of 0: no live token (a NaN stays one)
@@ -848,6 +861,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           H.begins = run_begins;
           H.rest = U.rest;
           H.leads = warp == 0 && first_run;
+          H.ncol = ncol;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -898,25 +912,21 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     }
   }
   __syncthreads();
-  // The leaders' sums are dealt over groups of warps.
-  const int count = __popc(leaders);
-  const int share = count > 0 && count < kWarps ? kWarps / count : 1;  // warps of a leader
-  const int gt = (warp % share) * 32 + lane;
-  for (int li = warp / share; li < count; li += kWarps / share) {
-    uint32_t later = leaders;
-    for (int k = 0; k < li; ++k) { later &= later - 1; }
+  // One (sequence, head) alone: all warps add it up; several: a warp each.
+  const bool alone = (leaders & (leaders - 1)) == 0;
+  const int gt = alone ? tid : lane, gn = alone ? kWarps * 32 : 32;
+  uint32_t later = leaders;
+  for (int turn = 0; later != 0; ++turn, later &= later - 1) {
+    if (!alone && turn % kWarps != warp) { continue; }
     const int n = __ffs(later) - 1;
     const uint32_t members = __shfl_sync(0xffffffffu, run, n);
     const EntryHead& H = s_entry[n];
-    const int rest = s_entry[31 - __clz(members)].rest;
-    const int kvh = H.h / A.blocks, blk = H.h - kvh * A.blocks;
-    const int ncol = min(A.cols, A.group - blk * A.cols);
+    const int rest = s_entry[31 - __clz(members)].rest, ncol = H.ncol;
     const bool whole = H.begins && rest == 0;
-    const int head0 = kvh * A.group + blk * A.cols;
-    __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head0 * D;
+    __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)H.h * D;
     // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: another, which it ends in
     const int64_t slot = (int64_t)blockIdx.x * 2 + (H.leads ? 0 : 1);
-    for (int i = gt; i < ncol * (D / 4); i += share * 32) {  // four values of a column
+    for (int i = gt; i < ncol * (D / 4); i += gn) {  // four values of a column
       const int col = i / (D / 4), d = (i % (D / 4)) * 4;
       const int at = col * (D / 4) + (entry_at<BITS>(col, d) >> 2);
       auto of = [&](int j) {
@@ -964,7 +974,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       }
     }
     if (!whole && H.begins && gt == 0) {
-      A.heads[blockIdx.x] = {H.b, H.h, H.leads ? 0 : 1, (int)div_u(cta1 + rest - 1, per_cta)};
+      A.heads[blockIdx.x] = {H.b, H.h, ncol * 2 + (H.leads ? 0 : 1), (int)div_u(cta1 + rest - 1, per_cta)};
     }
   }
 }
@@ -1000,10 +1010,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
   };
   fetch((int64_t)min(c0 + warp, (int)gridDim.x - 1) * 2 * A.cols + col);
   const CtaHead H = A.heads[c0];
-  if (H.last < 0) { return; }
-  const int blk = H.h % A.blocks;
-  if (col >= min(A.cols, A.group - blk * A.cols)) { return; }
-  if (warp == 0 && H.slot == 1) { fetch(((int64_t)c0 * 2 + 1) * A.cols + col); }
+  if (H.last < 0 || col >= (H.ncol_slot >> 1)) { return; }
+  if (warp == 0 && (H.ncol_slot & 1)) { fetch(((int64_t)c0 * 2 + 1) * A.cols + col); }
   float m = kNegInf, l = 0.0f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
@@ -1031,8 +1039,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
     sum = __fmaf_rn(f, s_l[w], sum);
     o = __fmaf_rn(f, s_acc[w][threadIdx.x], o);
   }
-  const int head = (H.h / A.blocks) * A.group + blk * A.cols + col;
-  __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)head * D;
+  __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)(H.h + col) * D;
   op[threadIdx.x] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : o / sum);
 }
 
