@@ -3,6 +3,7 @@
 // instructions per 16 bytes, each row read once and written once.
 #include "vpq_kv.cuh"
 
+#include <algorithm>
 #include <climits>
 
 namespace vpq {
@@ -11,26 +12,29 @@ __device__ uint32_t g_kv_status = 0;
 
 namespace {
 
-// How a token's heads are dealt: every part (q, k, v) is cut into chunks of HPT neighbouring heads, and one
-// lane group takes a chunk. A block holds the chunks of `tokens` whole tokens, or one token's chunks are spread
-// evenly over `token_blocks` blocks.
+// How rows are dealt: a block belongs to one part (q, k or v; so what goes by the part is the same for all its
+// threads), whose heads are cut into chunks of HPT neighbours; a lane group takes one chunk of every `step`-th
+// token. A block holds the chunks of `tokens` whole tokens, or one token's chunks are spread evenly over
+// `token_blocks` blocks.
 struct Deal {
-  int qc, kc;        // chunks of q, and of k (of v as many)
+  uint32_t first;    // the part's first block
   int chunks;        // of a token
   int per_block;     // of a token in a block
   int tokens, token_blocks;
   uint32_t rcp;      // 2^16 / per_block, rounded up: (g * rcp) >> 16 = g / per_block for g < 256
+  int64_t step;      // tokens that the part's blocks take at a time
 };
-// The calling lane group's token and chunk; false past the end (such lanes keep their warp's shuffles company).
+// The calling lane group's chunk, its first token and its block's; false if there is no chunk for it (such lanes
+// keep their warp's shuffles company).
 template <int LPH>
-__device__ __forceinline__ bool dealt(const Deal& d, int64_t M, int64_t& m, int& chunk) {
-  const uint32_t g = threadIdx.x / LPH;
-  const uint32_t tl = (g * d.rcp) >> 16;
-  const uint32_t tb = blockIdx.x / (uint32_t)d.token_blocks;
-  m = (int64_t)tb * d.tokens + tl;
-  chunk = (int)((blockIdx.x - tb * (uint32_t)d.token_blocks) * (uint32_t)d.per_block + (g - tl * d.per_block));
-  const bool in = (int)tl < d.tokens && m < M && chunk < d.chunks;
-  if (!in) { m = 0, chunk = 0; }
+__device__ __forceinline__ bool dealt(const Deal& d, int64_t& m0, int& tl, int& chunk) {
+  const uint32_t g = threadIdx.x / LPH, blk = blockIdx.x - d.first;
+  tl = (int)((g * d.rcp) >> 16);
+  const uint32_t tb = d.token_blocks == 1 ? blk : blk / (uint32_t)d.token_blocks;
+  m0 = (int64_t)tb * d.tokens;
+  chunk = (int)((blk - tb * (uint32_t)d.token_blocks) * (uint32_t)d.per_block + (g - tl * d.per_block));
+  const bool in = tl < d.tokens && chunk < d.chunks;
+  if (!in) { tl = chunk = 0; }
   return in;
 }
 
@@ -48,7 +52,7 @@ struct QkArgs {
   const int64_t* slots;
   int64_t M, table_rows, num_slots;
   int heads[3];
-  Deal deal;
+  Deal deal[3];
   int rot, interleaved;
   float eps, inv_d;
   KvView kv;
@@ -77,12 +81,36 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-// The 8-bit quantizer over the 64 values of eight lanes. The bias is the minimum rounded DOWN to
-// bf16 and the scale is rounded UP, so min and max both lie inside the code range: with nearest rounding a group
-// whose offset is large against its spread would lose values to clipping (the bias alone is off by
-// up to 2^-9 of the offset). The scale's floor of 2^-126 keeps its reciprocal finite; a group of
-// equal values takes code 0. A NaN or infinity among the 64 (or a spread beyond the largest float) makes the
-// pair NaN, so the group reads back as NaN.
+// The 8-bit quantizer over the 64 values of eight lanes, from their extremes. The bias is the minimum rounded
+// DOWN to bf16 and the scale is rounded UP, so min and max both lie inside the code range: with nearest rounding a
+// group whose offset is large against its spread would lose values to clipping (the bias alone is off by up to 2^-8
+// of the offset). The scale's floor of 2^-126 keeps its reciprocal finite; a group of equal values takes code 0. A
+// NaN or infinity among the 64 (or a spread beyond the largest float) makes the pair NaN, so the group reads back as
+// NaN. Directed rounding to bf16 is integer arithmetic on the bits; the quotient by 255 is rounded up exactly: a
+// product with a factor a little above 1 / 255 is cut to bf16, and the next number up is taken if 255 times that
+// (exact: 8 bits times 8) falls short.
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], float mn, float mx, uint32_t& pair) {
+  const uint32_t mb = __float_as_uint(mn);
+  const uint32_t bb = (mb + ((uint32_t)((int32_t)mb >> 31) & 0xffffu)) & 0xffff0000u;
+  const float b = __uint_as_float(bb);
+  const float range = __fsub_rn(mx, b);
+  const float cut = __uint_as_float(__float_as_uint(__fmul_rn(range, 0.0039215696f)) & 0xffff0000u);  // (1 + 2^-22) / 255
+  const uint32_t up = __fmul_rn(cut, 255.0f) >= range ? 0u : 0x10000u;
+  const float s = fmaxf(__uint_as_float(__float_as_uint(cut) + up), 1.17549435e-38f);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within one step; s and 1 / s are normal numbers
+  pair = range <= 3.402823466e38f ? (__float_as_uint(s) >> 16) | bb : 0x7fff7fffu;  // false for NaN
+  // Adding 2^23 rounds to an integer, ties to even, and leaves it in the low byte: b <= x and the rounded-up
+  // scale keep the quotient in [0, 255.0002], so there is nothing to clamp.
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { c[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[i], b), inv), 8388608.0f)); }
+  auto four = [](uint32_t a, uint32_t b2, uint32_t c2, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b2, 0x0040), __byte_perm(c2, d, 0x0040), 0x5410);
+  };
+  return make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
+}
+// The extremes of f32 values.
 __device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
   float mn = x[0], mx = x[0];
 #pragma unroll
@@ -95,149 +123,168 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], uint32_t& pair) {
     mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, d));
     mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, d));
   }
-  const __nv_bfloat16 b16 = __float2bfloat16_rd(mn);
-  const float b = __bfloat162float(b16);
-  const float range = __fsub_rn(mx, b);
-  const __nv_bfloat16 s16 = __float2bfloat16_ru(fmaxf(__fdiv_rn(range, 255.0f), 1.17549435e-38f));
-  const float inv = __frcp_rn(__bfloat162float(s16));
-  const bool fine = range <= 3.402823466e38f;  // false for NaN
-  pair = fine ? ((uint32_t)__bfloat16_as_ushort(s16) | ((uint32_t)__bfloat16_as_ushort(b16) << 16)) : 0x7fff7fffu;
-  // Adding 2^23 rounds to an integer, ties to even, and leaves it in the low byte: b <= x and the rounded-up
-  // scale keep the quotient in [0, 255.0001], so there is nothing to clamp.
-  uint32_t c[8];
+  return quant8(x, mn, mx, pair);
+}
+// Values that are bf16 already: extremes two at a time, then (minimum, -maximum) as one word.
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint2 quant8(const uint4 raw, uint32_t& pair) {
+  constexpr uint32_t kSign = 0x80008000u;
+  const uint32_t lo = min_nan2(min_nan2(raw.x, raw.y), min_nan2(raw.z, raw.w));
+  const uint32_t hi = min_nan2(min_nan2(raw.x ^ kSign, raw.y ^ kSign), min_nan2(raw.z ^ kSign, raw.w ^ kSign));
+  uint32_t m = min_nan2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[i], b), inv), 8388608.0f)); }
-  auto four = [](uint32_t a, uint32_t b2, uint32_t c2, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b2, 0x0040), __byte_perm(c2, d, 0x0040), 0x5410);
-  };
-  return make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
+  for (int d = 1; d < 8; d <<= 1) { m = min_nan2(m, __shfl_xor_sync(0xffffffffu, m, d)); }
+  float x[8];
+  unpack8(raw, x);
+  return quant8(x, __uint_as_float(m << 16), -__uint_as_float(m & 0xffff0000u), pair);
 }
 
-__device__ __forceinline__ int64_t slot_page(int64_t slot, int page_size) {
+__device__ __forceinline__ int64_t slot_page(int64_t slot, const KvView& kv) {
+  if (kv.page_shift >= 0) { return slot >> kv.page_shift; }
   // a 64-bit division costs five times as much
-  return (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
+  return (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)kv.page_size) : slot / kv.page_size;
 }
 
 // MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads of a chunk, all
 // requested before the first is used; their table row, norm weights and addresses are fetched once.
 template <int D, int MODE, int HPT>
-__global__ void __launch_bounds__(256) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
+__global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
   constexpr int LPH = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int part = MODE && blockIdx.x >= A.deal[2].first ? 2 : (blockIdx.x >= A.deal[1].first ? 1 : 0);
+  const Deal& deal = A.deal[part];
   const int l = threadIdx.x % LPH, d0 = l * 8;
-  int64_t m;
-  int chunk;
-  const bool in_range = dealt<LPH>(A.deal, A.M, m, chunk);
-  const int part = chunk < A.deal.qc ? 0 : (MODE == 0 || chunk < A.deal.qc + A.deal.kc ? 1 : 2);
-  const int h0 = HPT * (chunk - (part == 0 ? 0 : (part == 1 ? A.deal.qc : A.deal.qc + A.deal.kc)));
-  const int n = min(HPT, (part == 0 ? A.heads[0] : A.heads[1]) - h0);  // heads of this chunk
-
-  const uint8_t* in = (part == 0 ? A.in[0] : (part == 1 ? A.in[1] : A.in[2])) +
-                      m * (part == 0 ? A.in_stride[0] : (part == 1 ? A.in_stride[1] : A.in_stride[2])) +
-                      (int64_t)h0 * (D * 2) + l * 16;
-  uint4 raw[HPT];
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (in_range && i < n) { raw[i] = *reinterpret_cast<const uint4*>(in + i * (D * 2)); }
-  }
-
-  bool turn = in_range;  // whether this token is written at all
-  int64_t row = m;
-  if (A.cos_sin && A.positions) {
-    const int p = __ldg(A.positions + m);
-    turn = in_range && p >= 0 && p < A.table_rows;
-    if (in_range && p >= A.table_rows && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
-    row = turn ? p : 0;
-  }
-  uint8_t* out;                    // where head h0 of this token goes
-  int64_t out_step = D * 2;        // and from a head to the next
-  uint8_t* pairs = nullptr;
-  if (MODE == 0 || part == 0) {
-    out = (part == 0 ? A.out[0] : A.out[1]) + m * (part == 0 ? A.out_stride[0] : A.out_stride[1]) +
-          (int64_t)h0 * (D * 2) + l * 16;
-  } else {
-    const int64_t s = __ldg(A.slots + m);
-    turn = turn && s >= 0 && s < A.num_slots;
-    if (in_range && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-    const int64_t page = turn ? slot_page(s, A.kv.page_size) : 0, at = turn ? s - page * A.kv.page_size : 0;
-    out = (part == 1 ? A.kv.k : A.kv.v) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
-          l * (MODE == 8 ? 8 : 16);
-    out_step = A.kv.head_bytes;
-    if (MODE == 8) {
-      pairs = (part == 1 ? A.kv.ks : A.kv.vs) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes +
-              at * A.kv.stoken_bytes + (l >> 3) * 4;
-    }
-  }
+  int64_t m0;
+  int tl, chunk;
+  const bool mine = dealt<LPH>(deal, m0, tl, chunk);
+  const int h0 = HPT * chunk;
+  const int n = mine ? min(HPT, A.heads[part] - h0) : 0;  // heads of this chunk
+  const bool to_cache = MODE != 0 && part > 0;
 
   // This lane's eight values among the pairs: y = r (x cw + o sw), o the partner's values (in lane `partner`, or
   // the neighbours). The norm weights are folded into cos and sin, so that a head costs one product and one sum a
   // value, and the exchange does not wait for the norm.
   const int half = A.rot >> 1;
-  const bool rotated = A.cos_sin && d0 < A.rot && part < 2;
-  const bool swap = A.cos_sin && !A.interleaved;
-  const bool any_norm = A.norm_w[0] || A.norm_w[1];
-  const uint16_t* nw = part == 0 ? A.norm_w[0] : (part == 1 ? A.norm_w[1] : nullptr);
-  float cw[8], sw[8];
-  if (nw) {
-    unpack8(__ldg(reinterpret_cast<const uint4*>(nw + d0)), cw);
-  } else {
+  const bool turns = A.cos_sin && part < 2, rotated = turns && d0 < A.rot;
+  const bool swap = turns && !A.interleaved;
+  const bool second = d0 >= half;
+  const int partner = swap && rotated ? (second ? l - (half >> 3) : l + (half >> 3)) : l;
+  const uint16_t* nw = part < 2 ? A.norm_w[part] : nullptr;
+  uint4 w_own = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u), w_other;  // ones
+  if (nw) { w_own = __ldg(reinterpret_cast<const uint4*>(nw + d0)); }
+  w_other.x = __shfl_sync(0xffffffffu, w_own.x, partner, LPH);
+  w_other.y = __shfl_sync(0xffffffffu, w_own.y, partner, LPH);
+  w_other.z = __shfl_sync(0xffffffffu, w_own.z, partner, LPH);
+  w_other.w = __shfl_sync(0xffffffffu, w_own.w, partner, LPH);
+
+  int64_t m = m0 + tl;
+  // the longest chain first, and a token ahead: position, table row
+  int p = 0;
+  if (A.cos_sin && A.positions && mine && m < A.M) { p = __ldg(A.positions + m); }
+  for (; m0 < A.M; m0 += deal.step, m += deal.step) {
+    const bool live = mine && m < A.M;
+    const uint8_t* in = A.in[part] + m * A.in_stride[part] + (int64_t)h0 * (D * 2) + l * 16;
+    uint4 raw[HPT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { cw[e] = 1.0f; }
-  }
-  int partner = l;
-  if (swap) {
-    const bool second = d0 >= half;
-    if (rotated) { partner = second ? l - (half >> 3) : l + (half >> 3); }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { sw[e] = __shfl_sync(0xffffffffu, cw[e], partner, LPH); }
+    for (int i = 0; i < HPT; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (live && i < n) { raw[i] = *reinterpret_cast<const uint4*>(in + i * (D * 2)); }
+    }
+    bool turn = live;  // whether this token is written at all
+    int64_t row = live ? m : 0;
+    if (A.cos_sin && A.positions) {
+      turn = live && p >= 0 && p < A.table_rows;
+      if (live && p >= A.table_rows && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
+      row = turn ? p : 0;
+      if (mine && m + deal.step < A.M) { p = __ldg(A.positions + m + deal.step); }
+    }
+    float cw[8], sw[8];
+    unpack8(w_own, cw);
+    unpack8(w_other, sw);
     if (rotated) {
-      const float* tab = A.cos_sin + row * A.rot + (second ? d0 - half : d0);
-      const float sg = second ? 1.0f : -1.0f;
+      const float* tab = A.cos_sin + row * A.rot + (A.interleaved ? d0 >> 1 : (second ? d0 - half : d0));
+      if (swap) {
+        const float sg = second ? 1.0f : -1.0f;
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 c = __ldg(reinterpret_cast<const float4*>(tab + e)), s = __ldg(reinterpret_cast<const float4*>(tab + half + e));
-        cw[e] *= c.x, cw[e + 1] *= c.y, cw[e + 2] *= c.z, cw[e + 3] *= c.w;
-        sw[e] *= sg * s.x, sw[e + 1] *= sg * s.y, sw[e + 2] *= sg * s.z, sw[e + 3] *= sg * s.w;
+        for (int e = 0; e < 8; e += 4) {
+          const float4 c = __ldg(reinterpret_cast<const float4*>(tab + e)), s = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+          cw[e] *= c.x, cw[e + 1] *= c.y, cw[e + 2] *= c.z, cw[e + 3] *= c.w;
+          sw[e] *= sg * s.x, sw[e + 1] *= sg * s.y, sw[e + 2] *= sg * s.z, sw[e + 3] *= sg * s.w;
+        }
+      } else {
+        const float4 c4 = __ldg(reinterpret_cast<const float4*>(tab)), s4 = __ldg(reinterpret_cast<const float4*>(tab + half));
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float wa = cw[2 * e], wb = cw[2 * e + 1];
+          cw[2 * e] = wa * c[e], sw[2 * e] = -wb * s[e];
+          cw[2 * e + 1] = wb * c[e], sw[2 * e + 1] = wa * s[e];
+        }
       }
     }
-  } else if (rotated) {
-    const float* tab = A.cos_sin + row * A.rot + (d0 >> 1);
-    const float4 c4 = __ldg(reinterpret_cast<const float4*>(tab)), s4 = __ldg(reinterpret_cast<const float4*>(tab + half));
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float wa = cw[2 * e], wb = cw[2 * e + 1];
-      cw[2 * e] = wa * c[e], sw[2 * e] = -wb * s[e];
-      cw[2 * e + 1] = wb * c[e], sw[2 * e + 1] = wa * s[e];
-    }
-  }
-
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    if (__all_sync(0xffffffffu, i >= n)) { break; }
-    float x[8];
-    unpack8(raw[i], x);
-    // lanes of a warp can hold heads of different parts: the shuffles run for all, the values of v stay as they are
-    float r = 1.0f;
-    if (any_norm) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
-#pragma unroll
-      for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
-      if (nw) { r = rsqrtf(__fmaf_rn(ss, A.inv_d, A.eps)); }
-    }
-    float o[8];
-    if (swap) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { o[e] = __shfl_sync(0xffffffffu, x[e], partner, LPH); }
+    uint8_t* out;             // where head h0 of this token goes
+    int64_t out_step = D * 2; // and from a head to the next
+    uint8_t* pairs = nullptr;
+    if (to_cache) {
+      const int64_t s = __ldg(A.slots + (live ? m : 0));
+      turn = turn && s >= 0 && s < A.num_slots;
+      if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+      const int64_t page = turn ? slot_page(s, A.kv) : 0, at = turn ? s - page * A.kv.page_size : 0;
+      out = (part == 1 ? A.kv.k : A.kv.v) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
+            l * (MODE == 8 ? 8 : 16);
+      out_step = A.kv.head_bytes;
+      if (MODE == 8) {
+        pairs = (part == 1 ? A.kv.ks : A.kv.vs) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes + at * A.kv.stoken_bytes +
+                (l >> 3) * 4;
+      }
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { o[e] = x[e ^ 1]; }
+      out = A.out[MODE ? 0 : part] + m * A.out_stride[MODE ? 0 : part] + (int64_t)h0 * (D * 2) + l * 16;
     }
-    if (part < 2) {
+    const int writes = turn ? n : 0;
+    auto put_codes = [&](int i, uint2 c, uint32_t pair) {
+      if (i < writes) {
+        *reinterpret_cast<uint2*>(out + i * out_step) = c;
+        if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
+      }
+    };
+    if (MODE && part == 2) {  // values: as they are
+#pragma unroll
+      for (int i = 0; i < HPT; ++i) {
+        if (MODE == 16) {
+          if (i < writes) { *reinterpret_cast<uint4*>(out + i * out_step) = raw[i]; }
+        } else {
+          uint32_t pair;
+          const uint2 c = quant8(raw[i], pair);
+          put_codes(i, c, pair);
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < HPT; ++i) {
+      float x[8], o[8];
+      unpack8(raw[i], x);
+      float r = 1.0f;
+      if (nw) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { ss = __fmaf_rn(x[e], x[e], ss); }
+#pragma unroll
+        for (int d = 1; d < LPH; d <<= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, d); }
+        r = rsqrtf(__fmaf_rn(ss, A.inv_d, A.eps));
+      }
+      if (swap) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { o[e] = __shfl_sync(0xffffffffu, x[e], partner, LPH); }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { o[e] = x[e ^ 1]; }
+      }
       if (rotated) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) { x[e] = __fmaf_rn(o[e], sw[e], x[e] * cw[e]) * r; }
@@ -245,16 +292,14 @@ __global__ void __launch_bounds__(256) norm_rope_store_kernel(const __grid_const
 #pragma unroll
         for (int e = 0; e < 8; ++e) { x[e] = x[e] * cw[e] * r; }
       }
-    }
-    if (MODE == 8 && __any_sync(0xffffffffu, part > 0)) {
-      uint32_t pair;
-      const uint2 c = quant8(x, pair);
-      if (part > 0 && turn && i < n) {
-        *reinterpret_cast<uint2*>(out + i * out_step) = c;
-        if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
+      if (MODE == 8 && to_cache) {
+        uint32_t pair;
+        const uint2 c = quant8(x, pair);
+        put_codes(i, c, pair);
+      } else if (i < writes) {
+        *reinterpret_cast<uint4*>(out + i * out_step) = pack8(x);
       }
     }
-    if ((MODE != 8 || part == 0) && turn && i < n) { *reinterpret_cast<uint4*>(out + i * out_step) = pack8(x); }
   }
 }
 
@@ -264,107 +309,88 @@ struct CopyArgs {
   int64_t stride[2];  // bytes
   const int64_t* slots;
   int64_t M, num_slots;
-  Deal deal;
+  Deal deal[2];
 };
 
-// Rows into the cache.
-template <int D, int BITS, int HPT>
-__global__ void __launch_bounds__(256) kv_store_kernel(const __grid_constant__ CopyArgs A) {
+// Rows into the cache (STORE), or out of it: eight values a lane and head, 8 bytes of codes and their pair (or 16
+// bytes of bf16) on the cache's side, 16 bytes on the rows'.
+template <int D, int BITS, bool STORE, int HPT>
+__global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ CopyArgs A) {
   constexpr int LPH = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int is_v = blockIdx.x >= A.deal[1].first;
+  const Deal& deal = A.deal[is_v];
   const int l = threadIdx.x % LPH;
-  int64_t m;
-  int chunk;
-  const bool in_range = dealt<LPH>(A.deal, A.M, m, chunk);
-  const bool is_v = chunk >= A.deal.kc;
-  const int h0 = HPT * (is_v ? chunk - A.deal.kc : chunk);
-  const int n = in_range ? min(HPT, A.kv.kv_heads - h0) : 0;
-  const uint8_t* in = (is_v ? A.rows[1] : A.rows[0]) + m * (is_v ? A.stride[1] : A.stride[0]) + (int64_t)h0 * (D * 2) + l * 16;
-  uint4 raw[HPT];
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (i < n) { raw[i] = ldg_stream_v4(in + i * (D * 2)); }
-  }
-  const int64_t s = __ldg(A.slots + m);
-  if (n > 0 && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-  const bool live = s >= 0 && s < A.num_slots;
-  const int64_t page = live ? slot_page(s, A.kv.page_size) : 0, at = live ? s - page * A.kv.page_size : 0;
-  uint8_t* out = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
-                 l * (BITS == 16 ? 16 : 8);
-  uint8_t* pairs = (is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes + at * A.kv.stoken_bytes +
-                   (l >> 3) * 4;
-  const int writes = live ? n : 0;
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    if (BITS == 16) {
-      if (i < writes) { *reinterpret_cast<uint4*>(out + i * A.kv.head_bytes) = raw[i]; }
-    } else {
-      float x[8];
-      unpack8(raw[i], x);
-      uint32_t pair;
-      const uint2 c = quant8(x, pair);
-      if (i < writes) {
-        *reinterpret_cast<uint2*>(out + i * A.kv.head_bytes) = c;
-        if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
-      }
-    }
-  }
-}
-
-// Rows out of it: eight values a lane and head, 8 bytes of codes and their pair (or 16 bytes of bf16) in, 16 bytes out.
-template <int D, int BITS, int HPT>
-__global__ void __launch_bounds__(256) kv_load_kernel(const __grid_constant__ CopyArgs A) {
-  constexpr int LPH = D / 8;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int l = threadIdx.x % LPH;
-  int64_t m;
-  int chunk;
-  if (!dealt<LPH>(A.deal, A.M, m, chunk)) { return; }
-  const bool is_v = chunk >= A.deal.kc;
-  const int h0 = HPT * (is_v ? chunk - A.deal.kc : chunk);
+  int64_t m0;
+  int tl, chunk;
+  const bool mine = dealt<LPH>(deal, m0, tl, chunk);
+  const int h0 = HPT * chunk;
   const int n = min(HPT, A.kv.kv_heads - h0);
-  const int64_t s = __ldg(A.slots + m);
-  if (s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-  const bool live = s >= 0 && s < A.num_slots;
-  const int64_t page = live ? slot_page(s, A.kv.page_size) : 0, at = live ? s - page * A.kv.page_size : 0;
-  const uint8_t* in = (is_v ? A.kv.v : A.kv.k) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
-                      l * (BITS == 16 ? 16 : 8);
-  const uint8_t* pairs = (is_v ? A.kv.vs : A.kv.ks) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes +
-                         at * A.kv.stoken_bytes + (l >> 3) * 4;
-  uint4 y[HPT];
-  uint32_t pair[HPT];
+  int64_t m = m0 + tl;
+  uint8_t* cache0 = (is_v ? A.kv.v : A.kv.k) + h0 * A.kv.head_bytes + l * (BITS == 16 ? 16 : 8);
+  uint8_t* pairs0 = (is_v ? A.kv.vs : A.kv.ks) + h0 * A.kv.shead_bytes + (l >> 3) * 4;
+  int64_t s = mine && m < A.M ? __ldg(A.slots + m) : -1;
+  for (; m0 < A.M; m0 += deal.step, m += deal.step) {
+    const bool live = mine && m < A.M;
+    uint8_t* rows = A.rows[is_v] + m * A.stride[is_v] + (int64_t)h0 * (D * 2) + l * 16;
+    uint4 raw[HPT];
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    y[i] = make_uint4(0, 0, 0, 0);
-    pair[i] = 0;
-    if (live && i < n) {
-      if (BITS == 16) {
-        y[i] = *reinterpret_cast<const uint4*>(in + i * A.kv.head_bytes);
-      } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(in + i * A.kv.head_bytes);
-        y[i].x = c.x, y[i].y = c.y;
-        pair[i] = *reinterpret_cast<const uint32_t*>(pairs + i * A.kv.shead_bytes);
+    for (int i = 0; i < HPT; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (STORE && live && i < n) { raw[i] = ldg_stream_v4(rows + i * (D * 2)); }
+    }
+    const bool there = s >= 0 && s < A.num_slots;
+    if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+    const int64_t page = there ? slot_page(s, A.kv) : 0, at = there ? s - page * A.kv.page_size : 0;
+    s = mine && m + deal.step < A.M ? __ldg(A.slots + m + deal.step) : -1;  // of the next token
+    uint8_t* cache = cache0 + page * A.kv.page_bytes + at * A.kv.token_bytes;
+    uint8_t* pairs = pairs0 + page * A.kv.spage_bytes + at * A.kv.stoken_bytes;
+    if (STORE) {
+      const int writes = live && there ? n : 0;
+#pragma unroll
+      for (int i = 0; i < HPT; ++i) {
+        if (BITS == 16) {
+          if (i < writes) { *reinterpret_cast<uint4*>(cache + i * A.kv.head_bytes) = raw[i]; }
+        } else {
+          uint32_t pair;
+          const uint2 c = quant8(raw[i], pair);
+          if (i < writes) {
+            *reinterpret_cast<uint2*>(cache + i * A.kv.head_bytes) = c;
+            if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
+          }
+        }
+      }
+    } else {
+      uint32_t pair[HPT];
+#pragma unroll
+      for (int i = 0; i < HPT; ++i) {
+        pair[i] = 0;
+        if (live && there && i < n) {
+          if (BITS == 16) {
+            raw[i] = *reinterpret_cast<const uint4*>(cache + i * A.kv.head_bytes);
+          } else {
+            const uint2 c = *reinterpret_cast<const uint2*>(cache + i * A.kv.head_bytes);
+            raw[i].x = c.x, raw[i].y = c.y;
+            pair[i] = *reinterpret_cast<const uint32_t*>(pairs + i * A.kv.shead_bytes);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < HPT; ++i) {
+        if (BITS == 8) {
+          const float sc = __uint_as_float(pair[i] << 16), b = __uint_as_float(pair[i] & 0xffff0000u);
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // 2^23 + code is a float with the code in its low byte
+            x[e] = __fmaf_rn(sc, __fsub_rn(__uint_as_float(__byte_perm(raw[i].x, 0x4B000000u, 0x7650 | e)), 8388608.0f), b);
+            x[4 + e] = __fmaf_rn(sc, __fsub_rn(__uint_as_float(__byte_perm(raw[i].y, 0x4B000000u, 0x7650 | e)), 8388608.0f), b);
+          }
+          raw[i] = pack8(x);
+        }
+        if (live && i < n) { *reinterpret_cast<uint4*>(rows + i * (D * 2)) = raw[i]; }
       }
     }
-  }
-  uint8_t* out = (is_v ? A.rows[1] : A.rows[0]) + m * (is_v ? A.stride[1] : A.stride[0]) + (int64_t)h0 * (D * 2) + l * 16;
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    if (i >= n) { break; }
-    if (BITS == 8) {
-      const float sc = __uint_as_float(pair[i] << 16), b = __uint_as_float(pair[i] & 0xffff0000u);
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = dequant_f32(sc, (y[i].x >> (8 * e)) & 0xffu, b);
-        x[4 + e] = dequant_f32(sc, (y[i].y >> (8 * e)) & 0xffu, b);
-      }
-      y[i] = pack8(x);
-    }
-    *reinterpret_cast<uint4*>(out + i * (D * 2)) = y[i];
   }
 }
 
@@ -377,21 +403,36 @@ bool is_wide(int64_t M, int heads, int D) { return M * heads > (int64_t)num_sms(
 struct Launch {
   dim3 grid, block;
 };
-int deal(const char* who, int64_t M, int q_heads, int kv_heads, bool with_v, int hpt, int D, Deal* d, Launch* l) {
+// Deals `parts` parts of heads[] heads each. The blocks of all parts together are enough for `waves` times what the SMs
+// hold at 64 registers a thread, shared out by the parts' heads.
+void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, Deal* deals, Launch* l) {
   const int groups = 256 / (D / 8);
-  d->qc = (q_heads + hpt - 1) / hpt;
-  d->kc = (kv_heads + hpt - 1) / hpt;
-  d->chunks = d->qc + (with_v ? 2 : 1) * d->kc;
-  d->token_blocks = (d->chunks + groups - 1) / groups;
-  d->per_block = (d->chunks + d->token_blocks - 1) / d->token_blocks;
-  d->tokens = groups / d->per_block;
-  if (d->token_blocks > 1 || M < num_sms()) { d->tokens = 1; }
-  d->rcp = (65536u + d->per_block - 1) / d->per_block;
-  const int64_t blocks = (M + d->tokens - 1) / d->tokens;
-  if (blocks > INT_MAX / d->token_blocks) { return fail(VPQ_ERR_UNSUPPORTED, "%s: too many rows (M=%lld)", who, (long long)M); }
-  l->grid = dim3((unsigned)(blocks * d->token_blocks));
-  l->block = dim3((unsigned)((d->tokens * d->per_block * (D / 8) + 31) & ~31));
-  return VPQ_OK;
+  int total = 0, threads = 32;
+  for (int i = 0; i < parts; ++i) { total += heads[i]; }
+  uint32_t first = 0;
+  for (int i = 0; i < parts; ++i) {
+    Deal& d = deals[i];
+    d.chunks = (heads[i] + hpt - 1) / hpt;
+    d.token_blocks = (d.chunks + groups - 1) / groups;
+    d.per_block = (d.chunks + d.token_blocks - 1) / d.token_blocks;
+    d.tokens = groups / d.per_block;
+    // few tokens: spread them
+    if (d.token_blocks > 1 || M < num_sms()) { d.tokens = 1; }
+    d.rcp = (65536u + d.per_block - 1) / d.per_block;
+    threads = std::max(threads, d.tokens * d.per_block * (D / 8));
+  }
+  threads = (threads + 31) & ~31;
+  for (int i = 0; i < parts; ++i) {
+    Deal& d = deals[i];
+    const int64_t need = (M + d.tokens - 1) / d.tokens;
+    const int64_t cap = (int64_t)num_sms() * (1024 / threads) * waves * heads[i] / total / d.token_blocks;
+    const int64_t blocks = std::min(need, std::max<int64_t>(cap, 1));
+    d.first = first;
+    d.step = blocks * d.tokens;
+    first += (uint32_t)(blocks * d.token_blocks);
+  }
+  l->block = dim3((unsigned)threads);
+  l->grid = dim3(first);
 }
 
 template <typename K, typename A>
@@ -410,11 +451,11 @@ int launch_with_pdl(K kern, const Launch& d, cudaStream_t st, const A& a) {
 }
 
 template <int MODE>
-int launch_norm(const char* who, const QkArgs& a0, int D, cudaStream_t st) {
+int launch_norm(const QkArgs& a0, int D, cudaStream_t st) {
   QkArgs a = a0;
   Launch l;
   const bool wide = is_wide(a.M, a.heads[0] + (MODE ? 2 : 1) * a.heads[1], D);
-  if (int rc = deal(who, a.M, a.heads[0], a.heads[1], MODE != 0, wide ? 4 : 1, D, &a.deal, &l)) { return rc; }
+  deal(a.M, a.heads, MODE ? 3 : 2, wide ? 4 : 1, 4, D, a.deal, &l);
   if (D == 64) {
     return wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, l, st, a)
                 : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, l, st, a);
@@ -427,23 +468,20 @@ int launch_norm(const char* who, const QkArgs& a0, int D, cudaStream_t st) {
               : launch_with_pdl(norm_rope_store_kernel<256, MODE, 1>, l, st, a);
 }
 
-template <int BITS, bool STORE, int D>
-int launch_copy_d(bool wide, const Launch& l, cudaStream_t st, const CopyArgs& a) {
-  if (STORE) {
-    return wide ? launch_with_pdl(kv_store_kernel<D, BITS, 4>, l, st, a) : launch_with_pdl(kv_store_kernel<D, BITS, 1>, l, st, a);
-  }
-  return wide ? launch_with_pdl(kv_load_kernel<D, BITS, 4>, l, st, a) : launch_with_pdl(kv_load_kernel<D, BITS, 1>, l, st, a);
-}
-
 template <int BITS, bool STORE>
-int launch_copy(const char* who, const CopyArgs& a0, int D, cudaStream_t st) {
+int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
   CopyArgs a = a0;
   Launch l;
-  const bool wide = is_wide(a.M, 2 * a.kv.kv_heads, D);
-  if (int rc = deal(who, a.M, 0, a.kv.kv_heads, true, wide ? 4 : 1, D, &a.deal, &l)) { return rc; }
-  if (D == 64) { return launch_copy_d<BITS, STORE, 64>(wide, l, st, a); }
-  if (D == 128) { return launch_copy_d<BITS, STORE, 128>(wide, l, st, a); }
-  return launch_copy_d<BITS, STORE, 256>(wide, l, st, a);
+  const bool wide = a.kv.kv_heads >= 4 && is_wide(a.M, 2 * a.kv.kv_heads, D);
+  const int heads[2] = {a.kv.kv_heads, a.kv.kv_heads};
+  deal(a.M, heads, 2, wide ? 4 : 1, 8, D, a.deal, &l);
+  if (D == 64) {
+    return wide ? launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 1>, l, st, a);
+  }
+  if (D == 128) {
+    return wide ? launch_with_pdl(kv_copy_kernel<128, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<128, BITS, STORE, 1>, l, st, a);
+  }
+  return wide ? launch_with_pdl(kv_copy_kernel<256, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<256, BITS, STORE, 1>, l, st, a);
 }
 
 bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
@@ -580,6 +618,10 @@ int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
   view->shead_bytes = shs * 2;
   view->stoken_bytes = sts * 2;
   view->page_size = c->page_size;
+  view->page_shift = -1;
+  for (int s = 4; s <= 20; ++s) {
+    if (c->page_size == (1 << s)) { view->page_shift = s; }
+  }
   view->kv_heads = c->kv_heads;
   return VPQ_OK;
 }
@@ -616,7 +658,7 @@ extern "C" int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream)
     return fail(VPQ_ERR_INVALID_ARG, "%s: k_out is k with another row stride", who);
   }
   if (int rc = require_sm100()) { return rc; }
-  return launch_norm<0>(who, a, desc_host->head_dim, static_cast<cudaStream_t>(stream));
+  return launch_norm<0>(a, desc_host->head_dim, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const vpq_kv_cache* cache_host,
@@ -641,8 +683,8 @@ extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const 
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache_host->bits == 8 ? launch_norm<8>(who, a, desc_host->head_dim, st)
-                               : launch_norm<16>(who, a, desc_host->head_dim, st);
+  return cache_host->bits == 8 ? launch_norm<8>(a, desc_host->head_dim, st)
+                               : launch_norm<16>(a, desc_host->head_dim, st);
 }
 
 namespace {
@@ -664,7 +706,7 @@ int copy_rows(const char* who, const vpq_kv_cache* c, const void* k, const void*
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return c->bits == 8 ? launch_copy<8, STORE>(who, a, D, st) : launch_copy<16, STORE>(who, a, D, st);
+  return c->bits == 8 ? launch_copy<8, STORE>(a, D, st) : launch_copy<16, STORE>(a, D, st);
 }
 }  // namespace
 

@@ -21,6 +21,7 @@ struct KvView {
   int64_t page_bytes, head_bytes, token_bytes;     // k and v
   int64_t spage_bytes, shead_bytes, stoken_bytes;  // scale pairs
   int page_size, kv_heads;
+  int page_shift;  // log2 of page_size, or -1
 };
 
 // Checks a cache descriptor and fills `view`; kv_cache.cu.
