@@ -449,7 +449,7 @@ int vpq_affine_qmm_grouped_w8g64_bf16(int act, const uint32_t* w, const void* sc
  * of one byte, and per 64 values a bf16 pair (scale, bias) at page * scale_page_stride + head *
  * scale_head_stride + token * scale_token_stride + 2 * (i / 64) (all 0: dense
  * [num_pages, kv_heads, page_size, head_dim / 64, 2]); a code c stands for scale * c + bias.
- * head_dim 64, 128 or 256; page_size a multiple of 16. k, v, k_scales, v_scales and every stride are
+ * head_dim 64, 128 or 256; page_size a multiple of 16; token and head strides below 2^30 bytes. k, v, k_scales, v_scales and every stride are
  * 16-byte multiples, except that scale strides need only be multiples of head_dim / 32 elements.
  * No two (page, head, token) may share bytes. */
 typedef struct vpq_kv_cache {

@@ -22,20 +22,24 @@ struct Deal {
   int per_block;     // of a token in a block
   int tokens, token_blocks;
   uint32_t rcp;      // 2^16 / per_block, rounded up: (g * rcp) >> 16 = g / per_block for g < 256
-  int64_t step;      // tokens that the part's blocks take at a time
+  uint32_t step;     // tokens that the part's blocks take at a time
 };
 // The calling lane group's chunk, its first token and its block's; false if there is no chunk for it (such lanes
 // keep their warp's shuffles company).
 template <int LPH>
-__device__ __forceinline__ bool dealt(const Deal& d, int64_t& m0, int& tl, int& chunk) {
+__device__ __forceinline__ bool dealt(const Deal& d, uint32_t& m0, uint32_t& tl, int& chunk) {
   const uint32_t g = threadIdx.x / LPH, blk = blockIdx.x - d.first;
-  tl = (int)((g * d.rcp) >> 16);
+  tl = (g * d.rcp) >> 16;
   const uint32_t tb = d.token_blocks == 1 ? blk : blk / (uint32_t)d.token_blocks;
-  m0 = (int64_t)tb * d.tokens;
+  m0 = tb * (uint32_t)d.tokens;
   chunk = (int)((blk - tb * (uint32_t)d.token_blocks) * (uint32_t)d.per_block + (g - tl * d.per_block));
-  const bool in = tl < d.tokens && chunk < d.chunks;
-  if (!in) { tl = chunk = 0; }
+  const bool in = tl < (uint32_t)d.tokens && chunk < d.chunks;
+  if (!in) { tl = 0, chunk = 0; }
   return in;
+}
+// p + a b, one instruction.
+__device__ __forceinline__ uint8_t* at(const uint8_t* p, uint32_t a, uint32_t b) {
+  return const_cast<uint8_t*>(p) + (uint64_t)a * b;
 }
 
 // One head's row is D values, eight (16 bytes) per lane: LPH = D / 8 lanes hold it, and every
@@ -44,13 +48,14 @@ __device__ __forceinline__ bool dealt(const Deal& d, int64_t& m0, int& tl, int& 
 struct QkArgs {
   const uint8_t* in[3];  // q, k, v rows; null where there are none
   uint8_t* out[2];       // q, k rows out
-  int64_t in_stride[3];  // bytes
-  int64_t out_stride[2];
+  uint32_t in_stride[3];  // bytes
+  uint32_t out_stride[2];
   const uint16_t* norm_w[2];
   const float* cos_sin;
   const int32_t* positions;
   const int64_t* slots;
-  int64_t M, table_rows, num_slots;
+  uint32_t M, table_rows;
+  int64_t num_slots;
   int heads[3];
   Deal deal[3];
   int rot, interleaved;
@@ -143,10 +148,14 @@ __device__ __forceinline__ uint2 quant8(const uint4 raw, uint32_t& pair) {
   return quant8(x, __uint_as_float(m << 16), -__uint_as_float(m & 0xffff0000u), pair);
 }
 
-__device__ __forceinline__ int64_t slot_page(int64_t slot, const KvView& kv) {
-  if (kv.page_shift >= 0) { return slot >> kv.page_shift; }
-  // a 64-bit division costs five times as much
-  return (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)kv.page_size) : slot / kv.page_size;
+// A slot inside the cache as page and place. (Pages and places fit 32 bits; a 64-bit division costs five times as much.)
+__device__ __forceinline__ void split_slot(int64_t slot, const KvView& kv, uint32_t& page, uint32_t& place) {
+  if (kv.page_shift >= 0) {
+    page = (uint32_t)(slot >> kv.page_shift);
+  } else {
+    page = (slot >> 32) == 0 ? (uint32_t)slot / (uint32_t)kv.page_size : (uint32_t)(slot / kv.page_size);
+  }
+  place = (uint32_t)slot - page * (uint32_t)kv.page_size;
 }
 
 // MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads of a chunk, all
@@ -159,11 +168,11 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
   const int part = MODE && blockIdx.x >= A.deal[2].first ? 2 : (blockIdx.x >= A.deal[1].first ? 1 : 0);
   const Deal& deal = A.deal[part];
   const int l = threadIdx.x % LPH, d0 = l * 8;
-  int64_t m0;
-  int tl, chunk;
+  uint32_t m0, tl;
+  int chunk;
   const bool mine = dealt<LPH>(deal, m0, tl, chunk);
   const int h0 = HPT * chunk;
-  const int n = mine ? min(HPT, A.heads[part] - h0) : 0;  // heads of this chunk
+  const int n = min(HPT, A.heads[part] - h0);  // heads of this chunk
   const bool to_cache = MODE != 0 && part > 0;
 
   // This lane's eight values among the pairs: y = r (x cw + o sw), o the partner's values (in lane `partner`, or
@@ -175,39 +184,39 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
   const bool second = d0 >= half;
   const int partner = swap && rotated ? (second ? l - (half >> 3) : l + (half >> 3)) : l;
   const uint16_t* nw = part < 2 ? A.norm_w[part] : nullptr;
-  uint4 w_own = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u), w_other;  // ones
-  if (nw) { w_own = __ldg(reinterpret_cast<const uint4*>(nw + d0)); }
-  w_other.x = __shfl_sync(0xffffffffu, w_own.x, partner, LPH);
-  w_other.y = __shfl_sync(0xffffffffu, w_own.y, partner, LPH);
-  w_other.z = __shfl_sync(0xffffffffu, w_own.z, partner, LPH);
-  w_other.w = __shfl_sync(0xffffffffu, w_own.w, partner, LPH);
-
-  int64_t m = m0 + tl;
+  uint32_t m = m0 + tl;
   // the longest chain first, and a token ahead: position, table row
+  const bool by_position = A.cos_sin && A.positions;
   int p = 0;
-  if (A.cos_sin && A.positions && mine && m < A.M) { p = __ldg(A.positions + m); }
+  if (by_position && m < A.M) { p = __ldg(A.positions + m); }
   for (; m0 < A.M; m0 += deal.step, m += deal.step) {
     const bool live = mine && m < A.M;
-    const uint8_t* in = A.in[part] + m * A.in_stride[part] + (int64_t)h0 * (D * 2) + l * 16;
+    const uint32_t mm = live ? m : 0;  // a row to read in any case
+    const uint8_t* in = at(A.in[part], mm, A.in_stride[part]) + (h0 * (D * 2) + l * 16);
     uint4 raw[HPT];
 #pragma unroll
     for (int i = 0; i < HPT; ++i) {
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (live && i < n) { raw[i] = *reinterpret_cast<const uint4*>(in + i * (D * 2)); }
+      if (i > 0) { raw[i] = make_uint4(0, 0, 0, 0); }
+      if (i == 0 || i < n) { raw[i] = *reinterpret_cast<const uint4*>(in + i * (D * 2)); }
     }
     bool turn = live;  // whether this token is written at all
-    int64_t row = live ? m : 0;
-    if (A.cos_sin && A.positions) {
-      turn = live && p >= 0 && p < A.table_rows;
-      if (live && p >= A.table_rows && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
-      row = turn ? p : 0;
-      if (mine && m + deal.step < A.M) { p = __ldg(A.positions + m + deal.step); }
+    uint32_t row = mm;
+    if (by_position) {
+      turn = live && p >= 0 && (uint32_t)p < A.table_rows;
+      if (live && p >= 0 && !turn && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
+      row = turn ? (uint32_t)p : 0;
+      if (m + deal.step < A.M) { p = __ldg(A.positions + m + deal.step); }
     }
     float cw[8], sw[8];
-    unpack8(w_own, cw);
-    unpack8(w_other, sw);
+    if (nw) {
+      unpack8(__ldg(reinterpret_cast<const uint4*>(nw) + l), cw);
+      unpack8(__ldg(reinterpret_cast<const uint4*>(nw) + partner), sw);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { cw[e] = sw[e] = 1.0f; }
+    }
     if (rotated) {
-      const float* tab = A.cos_sin + row * A.rot + (A.interleaved ? d0 >> 1 : (second ? d0 - half : d0));
+      const float* tab = reinterpret_cast<const float*>(at(reinterpret_cast<const uint8_t*>(A.cos_sin), row, A.rot * 4)) + (A.interleaved ? d0 >> 1 : (second ? d0 - half : d0));
       if (swap) {
         const float sg = second ? 1.0f : -1.0f;
 #pragma unroll
@@ -227,28 +236,28 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
         }
       }
     }
-    uint8_t* out;             // where head h0 of this token goes
-    int64_t out_step = D * 2; // and from a head to the next
+    uint8_t* out;
     uint8_t* pairs = nullptr;
     if (to_cache) {
-      const int64_t s = __ldg(A.slots + (live ? m : 0));
-      turn = turn && s >= 0 && s < A.num_slots;
+      const int64_t s = __ldg(A.slots + mm);
       if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-      const int64_t page = turn ? slot_page(s, A.kv) : 0, at = turn ? s - page * A.kv.page_size : 0;
-      out = (part == 1 ? A.kv.k : A.kv.v) + page * A.kv.page_bytes + h0 * A.kv.head_bytes + at * A.kv.token_bytes +
+      turn = turn && s >= 0 && s < A.num_slots;
+      uint32_t page = 0, place = 0;
+      if (turn) { split_slot(s, A.kv, page, place); }
+      out = at(at((part == 1 ? A.kv.k : A.kv.v) + page * A.kv.page_bytes, place, A.kv.token_bytes), h0, A.kv.head_bytes) +
             l * (MODE == 8 ? 8 : 16);
-      out_step = A.kv.head_bytes;
       if (MODE == 8) {
-        pairs = (part == 1 ? A.kv.ks : A.kv.vs) + page * A.kv.spage_bytes + h0 * A.kv.shead_bytes + at * A.kv.stoken_bytes +
-                (l >> 3) * 4;
+        pairs = at(at((part == 1 ? A.kv.ks : A.kv.vs) + page * A.kv.spage_bytes, place, A.kv.stoken_bytes), h0,
+                   A.kv.shead_bytes) + (l >> 3) * 4;
       }
     } else {
-      out = A.out[MODE ? 0 : part] + m * A.out_stride[MODE ? 0 : part] + (int64_t)h0 * (D * 2) + l * 16;
+      out = at(A.out[MODE ? 0 : part], mm, A.out_stride[MODE ? 0 : part]) + (h0 * (D * 2) + l * 16);
     }
+    const uint32_t to_step = to_cache ? A.kv.head_bytes : D * 2;  // from a head to the next
     const int writes = turn ? n : 0;
     auto put_codes = [&](int i, uint2 c, uint32_t pair) {
       if (i < writes) {
-        *reinterpret_cast<uint2*>(out + i * out_step) = c;
+        *reinterpret_cast<uint2*>(out + i * to_step) = c;
         if ((l & 7) == 0) { *reinterpret_cast<uint32_t*>(pairs + i * A.kv.shead_bytes) = pair; }
       }
     };
@@ -256,7 +265,7 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
 #pragma unroll
       for (int i = 0; i < HPT; ++i) {
         if (MODE == 16) {
-          if (i < writes) { *reinterpret_cast<uint4*>(out + i * out_step) = raw[i]; }
+          if (i < writes) { *reinterpret_cast<uint4*>(out + i * to_step) = raw[i]; }
         } else {
           uint32_t pair;
           const uint2 c = quant8(raw[i], pair);
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
         const uint2 c = quant8(x, pair);
         put_codes(i, c, pair);
       } else if (i < writes) {
-        *reinterpret_cast<uint4*>(out + i * out_step) = pack8(x);
+        *reinterpret_cast<uint4*>(out + i * to_step) = pack8(x);
       }
     }
   }
@@ -306,9 +315,10 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
 struct CopyArgs {
   KvView kv;
   uint8_t* rows[2];   // k, v: read by the store, written by the load
-  int64_t stride[2];  // bytes
+  uint32_t stride[2];  // bytes
+  uint32_t M;
   const int64_t* slots;
-  int64_t M, num_slots;
+  int64_t num_slots;
   Deal deal[2];
 };
 
@@ -322,30 +332,34 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
   const int is_v = blockIdx.x >= A.deal[1].first;
   const Deal& deal = A.deal[is_v];
   const int l = threadIdx.x % LPH;
-  int64_t m0;
-  int tl, chunk;
+  uint32_t m0, tl;
+  int chunk;
   const bool mine = dealt<LPH>(deal, m0, tl, chunk);
   const int h0 = HPT * chunk;
   const int n = min(HPT, A.kv.kv_heads - h0);
-  int64_t m = m0 + tl;
-  uint8_t* cache0 = (is_v ? A.kv.v : A.kv.k) + h0 * A.kv.head_bytes + l * (BITS == 16 ? 16 : 8);
-  uint8_t* pairs0 = (is_v ? A.kv.vs : A.kv.ks) + h0 * A.kv.shead_bytes + (l >> 3) * 4;
-  int64_t s = mine && m < A.M ? __ldg(A.slots + m) : -1;
+  uint32_t m = m0 + tl;
+  const uint8_t* rows0 = A.rows[is_v] + h0 * (D * 2) + l * 16;
+  const uint8_t* cache0 = at(is_v ? A.kv.v : A.kv.k, h0, A.kv.head_bytes) + l * (BITS == 16 ? 16 : 8);
+  const uint8_t* pairs0 = at(is_v ? A.kv.vs : A.kv.ks, h0, A.kv.shead_bytes) + (l >> 3) * 4;
+  int64_t s = m < A.M ? __ldg(A.slots + m) : -1;
   for (; m0 < A.M; m0 += deal.step, m += deal.step) {
     const bool live = mine && m < A.M;
-    uint8_t* rows = A.rows[is_v] + m * A.stride[is_v] + (int64_t)h0 * (D * 2) + l * 16;
+    uint8_t* rows = at(rows0, live ? m : 0, A.stride[is_v]);
     uint4 raw[HPT];
+    if (STORE) {
 #pragma unroll
-    for (int i = 0; i < HPT; ++i) {
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (STORE && live && i < n) { raw[i] = ldg_stream_v4(rows + i * (D * 2)); }
+      for (int i = 0; i < HPT; ++i) {
+        if (i > 0) { raw[i] = make_uint4(0, 0, 0, 0); }
+        if (i == 0 || i < n) { raw[i] = ldg_stream_v4(rows + i * (D * 2)); }
+      }
     }
     const bool there = s >= 0 && s < A.num_slots;
     if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
-    const int64_t page = there ? slot_page(s, A.kv) : 0, at = there ? s - page * A.kv.page_size : 0;
-    s = mine && m + deal.step < A.M ? __ldg(A.slots + m + deal.step) : -1;  // of the next token
-    uint8_t* cache = cache0 + page * A.kv.page_bytes + at * A.kv.token_bytes;
-    uint8_t* pairs = pairs0 + page * A.kv.spage_bytes + at * A.kv.stoken_bytes;
+    uint32_t page = 0, place = 0;
+    if (there) { split_slot(s, A.kv, page, place); }
+    s = m + deal.step < A.M ? __ldg(A.slots + m + deal.step) : -1;  // of the next token
+    uint8_t* cache = at(cache0 + page * A.kv.page_bytes, place, A.kv.token_bytes);
+    uint8_t* pairs = at(pairs0 + page * A.kv.spage_bytes, place, A.kv.stoken_bytes);
     if (STORE) {
       const int writes = live && there ? n : 0;
 #pragma unroll
@@ -363,10 +377,12 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
       }
     } else {
       uint32_t pair[HPT];
+      const int reads = live && there ? n : 0;
 #pragma unroll
       for (int i = 0; i < HPT; ++i) {
-        pair[i] = 0;
-        if (live && there && i < n) {
+        pair[i] = 0;  // scale and bias 0: the value 0
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (i < reads) {
           if (BITS == 16) {
             raw[i] = *reinterpret_cast<const uint4*>(cache + i * A.kv.head_bytes);
           } else {
@@ -428,7 +444,7 @@ void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, Dea
     const int64_t cap = (int64_t)num_sms() * (1024 / threads) * waves * heads[i] / total / d.token_blocks;
     const int64_t blocks = std::min(need, std::max<int64_t>(cap, 1));
     d.first = first;
-    d.step = blocks * d.tokens;
+    d.step = (uint32_t)(blocks * d.tokens);
     first += (uint32_t)(blocks * d.token_blocks);
   }
   l->block = dim3((unsigned)threads);
@@ -487,19 +503,18 @@ int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
 bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
 
 // Fills and checks one row operand; stride 0 = dense.
-int take_rows(const char* who, const char* name, const void* p, int64_t stride, int64_t heads, int D, int64_t M,
-              int64_t* bytes) {
+int take_rows(const char* who, const char* name, const void* p, int64_t stride, int64_t heads, int D, uint32_t* bytes) {
   if (!p) { return fail(VPQ_ERR_INVALID_ARG, "%s: %s is null", who, name); }
   if (stride == 0) { stride = heads * D; }
   if (stride < heads * D) {
     return fail(VPQ_ERR_INVALID_ARG, "%s: %s rows overlap (stride %lld for %lld values)", who, name, (long long)stride,
                 (long long)(heads * D));
   }
-  if (stride > (INT64_MAX / 2) / M) { return fail(VPQ_ERR_INVALID_ARG, "%s: %s stride out of range", who, name); }
+  if (stride > INT_MAX / 2) { return fail(VPQ_ERR_INVALID_ARG, "%s: the rows of %s are 2^31 bytes or more apart", who, name); }
   if (!aligned16(p) || (stride & 7)) {
     return fail(VPQ_ERR_ALIGNMENT, "%s: %s and its row stride must be multiples of 16 bytes", who, name);
   }
-  *bytes = stride * 2;
+  *bytes = (uint32_t)(stride * 2);
   return VPQ_OK;
 }
 
@@ -512,8 +527,8 @@ int take_qk(const char* who, const vpq_qk_desc& d, QkArgs* a) {
   if (!known_dim(d.head_dim)) {
     return fail(VPQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256 (got %d)", who, d.head_dim);
   }
-  if (d.q_heads > 65536 || d.kv_heads > 65536 || d.M > (int64_t)1 << 40) {
-    return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 heads and 2^40 rows", who);
+  if (d.q_heads > 65536 || d.kv_heads > 65536 || d.M > INT_MAX / 2) {
+    return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 heads and 2^30 rows", who);
   }
   if (d.cos_sin) {
     if (d.rot_dim <= 0 || d.rot_dim > d.head_dim || (d.rot_dim & 15)) {
@@ -538,8 +553,8 @@ int take_qk(const char* who, const vpq_qk_desc& d, QkArgs* a) {
   a->norm_w[1] = static_cast<const uint16_t*>(d.k_norm_w);
   a->cos_sin = d.cos_sin;
   a->positions = d.positions;
-  a->M = d.M;
-  a->table_rows = d.table_rows;
+  a->M = (uint32_t)d.M;
+  a->table_rows = (uint32_t)std::min<int64_t>(d.table_rows, INT_MAX);  // positions name no more
   a->heads[0] = d.q_heads;
   a->heads[1] = d.kv_heads;
   a->heads[2] = d.kv_heads;
@@ -547,9 +562,9 @@ int take_qk(const char* who, const vpq_qk_desc& d, QkArgs* a) {
   a->interleaved = d.interleaved != 0;
   a->eps = d.eps;
   a->inv_d = 1.0f / (float)d.head_dim;
-  if (int rc = take_rows(who, "q", d.q, d.q_stride, d.q_heads, d.head_dim, d.M, &a->in_stride[0])) { return rc; }
-  if (int rc = take_rows(who, "k", d.k, d.k_stride, d.kv_heads, d.head_dim, d.M, &a->in_stride[1])) { return rc; }
-  if (int rc = take_rows(who, "q_out", d.q_out, d.q_out_stride, d.q_heads, d.head_dim, d.M, &a->out_stride[0])) { return rc; }
+  if (int rc = take_rows(who, "q", d.q, d.q_stride, d.q_heads, d.head_dim, &a->in_stride[0])) { return rc; }
+  if (int rc = take_rows(who, "k", d.k, d.k_stride, d.kv_heads, d.head_dim, &a->in_stride[1])) { return rc; }
+  if (int rc = take_rows(who, "q_out", d.q_out, d.q_out_stride, d.q_heads, d.head_dim, &a->out_stride[0])) { return rc; }
   a->in[0] = static_cast<const uint8_t*>(d.q);
   a->in[1] = static_cast<const uint8_t*>(d.k);
   a->out[0] = static_cast<uint8_t*>(d.q_out);
@@ -596,10 +611,10 @@ int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
       (q && (sts < pairs || (shs < pairs && c->kv_heads > 1) || (sps < pairs && c->num_pages > 1) || shs < 0 || sps < 0))) {
     return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is smaller than a row", who);
   }
-  const int64_t lim = (int64_t)1 << 46;  // of one term, in elements: no sum of three passes 2^48
-  if (ts > lim / c->page_size || hs > lim / c->kv_heads || ps > lim / c->num_pages || sts > lim / c->page_size ||
-      shs > lim / c->kv_heads || sps > lim / c->num_pages) {
-    return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is out of range", who);
+  const int64_t lim = INT_MAX / 2 / elt;  // four heads' offsets fit 32 bits
+  if (ts > lim || hs > lim || sts > lim || shs > lim || ps > ((int64_t)1 << 46) / c->num_pages ||
+      sps > ((int64_t)1 << 46) / c->num_pages) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is out of range (token and head strides stay below 2^30 bytes)", who);
   }
   const int64_t mult = 16 / elt;
   if (!strides_ok(ts, mult) || !strides_ok(hs, mult) || !strides_ok(ps, mult) ||
@@ -612,11 +627,11 @@ int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
   view->vs = static_cast<uint8_t*>(c->v_scales);
   view->num_pages = c->num_pages;
   view->page_bytes = ps * elt;
-  view->head_bytes = hs * elt;
-  view->token_bytes = ts * elt;
+  view->head_bytes = (uint32_t)(hs * elt);
+  view->token_bytes = (uint32_t)(ts * elt);
   view->spage_bytes = sps * 2;
-  view->shead_bytes = shs * 2;
-  view->stoken_bytes = sts * 2;
+  view->shead_bytes = (uint32_t)(shs * 2);
+  view->stoken_bytes = (uint32_t)(sts * 2);
   view->page_size = c->page_size;
   view->page_shift = -1;
   for (int s = 4; s <= 20; ++s) {
@@ -649,8 +664,7 @@ extern "C" int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream)
   if (!desc_host) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
   QkArgs a = {};
   if (int rc = take_qk(who, *desc_host, &a)) { return rc; }
-  if (int rc = take_rows(who, "k_out", desc_host->k_out, desc_host->k_out_stride, desc_host->kv_heads, desc_host->head_dim,
-                         desc_host->M, &a.out_stride[1])) {
+  if (int rc = take_rows(who, "k_out", desc_host->k_out, desc_host->k_out_stride, desc_host->kv_heads, desc_host->head_dim, &a.out_stride[1])) {
     return rc;
   }
   a.out[1] = static_cast<uint8_t*>(desc_host->k_out);
@@ -668,8 +682,7 @@ extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const 
   if (!desc_host) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
   QkArgs a = {};
   if (int rc = take_qk(who, *desc_host, &a)) { return rc; }
-  if (int rc = take_rows(who, "v", desc_host->v, desc_host->v_stride, desc_host->kv_heads, desc_host->head_dim,
-                         desc_host->M, &a.in_stride[2])) {
+  if (int rc = take_rows(who, "v", desc_host->v, desc_host->v_stride, desc_host->kv_heads, desc_host->head_dim, &a.in_stride[2])) {
     return rc;
   }
   a.in[2] = static_cast<const uint8_t*>(desc_host->v);
@@ -694,15 +707,16 @@ int copy_rows(const char* who, const vpq_kv_cache* c, const void* k, const void*
   clear_error();
   CopyArgs a = {};
   if (int rc = kv_check(who, c, &a.kv)) { return rc; }
-  if (M <= 0 || M > (int64_t)1 << 40) { return fail(VPQ_ERR_INVALID_ARG, "%s: need 0 < M <= 2^40 (M=%lld)", who, (long long)M); }
+  if (M <= 0) { return fail(VPQ_ERR_INVALID_ARG, "%s: need M > 0 (M=%lld)", who, (long long)M); }
+  if (M > INT_MAX / 2) { return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 2^30 rows (M=%lld)", who, (long long)M); }
   const int D = c->head_dim, H = c->kv_heads;
-  if (int rc = take_rows(who, STORE ? "k" : "k_out", k, k_stride, H, D, M, &a.stride[0])) { return rc; }
-  if (int rc = take_rows(who, STORE ? "v" : "v_out", v, v_stride, H, D, M, &a.stride[1])) { return rc; }
+  if (int rc = take_rows(who, STORE ? "k" : "k_out", k, k_stride, H, D, &a.stride[0])) { return rc; }
+  if (int rc = take_rows(who, STORE ? "v" : "v_out", v, v_stride, H, D, &a.stride[1])) { return rc; }
   if (int rc = take_slots(who, slots)) { return rc; }
   a.rows[0] = static_cast<uint8_t*>(const_cast<void*>(k));
   a.rows[1] = static_cast<uint8_t*>(const_cast<void*>(v));
   a.slots = slots;
-  a.M = M;
+  a.M = (uint32_t)M;
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);

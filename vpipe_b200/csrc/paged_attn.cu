@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   constexpr int kRowsPer = CH < 32 ? 32 / CH : 1;    // rows that one round of the warp's copies covers
   constexpr int kRounds = 16 * CH / 32;
   const int crow = CH < 32 ? lane / CH : 0, cch = lane % CH;
-  const int64_t lane_off = crow * A.kv.token_bytes + cch * 16;
+  const int64_t lane_off = (int64_t)crow * A.kv.token_bytes + cch * 16;
 
   // Requests the next unit into stage `st`; commits a group in any case.
   auto request = [&](int st) {
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         const int rlo = ok ? lo - 16 * i : 16, rhi = ok ? hi - 16 * i : 0;
         if (!ok && lo < 16 * i + 16 && hi > 16 * i) { bad |= 1 << i; }
         const int64_t pp = ok ? page[i] : 0;
-        const int64_t o = pp * A.kv.page_bytes + lkv * A.kv.head_bytes + (int64_t)off * A.kv.token_bytes + lane_off;
+        const int64_t o = pp * A.kv.page_bytes + (int64_t)lkv * A.kv.head_bytes + (int64_t)off * A.kv.token_bytes + lane_off;
         const uint8_t* kp = A.kv.k + o;
         const uint8_t* vp = A.kv.v + o;
 #pragma unroll
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         if (BITS == 8) {
           const int row = lane & 15;
           const bool live = row >= rlo && row < rhi;
-          const uint8_t* sp = (lane < 16 ? A.kv.ks : A.kv.vs) + pp * A.kv.spage_bytes + lkv * A.kv.shead_bytes +
+          const uint8_t* sp = (lane < 16 ? A.kv.ks : A.kv.vs) + pp * A.kv.spage_bytes + (int64_t)lkv * A.kv.shead_bytes +
                               (int64_t)(off + row) * A.kv.stoken_bytes;
           cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + (16 * i + row) * kPair, sp, live);
         }

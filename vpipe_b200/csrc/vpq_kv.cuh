@@ -18,8 +18,8 @@ struct KvView {
   uint8_t* ks;
   uint8_t* vs;
   int64_t num_pages;
-  int64_t page_bytes, head_bytes, token_bytes;     // k and v
-  int64_t spage_bytes, shead_bytes, stoken_bytes;  // scale pairs
+  int64_t page_bytes, spage_bytes;                  // k and v; scale pairs
+  uint32_t head_bytes, token_bytes, shead_bytes, stoken_bytes;
   int page_size, kv_heads;
   int page_shift;  // log2 of page_size, or -1
 };
