@@ -451,45 +451,48 @@ def qmm_grouped_down(codes, scales, biases, x_sorted, tile2e, sdst=None, y_rows=
 
 
 # ---- the attention block between the q | k | v and the o projection
+# A decode step makes these calls once a layer, so the checks below are written for a short way through Python.
+_BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+_DENSE = torch.contiguous_format
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 class _Placed:
-    """Makes `device` (and `stream`, if given) current for a call, so that what the call allocates belongs to the
+    """Makes a device (and `stream`, if given) current for a call, so that what the call allocates belongs to the
     stream that it runs on."""
     __slots__ = ("ctx",)
 
-    def __init__(self, device, stream):
-        if stream is not None:
-            self.ctx = torch.cuda.stream(stream)
-        else:
-            self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    def __init__(self, dev, stream):
+        self.ctx = torch.cuda.stream(stream) if stream is not None else torch.cuda.device(dev)
 
     def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+        self.ctx.__enter__()
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+        self.ctx.__exit__(*exc)
 
 
-def _heads(name, t, device, shape=None):
-    """Pointer and row stride (elements) of rows [M, heads, dim]: strides beyond the row's are the caller's."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3:
-        raise ValueError(f"vpipe_b200.ops: {name} must be bfloat16 [rows, heads, head_dim]")
-    if not t.is_cuda or t.device != device:
-        raise ValueError(f"vpipe_b200.ops: {name} must live on {device} (no CPU path)")
-    m, h, d = t.shape
-    if shape is not None and (m, h, d) != shape:
-        raise ValueError(f"vpipe_b200.ops: {name} has shape {tuple(t.shape)}, {shape} is wanted")
+def _elsewhere(dev, stream) -> bool:
+    """Whether a call for tensors of device `dev` has to switch to it or to `stream` first."""
+    if dev < 0:
+        raise ValueError("vpipe_b200.ops: rows must be bfloat16 on a CUDA device (no CPU path)")
+    return stream is not None or dev != torch.cuda.current_device()
+
+
+def _heads(name, t, dev, shape):
+    """Pointer and row stride (elements) of bfloat16 rows [M, heads, dim]: strides beyond the row's are the caller's."""
+    if t.dtype is not _BF16 or t.get_device() != dev or t.shape != shape:
+        raise ValueError(f"vpipe_b200.ops: {name} must be bfloat16 {tuple(shape)} on cuda:{dev} (no CPU path), "
+                         f"not {t.dtype} {tuple(t.shape)} on {t.device}")
     sm, sh, sd = t.stride()
-    if (d > 1 and sd != 1) or (h > 1 and sh != d):
+    if sd != 1 or (sh != shape[2] and shape[1] > 1):
         raise ValueError(f"vpipe_b200.ops: the heads of a row of {name} must be contiguous")
-    return t.data_ptr(), sm if m > 1 else 0
+    return t.data_ptr(), sm if shape[0] > 1 else 0
 
 
-def _index(name, t, device, dtype, shape):
-    if t.dtype != dtype or not t.is_cuda or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"vpipe_b200.ops: {name} must be a contiguous {dtype} tensor {shape} on {device}")
+def _index(name, t, dev, dtype, shape):
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"vpipe_b200.ops: {name} must be a contiguous {dtype} tensor {tuple(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
@@ -526,6 +529,8 @@ class PagedKVCache:
             d.k_scales, d.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
             d.scale_page_stride, d.scale_head_stride, d.scale_token_stride = k_scales.stride()[:3]
         self.ref = C.byref(d)
+        self._dev = k.get_device()
+        self._rows = k_scales if quantised else k  # a bfloat16 tensor of this device
         self._workspace_bytes = {}
 
     @classmethod
@@ -541,24 +546,30 @@ class PagedKVCache:
         return cls(*codes, *pairs)
 
 
-def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved):
-    dev = q.device
-    d = _lib.QkDesc()
-    d.q, d.q_stride = _heads("q", q, dev)
-    d.k, d.k_stride = _heads("k", k, dev, (q.shape[0], k.shape[1], q.shape[2]))
-    d.M, d.q_heads, d.head_dim = q.shape
-    d.kv_heads, d.eps, d.interleaved = k.shape[1], eps, int(interleaved)
-    for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-        if w is not None:
-            setattr(d, name, _index(name, w, dev, torch.bfloat16, (q.shape[2],)))
+def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, k_out):
+    shape = q.shape
+    if len(shape) != 3 or k.dim() != 3:
+        raise ValueError("vpipe_b200.ops: q and k must be bfloat16 [rows, heads, head_dim]")
+    M, hq, D = shape
+    hkv = k.shape[1]
+    kshape = (M, hkv, D)
+    pq, sq = _heads("q", q, dev, shape)
+    pk, sk = _heads("k", k, dev, kshape)
+    pv, sv = _heads("v", v, dev, kshape) if v is not None else (None, 0)
+    po, so = _heads("q_out", q_out, dev, shape)
+    pj, sj = _heads("k_out", k_out, dev, kshape) if k_out is not None else (None, 0)
+    wq = _index("q_norm_w", q_norm_w, dev, _BF16, (D,)) if q_norm_w is not None else None
+    wk = _index("k_norm_w", k_norm_w, dev, _BF16, (D,)) if k_norm_w is not None else None
+    pt, pp, rows, rot = None, None, 0, 0
     if cos_sin is not None:
         if cos_sin.dim() != 2:
             raise ValueError("vpipe_b200.ops: cos_sin must be float32 [rows, rot_dim]")
-        d.cos_sin = _index("cos_sin", cos_sin, dev, torch.float32, tuple(cos_sin.shape))
-        d.table_rows, d.rot_dim = cos_sin.shape
+        rows, rot = cos_sin.shape
+        pt = _index("cos_sin", cos_sin, dev, _F32, (rows, rot))
     if positions is not None:
-        d.positions = _index("positions", positions, dev, torch.int32, (q.shape[0],))
-    return d
+        pp = _index("positions", positions, dev, _I32, (M,))
+    return _lib.QkDesc(pq, pk, pv, po, pj, sq, sk, sv, so, sj, wq, wk, pt, pp, M, rows, hq, hkv, D, rot, int(interleaved),
+                       eps)
 
 
 def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=None, eps=1e-6, interleaved=False,
@@ -567,16 +578,15 @@ def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=Non
     q [M, q_heads, D], k [M, kv_heads, D] bfloat16, rows with any stride (parts of one q | k | v row are fine);
     cos_sin float32 [rows, rot_dim] = cos | sin of the pairs' angles; token m takes row positions[m] (int32; None: row
     m) and is left as it was if that is outside of the table. q_out / k_out may be q / k. Returns (q_out, k_out)."""
-    dev = q.device
-    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved)
-    with _Placed(dev, stream) as st:
-        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if q_out is None else q_out
-        k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if k_out is None else k_out
-        if q.shape[0] == 0:
-            return q_out, k_out
-        d.q_out, d.q_out_stride = _heads("q_out", q_out, dev, tuple(q.shape))
-        d.k_out, d.k_out_stride = _heads("k_out", k_out, dev, tuple(k.shape))
-        check(lib().vpq_qk_norm_rope_bf16(C.byref(d), st))
+    dev = q.get_device()
+    if _elsewhere(dev, stream):
+        with _Placed(dev, stream):
+            return qk_norm_rope(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, q_out, k_out)
+    q_out = torch.empty_like(q, memory_format=_DENSE) if q_out is None else q_out
+    k_out = torch.empty_like(k, memory_format=_DENSE) if k_out is None else k_out
+    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, None, q_out, k_out)
+    if d.M != 0:
+        check(lib().vpq_qk_norm_rope_bf16(C.byref(d), _raw_stream(dev)))
     return q_out, k_out
 
 
@@ -584,46 +594,49 @@ def qkv_norm_rope_store(q, k, v, q_norm_w, k_norm_w, cos_sin, positions, cache, 
                         q_out=None, stream=None):
     """qk_norm_rope with the keys, and the values as they are, going straight into the cache: row m to slot slots[m]
     (int64; page * page_size + place; negative: nowhere) (vpq_qkv_norm_rope_store_bf16). Returns q_out."""
-    dev = cache.device
-    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved)
-    d.v, d.v_stride = _heads("v", v, dev, tuple(k.shape))
-    s = _index("slots", slots, dev, torch.int64, (q.shape[0],))
-    with _Placed(dev, stream) as st:
-        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if q_out is None else q_out
-        if q.shape[0] == 0:
-            return q_out
-        d.q_out, d.q_out_stride = _heads("q_out", q_out, dev, tuple(q.shape))
-        check(lib().vpq_qkv_norm_rope_store_bf16(C.byref(d), cache.ref, s, st))
+    dev = cache._dev
+    if _elsewhere(dev, stream):
+        with _Placed(dev, stream):
+            return qkv_norm_rope_store(q, k, v, q_norm_w, k_norm_w, cos_sin, positions, cache, slots, eps, interleaved,
+                                       q_out)
+    q_out = torch.empty_like(q, memory_format=_DENSE) if q_out is None else q_out
+    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, None)
+    s = _index("slots", slots, dev, _I64, (d.M,))
+    if d.M != 0:
+        check(lib().vpq_qkv_norm_rope_store_bf16(C.byref(d), cache.ref, s, _raw_stream(dev)))
     return q_out
 
 
 def kv_store(k, v, cache, slots, stream=None):
     """Rows k, v [M, kv_heads, head_dim] into slots [M] of the cache, quantised if it is (vpq_kv_store_bf16)."""
-    dev = cache.device
+    dev = cache._dev
+    if _elsewhere(dev, stream):
+        with _Placed(dev, stream):
+            return kv_store(k, v, cache, slots)
     shape = (k.shape[0], cache.kv_heads, cache.head_dim)
     pk, sk = _heads("k", k, dev, shape)
     pv, sv = _heads("v", v, dev, shape)
-    s = _index("slots", slots, dev, torch.int64, shape[:1])
-    if shape[0] == 0:
-        return
-    with _Placed(dev, stream) as st:
-        check(lib().vpq_kv_store_bf16(cache.ref, pk, pv, sk, sv, s, shape[0], st))
+    s = _index("slots", slots, dev, _I64, shape[:1])
+    if shape[0] != 0:
+        check(lib().vpq_kv_store_bf16(cache.ref, pk, pv, sk, sv, s, shape[0], _raw_stream(dev)))
 
 
 def kv_load(cache, slots, k_out=None, v_out=None, stream=None):
     """The values of slots [M]: (k, v) bfloat16 [M, kv_heads, head_dim], zeros for a slot outside of the cache
     (vpq_kv_load_bf16)."""
-    dev = cache.device
-    s = _index("slots", slots, dev, torch.int64, (slots.numel(),))
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    with _Placed(dev, stream) as st:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if k_out is None else k_out
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_out is None else v_out
-        if shape[0] == 0:
-            return k_out, v_out
-        pk, sk = _heads("k_out", k_out, dev, shape)
-        pv, sv = _heads("v_out", v_out, dev, shape)
-        check(lib().vpq_kv_load_bf16(cache.ref, pk, pv, sk, sv, s, shape[0], st))
+    dev = cache._dev
+    if _elsewhere(dev, stream):
+        with _Placed(dev, stream):
+            return kv_load(cache, slots, k_out, v_out)
+    M = slots.numel()
+    s = _index("slots", slots, dev, _I64, (M,))
+    shape = (M, cache.kv_heads, cache.head_dim)
+    k_out = cache._rows.new_empty(shape) if k_out is None else k_out
+    v_out = cache._rows.new_empty(shape) if v_out is None else v_out
+    pk, sk = _heads("k_out", k_out, dev, shape)
+    pv, sv = _heads("v_out", v_out, dev, shape)
+    if M != 0:
+        check(lib().vpq_kv_load_bf16(cache.ref, pk, pv, sk, sv, s, M, _raw_stream(dev)))
     return k_out, v_out
 
 
@@ -632,34 +645,33 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
     page_table int32 [B, max_pages], seq_lens int32 [B] (the new token's own key included), window 0 = all tokens.
     Lengths are read on the device, so a captured call serves any. The workspace is allocated per call on the stream
     that the call runs on."""
-    dev = cache.device
-    shape = tuple(q.shape)
-    d = _lib.PagedAttentionDesc()
-    d.q, d.q_stride = _heads("q", q, dev)
-    if shape[2] != cache.head_dim:
-        raise ValueError(f"vpipe_b200.ops: q has head_dim {shape[2]}, the cache {cache.head_dim}")
-    if page_table.dim() != 2:
-        raise ValueError("vpipe_b200.ops: page_table must be int32 [batch, max_pages]")
-    d.page_table = _index("page_table", page_table, dev, torch.int32, (shape[0], page_table.shape[1]))
-    d.seq_lens = _index("seq_lens", seq_lens, dev, torch.int32, shape[:1])
-    d.batch, d.q_heads = shape[:2]
-    d.max_pages = page_table.shape[1]
-    d.window = window
-    if scale is not None:
-        if not scale > 0:
-            raise ValueError("vpipe_b200.ops: scale must be positive")
-        d.scale = scale
-    with _Placed(dev, stream) as st:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if out is None else out
-        if shape[0] == 0:
-            return out
-        d.out, d.out_stride = _heads("out", out, dev, shape)
-        ref = C.byref(d)
-        need = cache._workspace_bytes.get(shape)
-        if need is None:
-            need = cache._workspace_bytes[shape] = int(lib().vpq_paged_attention_bytes(ref, cache.ref))
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        check(lib().vpq_paged_attention_bf16(ref, cache.ref, ws.data_ptr(), need, st))
+    dev = cache._dev
+    if _elsewhere(dev, stream):
+        with _Placed(dev, stream):
+            return paged_attention(q, cache, page_table, seq_lens, scale, window, out)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or page_table.dim() != 2:
+        raise ValueError(f"vpipe_b200.ops: q must be bfloat16 [batch, q_heads, {cache.head_dim}], page_table int32 "
+                         "[batch, max_pages]")
+    B, hq, _ = shape
+    pages = page_table.shape[1]
+    if scale is None:
+        scale = 0.0
+    elif not scale > 0:
+        raise ValueError("vpipe_b200.ops: scale must be positive")
+    out = torch.empty_like(q, memory_format=_DENSE) if out is None else out
+    pq, sq = _heads("q", q, dev, shape)
+    po, so = _heads("out", out, dev, shape)
+    d = _lib.PagedAttentionDesc(pq, po, sq, so, _index("page_table", page_table, dev, _I32, (B, pages)),
+                                _index("seq_lens", seq_lens, dev, _I32, (B,)), 0, B, pages, hq, window, scale)
+    if B == 0:
+        return out
+    L, ref = lib(), C.byref(d)
+    need = cache._workspace_bytes.get(hq)  # goes by the heads alone
+    if need is None:
+        need = cache._workspace_bytes[hq] = int(L.vpq_paged_attention_bytes(ref, cache.ref))
+    ws = cache._rows.new_empty((need + 1) // 2)  # bfloat16: two bytes each
+    check(L.vpq_paged_attention_bf16(ref, cache.ref, ws.data_ptr(), need, _raw_stream(dev)))
     return out
 
 
