@@ -67,6 +67,7 @@ struct AttnArgs {
   int cols;          // query heads a unit serves (a column block): min(group, 8 NT)
   int blocks;        // column blocks of a key head
   int hk;            // kv_heads * blocks
+  uint32_t cta_rcp;  // 2^32 / CTAs, rounded up: a quotient may come out one too large, which is as good a cut
   bool few;          // at most 32 sequences, and few enough units for 32-bit sums
   float scale_log2;
   int stage_bytes, ring_bytes;  // shared memory: a stage, a warp's ring
@@ -295,7 +296,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     __syncthreads();
   }
   const int64_t places = total * A.hk;
-  int64_t per_cta = div_u(places + gridDim.x - 1, gridDim.x);
+  // (32-bit numbers by the reciprocal that the host has made of the number of CTAs)
+  int64_t per_cta = (places + gridDim.x) >> 31 == 0 ? (int64_t)__umulhi((uint32_t)places + gridDim.x - 1, A.cta_rcp)
+                                                    : (places + gridDim.x - 1) / gridDim.x;
   per_cta = per_cta > kWarps ? per_cta : kWarps;
   const int64_t cta0 = (int64_t)blockIdx.x * per_cta;
   if (cta0 >= places) { return; }  // the whole CTA
@@ -312,9 +315,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   bool fresh = true;       // the next unit begins a (sequence, head) for this warp
   int page[TM];            // page numbers of the next unit, fetched one unit ahead; -1: none
   auto enter = [&]() {     // to the first token of unit ltile
-    const int64_t at = (int64_t)ltile * kUnit;
-    pg = (int)((uint32_t)at / (uint32_t)A.kv.page_size);
-    off = (int)((uint32_t)at % (uint32_t)A.kv.page_size);
+    const uint32_t at = (uint32_t)ltile * kUnit;
+    pg = (int)(A.kv.page_shift >= 0 ? at >> A.kv.page_shift : at / (uint32_t)A.kv.page_size);
+    off = (int)(at - (uint32_t)pg * (uint32_t)A.kv.page_size);
   };
   auto fetch_pages = [&]() {
     int c = pg, o = off;
@@ -365,7 +368,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     const int place = (int)(in_seq - (int64_t)lh * span);
     ltile = ltile0 + (place > 0 ? place - 1 : 0);
     if (place == 0) { --left; }
-    lkv = lh / A.blocks;
+    lkv = A.blocks == 1 ? lh : lh / A.blocks;
     lblk = lh - lkv * A.blocks;
     if (left > 0) {
       enter();
@@ -912,12 +915,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     }
   }
   __syncthreads();
-  // One (sequence, head) alone: all warps add it up; several: a warp each.
-  const bool alone = (leaders & (leaders - 1)) == 0;
-  const int gt = alone ? tid : lane, gn = alone ? kWarps * 32 : 32;
-  uint32_t later = leaders;
-  for (int turn = 0; later != 0; ++turn, later &= later - 1) {
-    if (!alone && turn % kWarps != warp) { continue; }
+  // The sums, 32 lanes times four values at a time, dealt over the warps in turn.
+  int turn = warp;
+  for (uint32_t later = leaders; later != 0; later &= later - 1) {
     const int n = __ffs(later) - 1;
     const uint32_t members = __shfl_sync(0xffffffffu, run, n);
     const EntryHead& H = s_entry[n];
@@ -926,7 +926,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(A.out + (int64_t)H.b * A.out_stride) + (int64_t)H.h * D;
     // slot 0: the (sequence, head) that the CTA's run begins in; slot 1: another, which it ends in
     const int64_t slot = (int64_t)blockIdx.x * 2 + (H.leads ? 0 : 1);
-    for (int i = gt; i < ncol * (D / 4); i += gn) {  // four values of a column
+    const int rounds = (ncol * (D / 4) + 31) / 32;
+    const int first = turn;
+    for (; turn < rounds; turn += kWarps) {
+      const int i = turn * 32 + lane;  // four values of a column
+      if (i >= ncol * (D / 4)) { continue; }
       const int col = i / (D / 4), d = (i % (D / 4)) * 4;
       const int at = col * (D / 4) + (entry_at<BITS>(col, d) >> 2);
       auto of = [&](int j) {
@@ -973,7 +977,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         }
       }
     }
-    if (!whole && H.begins && gt == 0) {
+    turn -= rounds;
+    if (!whole && H.begins && first == 0 && lane == 0) {
       A.heads[blockIdx.x] = {H.b, H.h, ncol * 2 + (H.leads ? 0 : 1), (int)div_u(cta1 + rest - 1, per_cta)};
     }
   }
@@ -1000,34 +1005,49 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // A warp's first part is fetched together with the record that says whether there is one (whatever lies
-  // there is inside the workspace); the record's own CTA may have it in slot 1.
-  float m1, l1, x[D / 32];
-  auto fetch = [&](int64_t slot) {
-    m1 = A.ml[slot * 2];
-    l1 = A.ml[slot * 2 + 1];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) { x[i] = A.part[slot * D + i * 32 + lane]; }
+  // there is inside the workspace); the record's own CTA may have it in slot 1. The others four at a time.
+  constexpr int V = D / 32;  // a lane's values: V neighbours
+  struct Part {
+    float m, l, x[V];
   };
-  fetch((int64_t)min(c0 + warp, (int)gridDim.x - 1) * 2 * A.cols + col);
+  auto fetch = [&](Part& p, int64_t slot) {
+    p.m = A.ml[slot * 2];
+    p.l = A.ml[slot * 2 + 1];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 w = *reinterpret_cast<const float2*>(A.part + slot * D + lane * V + i);
+      p.x[i] = w.x, p.x[i + 1] = w.y;
+    }
+  };
+  Part first;
+  fetch(first, (int64_t)min(c0 + warp, (int)gridDim.x - 1) * 2 * A.cols + col);
   const CtaHead H = A.heads[c0];
   if (H.last < 0 || col >= (H.ncol_slot >> 1)) { return; }
-  if (warp == 0 && (H.ncol_slot & 1)) { fetch(((int64_t)c0 * 2 + 1) * A.cols + col); }
-  float m = kNegInf, l = 0.0f, acc[D / 32];
+  if (warp == 0 && (H.ncol_slot & 1)) { fetch(first, ((int64_t)c0 * 2 + 1) * A.cols + col); }
+  float m = kNegInf, l = 0.0f, acc[V];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) { acc[i] = 0.0f; }
-  for (int c = c0 + warp; c <= H.last; c += kJoinWarps) {
-    if (c != c0 + warp) { fetch((int64_t)c * 2 * A.cols + col); }
-    const float mj = m1, lj = l1;
-    const float m2 = fmaxf(m, mj);
-    const float f0 = weight_of(m, l, m2), f1 = weight_of(mj, lj, m2);
+  for (int i = 0; i < V; ++i) { acc[i] = 0.0f; }
+  auto add = [&](const Part& p) {
+    const float m2 = fmaxf(m, p.m);
+    const float f0 = weight_of(m, l, m2), f1 = weight_of(p.m, p.l, m2);
     m = m2;
-    l = __fmaf_rn(f1, lj, f0 * l);
+    l = __fmaf_rn(f1, p.l, f0 * l);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) { acc[i] = __fmaf_rn(f1, x[i], f0 * acc[i]); }
+    for (int i = 0; i < V; ++i) { acc[i] = __fmaf_rn(f1, p.x[i], f0 * acc[i]); }
+  };
+  if (c0 + warp <= H.last) { add(first); }
+  for (int c = c0 + warp + kJoinWarps; c <= H.last; c += 4 * kJoinWarps) {
+    Part p[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { fetch(p[k], (int64_t)min(c + k * kJoinWarps, H.last) * 2 * A.cols + col); }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c + k * kJoinWarps <= H.last) { add(p[k]); }
+    }
   }
   if (lane == 0) { s_m[warp] = m, s_l[warp] = l; }
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) { s_acc[warp][i * 32 + lane] = acc[i]; }
+  for (int i = 0; i < D / 32; ++i) { s_acc[warp][lane * V + i] = acc[i]; }
   __syncthreads();
   if (threadIdx.x >= D) { return; }
   float top = kNegInf, sum = 0.0f, o = 0.0f;
@@ -1189,6 +1209,7 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   a.cols = s.cols;
   a.blocks = s.blocks;
   a.hk = cache_host->kv_heads * s.blocks;
+  a.cta_rcp = (uint32_t)((((uint64_t)1 << 32) + s.ctas - 1) / s.ctas);
   a.few = d.batch <= 32 && (int64_t)d.max_pages * cache_host->page_size <= INT_MAX / 4;
   const float scale = d.scale != 0.0f ? d.scale : 1.0f / sqrtf((float)cache_host->head_dim);
   a.scale_log2 = scale * 1.4426950408889634f;
