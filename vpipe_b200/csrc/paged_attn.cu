@@ -68,6 +68,7 @@ struct AttnArgs {
   int blocks;        // column blocks of a key head
   int hk;            // kv_heads * blocks
   uint32_t cta_rcp;  // 2^32 / CTAs, rounded up: a quotient may come out one too large, which is as good a cut
+  bool dense;        // rows of a page's head lie back to back
   bool few;          // at most 32 sequences, and few enough units for 32-bit sums
   float scale_log2;
   int stage_bytes, ring_bytes;  // shared memory: a stage, a warp's ring
@@ -75,6 +76,9 @@ struct AttnArgs {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int BYTES>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool live) {
@@ -197,15 +201,15 @@ __device__ __forceinline__ int span_of(int start, int len) {
   return n > 0 ? n + 1 : 0;
 }
 
-// Where 16-byte chunk c of row `row` lies in a K or V tile. 16 bits: the eight rows that an ldmatrix
-// reads fall into eight bank groups. 8 bits: see the loads in the loop.
+// Where 16-byte chunk c of row `row` lies in a K or V tile: chunk c ^ swz(row). 16 bits: the eight rows that an
+// ldmatrix reads fall into eight bank groups. 8 bits: see the loads in the loop.
 template <int D, int BITS>
-__device__ __forceinline__ int swz_k(int row, int c) {
-  return BITS == 16 ? (c ^ (row & 7)) : (D >= 128 ? (c ^ ((row & 1) << 2)) : c);
+__device__ __forceinline__ constexpr int swz_k(int row) {
+  return BITS == 16 ? row & 7 : (D >= 128 ? (row & 1) << 2 : 0);
 }
 template <int D, int BITS>
-__device__ __forceinline__ int swz_v(int row, int c) {
-  return BITS == 16 ? (c ^ (row & 7)) : (D >= 128 ? (c ^ (row & 6)) : (c ^ (row & 2)));
+__device__ __forceinline__ constexpr int swz_v(int row) {
+  return BITS == 16 ? row & 7 : (D >= 128 ? row & 6 : row & 2);
 }
 
 // What a unit in flight is: written by lane 0 with its copies, read when its turn comes.
@@ -384,7 +388,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   constexpr int kRowsPer = CH < 32 ? 32 / CH : 1;    // rows that one round of the warp's copies covers
   constexpr int kRounds = 16 * CH / 32;
   const int crow = CH < 32 ? lane / CH : 0, cch = lane % CH;
-  const int64_t lane_off = (int64_t)crow * A.kv.token_bytes + cch * 16;
+  // A lane's place in a tile; the swizzles of the lane's row and of a round's act on different bits.
+  const uint32_t lane_k = crow * kRow + ((cch ^ swz_k<D, BITS>(crow)) << 4);
+  const uint32_t lane_v = crow * kRow + ((cch ^ swz_v<D, BITS>(crow)) << 4);
+  const int64_t v_minus_k = A.kv.v - A.kv.k;
+  const uint8_t *head_k = nullptr, *head_s = nullptr;  // this lane's row of page 0 of the current key head
+  auto enter_head = [&]() {
+    head_k = A.kv.k + (uint64_t)(uint32_t)lkv * A.kv.head_bytes + (uint64_t)(uint32_t)crow * A.kv.token_bytes + cch * 16;
+    if (BITS == 8) {
+      head_s = (lane < 16 ? A.kv.ks : A.kv.vs) + (uint64_t)(uint32_t)lkv * A.kv.shead_bytes +
+               (uint64_t)(uint32_t)(lane & 15) * A.kv.stoken_bytes;
+    }
+  };
+  enter_head();
 
   // Requests the next unit into stage `st`; commits a group in any case.
   auto request = [&](int st) {
@@ -394,35 +410,59 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       int hi = llen - ltile * kUnit;
       hi = hi < kUnit ? hi : kUnit;
       const uint32_t dst = ring_s + st * A.stage_bytes;
+      bool plain = A.dense && lo == 0 && hi == kUnit;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) { plain = plain && (uint32_t)page[i] < (uint32_t)A.kv.num_pages; }
       int bad = 0;
+      if (plain) {
+        // every row lives, rows lie back to back: nothing but copies at constant distances
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const bool ok = (uint32_t)page[i] < (uint32_t)A.kv.num_pages;
-        // A page without live tokens, or none: rows of zeros. Dead rows of a page become zeros too: whatever
-        // they hold, their weight 0 has to add 0.
-        const int rlo = ok ? lo - 16 * i : 16, rhi = ok ? hi - 16 * i : 0;
-        if (!ok && lo < 16 * i + 16 && hi > 16 * i) { bad |= 1 << i; }
-        const int64_t pp = ok ? page[i] : 0;
-        const int64_t o = pp * A.kv.page_bytes + (int64_t)lkv * A.kv.head_bytes + (int64_t)off * A.kv.token_bytes + lane_off;
-        const uint8_t* kp = A.kv.k + o;
-        const uint8_t* vp = A.kv.v + o;
+        for (int i = 0; i < TM; ++i) {
+          const uint8_t* kp = head_k + (uint64_t)(uint32_t)page[i] * A.kv.page_bytes + off * kRow;
+          const uint8_t* vp = kp + v_minus_k;
 #pragma unroll
-        for (int j = 0; j < kRounds; ++j) {
-          const int row = CH <= 32 ? crow + j * kRowsPer : 0;
-          const bool live = row >= rlo && row < rhi;
-          const int64_t so = (int64_t)(j * kRowsPer) * A.kv.token_bytes;
-          cp_async16(dst + (16 * i + row) * kRow + swz_k<D, BITS>(row, cch) * 16, kp + so, live);
-          cp_async16(dst + kTile + (16 * i + row) * kRow + swz_v<D, BITS>(row, cch) * 16, vp + so, live);
+          for (int j = 0; j < kRounds; ++j) {
+            constexpr int kStep = kRowsPer;
+            cp_async16(dst + (lane_k ^ (swz_k<D, BITS>(j * kStep) << 4)) + (16 * i + j * kStep) * kRow, kp + j * kStep * kRow);
+            cp_async16(dst + (lane_v ^ (swz_v<D, BITS>(j * kStep) << 4)) + kTile + (16 * i + j * kStep) * kRow,
+                       vp + j * kStep * kRow);
+          }
+          if (BITS == 8) {
+            cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + (16 * i + (lane & 15)) * kPair,
+                                              head_s + (uint64_t)(uint32_t)page[i] * A.kv.spage_bytes + off * kPair, true);
+          }
+          off += 16;
+          if (off == A.kv.page_size) { off = 0, ++pg; }
         }
-        if (BITS == 8) {
-          const int row = lane & 15;
-          const bool live = row >= rlo && row < rhi;
-          const uint8_t* sp = (lane < 16 ? A.kv.ks : A.kv.vs) + pp * A.kv.spage_bytes + (int64_t)lkv * A.kv.shead_bytes +
-                              (int64_t)(off + row) * A.kv.stoken_bytes;
-          cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + (16 * i + row) * kPair, sp, live);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < TM; ++i) {
+          const int pi = TM == 2 && i == 1 ? page[TM - 1] : page[0];
+          const bool ok = (uint32_t)pi < (uint32_t)A.kv.num_pages;
+          // A page without live tokens, or none: rows of zeros. Dead rows of a page become zeros too: whatever
+          // they hold, their weight 0 has to add 0.
+          const int rlo = ok ? lo - 16 * i : 16, rhi = ok ? hi - 16 * i : 0;
+          if (!ok && lo < 16 * i + 16 && hi > 16 * i) { bad |= 1 << i; }
+          const uint64_t pp = ok ? (uint32_t)pi : 0;
+          const uint8_t* kp = head_k + pp * A.kv.page_bytes + (uint64_t)(uint32_t)off * A.kv.token_bytes;
+#pragma unroll
+          for (int j = 0; j < kRounds; ++j) {
+            const int row = crow + j * kRowsPer;
+            const bool live = row >= rlo && row < rhi;
+            const uint8_t* kr = kp + (uint64_t)(j * kRowsPer) * A.kv.token_bytes;
+            const uint32_t to = dst + (16 * i + j * kRowsPer) * kRow;
+            cp_async16(to + (lane_k ^ (swz_k<D, BITS>(j * kRowsPer) << 4)), kr, live);
+            cp_async16(to + kTile + (lane_v ^ (swz_v<D, BITS>(j * kRowsPer) << 4)), kr + v_minus_k, live);
+          }
+          if (BITS == 8) {
+            const int row = lane & 15;
+            cp_async_small<kPair ? kPair : 4>(dst + 2 * kTile + (lane < 16 ? 0 : kPairs) + (16 * i + row) * kPair,
+                                              head_s + pp * A.kv.spage_bytes + (uint64_t)(uint32_t)off * A.kv.stoken_bytes,
+                                              row >= rlo && row < rhi);
+          }
+          off += 16;
+          if (off == A.kv.page_size) { off = 0, ++pg; }
         }
-        off += 16;
-        if (off == A.kv.page_size) { off = 0, ++pg; }
       }
       if (bad) {  // a page outside the cache holds no tokens: the live rows shrink to what is left
         if (lane == 0) { atomicOr(&g_attn_status, kBadPage); }
@@ -438,7 +478,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       const int ncol = min(A.cols, A.group - lblk * A.cols);
       if (fresh) {
         const uint8_t* qp = A.q + (int64_t)lb * A.q_stride + (int64_t)h0 * (D * 2);
-        for (int i = lane; i < ncol * (D / 8); i += 32) { cp_async16(dst + 2 * kTile + 2 * kPairs + i * 16, qp + i * 16, true); }
+        for (int i = lane; i < ncol * (D / 8); i += 32) { cp_async16(dst + 2 * kTile + 2 * kPairs + i * 16, qp + i * 16); }
       }
       const int rest = ltile_end - 1 - ltile;
       if (lane == 0) {
@@ -468,6 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
           ltile = ltile0;
           enter();
+          enter_head();
         }
         fetch_pages();
       }
@@ -570,7 +611,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           uint32_t a[4];
-          ldsm4(a, kt + (16 * i + row) * kRow + swz_k<D, BITS>(row, 2 * k + ch) * 16);
+          ldsm4(a, kt + (16 * i + row) * kRow + ((2 * k + ch) ^ swz_k<D, BITS>(row)) * 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) { mma<false>(s[i][n], a, qf[n][k][0], qf[n][k][1]); }
         }
@@ -598,8 +639,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           // a lane's 16 codes feed four k steps: the k order is permuted the same way in q
-          const uint4 x = lds128(kt + (16 * i + r) * kRow + swz_k<D, BITS>(r, 4 * g + t) * 16);
-          const uint4 y = lds128(kt + (16 * i + r + 8) * kRow + swz_k<D, BITS>(r + 8, 4 * g + t) * 16);
+          const uint4 x = lds128(kt + (16 * i + r) * kRow + ((4 * g + t) ^ swz_k<D, BITS>(r)) * 16);
+          const uint4 y = lds128(kt + (16 * i + r + 8) * kRow + ((4 * g + t) ^ swz_k<D, BITS>(r + 8)) * 16);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
           float c[NT][4];
 #pragma unroll
@@ -736,7 +777,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int k = 0; k < MT; ++k) {
           uint32_t a[4];
-          ldsm4t(a, vt + (16 * i + row) * kRow + swz_v<D, BITS>(row, 2 * k + ch) * 16);
+          ldsm4t(a, vt + (16 * i + row) * kRow + ((2 * k + ch) ^ swz_v<D, BITS>(row)) * 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) { mma<false>(o_acc[n][k], a, b[n][0], b[n][1]); }
         }
@@ -768,7 +809,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int row = 2 * t + (j & 1) + (j >> 1) * 8;
-            w[j] = lds64(vt + (16 * i + row) * kRow + swz_v<D, BITS>(row, 4 * g + (r >> 1)) * 16 + (r & 1) * 8);
+            w[j] = lds64(vt + (16 * i + row) * kRow + ((4 * g + (r >> 1)) ^ swz_v<D, BITS>(row)) * 16 + (r & 1) * 8);
           }
           uint32_t x[2][4];  // per token pair: values 0|1, 2|3, 4|5, 6|7 as bytes (even token, odd token, ...)
 #pragma unroll
@@ -1209,6 +1250,8 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   a.cols = s.cols;
   a.blocks = s.blocks;
   a.hk = cache_host->kv_heads * s.blocks;
+  a.dense = a.kv.token_bytes == (uint32_t)(cache_host->head_dim * cache_host->bits / 8) &&
+            (cache_host->bits == 16 || a.kv.stoken_bytes == (uint32_t)(cache_host->head_dim / kKvGroup * 4));
   a.cta_rcp = (uint32_t)((((uint64_t)1 << 32) + s.ctas - 1) / s.ctas);
   a.few = d.batch <= 32 && (int64_t)d.max_pages * cache_host->page_size <= INT_MAX / 4;
   const float scale = d.scale != 0.0f ? d.scale : 1.0f / sqrtf((float)cache_host->head_dim);
