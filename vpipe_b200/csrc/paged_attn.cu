@@ -172,9 +172,10 @@ __device__ __forceinline__ void lds_pairs(uint32_t (&p)[G], uint32_t a) {
 }
 // Where value d of column col lies in its row of a warp's partial result: the 32 lanes that store
 // together fall into 32 banks.
-template <int BITS>
+template <int BITS, bool HALF>
 __device__ __forceinline__ int entry_at(int col, int d) {
-  return BITS == 16 ? d ^ ((col & 6) << 2) : d ^ ((col >> 1) & 3) ^ ((d >> 3) & 4);
+  const int t = (HALF ? col : col >> 1) & 3;  // the lanes of a quad
+  return BITS == 16 ? d ^ (t << 3) : d ^ t ^ ((d >> 3) & 4);
 }
 // The factor that takes a partial result (maximum m, sum l) to the joint maximum; one without a live token
 // counts nothing, unless it holds a NaN.
@@ -231,7 +232,7 @@ struct EntryHead {
   float m[16], l[16];
 };
 
-template <int D, int BITS, int NT, int TM, int kWarps, int STAGES>
+template <int D, int BITS, int NT, bool HALF, int TM, int kWarps, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnArgs A) {
   constexpr int kUnit = 16 * TM;
   constexpr int kRow = D * BITS / 8;
@@ -240,6 +241,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   constexpr int kPair = BITS == 8 ? G * 4 : 0;  // scale pairs of a row
   constexpr int kPairs = kUnit * kPair;
   constexpr int MT = D / 16;  // 16-row blocks of O^T
+  // Up to four query heads (HALF) sit in every other column, so that a lane of a product has one live column and not
+  // two (or none): half the work between the two products.
+  static_assert(!HALF || NT == 1, "four columns fit one product");
+  constexpr int CN = HALF ? 1 : 2;  // live columns of a lane
+  constexpr int kNone = 1 << 20;
 
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_excl[kWarps * 32];
@@ -251,6 +257,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, t = lane & 3;
+  auto col_of = [&](int n, int c) { return HALF ? t : n * 8 + 2 * t + c; };        // of this lane's accumulators
+  auto col_in = [&](int n) { return HALF ? ((r & 1) ? kNone : r >> 1) : n * 8 + r; };  // of its operands
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -517,8 +525,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   };
 
   float o_acc[NT][MT][4];
-  float m_run[NT][2], l_run[NT][2];
-  float o_mean[NT][G][4], o_bias[NT][G][2], q_sum[NT][G][2], q_mul[NT][2];  // 8 bits
+  float m_run[NT][CN], l_run[NT][CN];
+  float o_mean[NT][G][4], o_bias[NT][G][CN], q_sum[NT][G][CN], q_mul[NT][CN];  // 8 bits
   uint32_t qf[NT][D / 16][2];
   int sigma = -100;      // 8 bits: exponent of the power of two above every value scale so far
   bool run_begins = false, first_run = true;
@@ -540,12 +548,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       sigma = -100;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        m_run[n][0] = m_run[n][1] = kNegInf;
-        l_run[n][0] = l_run[n][1] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CN; ++c) { m_run[n][c] = kNegInf, l_run[n][c] = 0.0f; }
 #pragma unroll
         for (int i = 0; i < MT; ++i) { o_acc[n][i][0] = o_acc[n][i][1] = o_acc[n][i][2] = o_acc[n][i][3] = 0.0f; }
-        const bool live = n * 8 + r < ncol;  // this lane's column
-        const uint32_t qrow = qt + (n * 8 + r) * (D * 2);
+        const bool live = col_in(n) < ncol;
+        const uint32_t qrow = qt + (live ? col_in(n) : 0) * (D * 2);
         if (BITS == 16) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -585,12 +593,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
             for (int i = 0; i < 2; ++i) { qf[n][k][i] = pack_f16x2(lo16(qf[n][k][i]) * up, hi16(qf[n][k][i]) * up); }
           }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {  // the same for the columns of this lane's scores
+          for (int c = 0; c < CN; ++c) {  // the same for the columns of this lane's scores
             q_mul[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * (A.scale_log2 * 16777216.0f);  // codes' 2^24
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               q_sum[n][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * t + c) * 4) * A.scale_log2;
-              o_bias[n][g][c] = o_mean[n][g][c] = o_mean[n][g][2 + c] = 0.0f;
+              o_bias[n][g][c] = 0.0f;
+              o_mean[n][g][0] = o_mean[n][g][1] = o_mean[n][g][2] = o_mean[n][g][3] = 0.0f;
             }
           }
         }
@@ -621,7 +630,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { s[i][n][e] *= A.scale_log2; }
+          for (int e = 0; e < 4; e += 3 - CN) { s[i][n][e] *= A.scale_log2; }
         }
       }
     } else {
@@ -634,7 +643,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { s[i][n][e] = bias[n][e] = 0.0f; }
+          for (int e = 0; e < 4; e += 3 - CN) { s[i][n][e] = bias[n][e] = 0.0f; }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -654,17 +663,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; e += 3 - CN) {
               const uint32_t p = e < 2 ? p0[g] : p1[g];
               s[i][n][e] = __fmaf_rn(c[n][e], lo16(p), s[i][n][e]);
-              bias[n][e] = __fmaf_rn(hi16(p), q_sum[n][g][e & 1], bias[n][e]);
+              bias[n][e] = __fmaf_rn(hi16(p), q_sum[n][g][e & (CN - 1)], bias[n][e]);
             }
           }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { s[i][n][e] = __fmaf_rn(s[i][n][e], q_mul[n][e & 1], bias[n][e]); }
+          for (int e = 0; e < 4; e += 3 - CN) { s[i][n][e] = __fmaf_rn(s[i][n][e], q_mul[n][e & (CN - 1)], bias[n][e]); }
         }
       }
     }
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 4; e += 3 - CN) {
             const int row = 16 * i + r + (e < 2 ? 0 : 8);
             s[i][n][e] = row >= lo && row < hi ? s[i][n][e] : kNegInf;
           }
@@ -683,11 +692,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       }
     }
     bool grows = false;
-    float m_new[NT][2];
+    float m_new[NT][CN];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < CN; ++c) {
         float x = fmaxf(s[0][n][c], s[0][n][2 + c]);
 #pragma unroll
         for (int i = 1; i < TM; ++i) { x = fmaxf(x, fmaxf(s[i][n][c], s[i][n][2 + c])); }
@@ -725,7 +734,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < CN; ++c) {
           const float f = m_new[n][c] > m_run[n][c] ? ex2(m_run[n][c] - m_new[n][c]) : 1.0f;
           m_run[n][c] = m_new[n][c];
           l_run[n][c] *= f;
@@ -748,7 +757,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < CN; ++c) {
         const float m = m_run[n][c] == kNegInf ? 0.0f : m_run[n][c];  // no live token yet: 2^-inf, not NaN
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -767,9 +776,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t w = pack_bf16x2(s[i][n][2 * h], s[i][n][2 * h + 1]);
+            const uint32_t w = pack_bf16x2(s[i][n][2 * h], HALF ? 0.0f : s[i][n][2 * h + 1]);
             l_run[n][0] += lo16(w);
-            l_run[n][1] += hi16(w);
+            if (!HALF) { l_run[n][CN - 1] += hi16(w); }
             b[n][h] = movm(w);
           }
         }
@@ -784,8 +793,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          l_run[n][0] += s[i][n][0] + s[i][n][2];
-          l_run[n][1] += s[i][n][1] + s[i][n][3];
+#pragma unroll
+          for (int c = 0; c < CN; ++c) { l_run[n][c] += s[i][n][c] + s[i][n][2 + c]; }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -795,9 +804,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
             const float sc = lo16(vp[i][h][g]), f = sc * up, bb = __fmaf_rn(128.0f, sc, hi16(vp[i][h][g]));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              b[n][h] = movm(pack_f16x2(s[i][n][2 * h] * f, s[i][n][2 * h + 1] * f));
-              o_bias[n][g][0] = __fmaf_rn(s[i][n][2 * h], bb, o_bias[n][g][0]);
-              o_bias[n][g][1] = __fmaf_rn(s[i][n][2 * h + 1], bb, o_bias[n][g][1]);
+              b[n][h] = movm(pack_f16x2(s[i][n][2 * h] * f, HALF ? 0.0f : s[i][n][2 * h + 1] * f));
+#pragma unroll
+              for (int c = 0; c < CN; ++c) { o_bias[n][g][c] = __fmaf_rn(s[i][n][2 * h + c], bb, o_bias[n][g][c]); }
             }
           }
           const uint32_t mean[4] = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // the code 128
@@ -836,7 +845,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < CN; ++c) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
             l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], d);
@@ -850,8 +859,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o_acc[n][i][e] = __fmaf_rn((o_acc[n][i][e] - o_mean[n][i / 4][e & 1]) * 16777216.0f, o_mul, o_bias[n][i / 4][e & 1]);
+            for (int e = 0; e < 4; e += 3 - CN) {
+              o_acc[n][i][e] =
+                  __fmaf_rn((o_acc[n][i][e] - o_mean[n][i / 4][e & 1]) * 16777216.0f, o_mul, o_bias[n][i / 4][e & (CN - 1)]);
             }
           }
         }
@@ -861,16 +871,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // a sum of 0: no live token (a NaN stays one)
-          const float i0 = l_run[n][0] == 0.0f ? 0.0f : 1.0f / l_run[n][0];
-          const float i1 = l_run[n][1] == 0.0f ? 0.0f : 1.0f / l_run[n][1];
+          float inv[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) { inv[c] = c >= CN || l_run[n][c % CN] == 0.0f ? 0.0f : 1.0f / l_run[n][c % CN]; }
           if (BITS == 16) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const uint32_t w = movm(pack_bf16x2(o_acc[n][i][2 * h] * i0, o_acc[n][i][2 * h + 1] * i1));
-                if (n * 8 + r < ncol) {
-                  *reinterpret_cast<uint32_t*>(op + (n * 8 + r) * (D * 2) + (16 * i + 8 * h + 2 * t) * 2) = w;
+                const uint32_t w = movm(pack_bf16x2(o_acc[n][i][2 * h] * inv[0], HALF ? 0.0f : o_acc[n][i][2 * h + 1] * inv[1]));
+                if (col_in(n) < ncol) {
+                  *reinterpret_cast<uint32_t*>(op + col_in(n) * (D * 2) + (16 * i + 8 * h + 2 * t) * 2) = w;
                 }
               }
             }
@@ -878,14 +889,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
             for (int g = 0; g < G; ++g) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float inv = c ? i1 : i0;
-                const int col = n * 8 + 2 * t + c;
+              for (int c = 0; c < CN; ++c) {
+                const int col = col_of(n, c);
                 uint4 y;
-                y.x = pack_bf16x2(o_acc[n][g * 4][c] * inv, o_acc[n][g * 4][2 + c] * inv);
-                y.y = pack_bf16x2(o_acc[n][g * 4 + 1][c] * inv, o_acc[n][g * 4 + 1][2 + c] * inv);
-                y.z = pack_bf16x2(o_acc[n][g * 4 + 2][c] * inv, o_acc[n][g * 4 + 2][2 + c] * inv);
-                y.w = pack_bf16x2(o_acc[n][g * 4 + 3][c] * inv, o_acc[n][g * 4 + 3][2 + c] * inv);
+                y.x = pack_bf16x2(o_acc[n][g * 4][c] * inv[c], o_acc[n][g * 4][2 + c] * inv[c]);
+                y.y = pack_bf16x2(o_acc[n][g * 4 + 1][c] * inv[c], o_acc[n][g * 4 + 1][2 + c] * inv[c]);
+                y.z = pack_bf16x2(o_acc[n][g * 4 + 2][c] * inv[c], o_acc[n][g * 4 + 2][2 + c] * inv[c]);
+                y.w = pack_bf16x2(o_acc[n][g * 4 + 3][c] * inv[c], o_acc[n][g * 4 + 3][2 + c] * inv[c]);
                 if (col < ncol) { *reinterpret_cast<uint4*>(op + col * (D * 2) + (64 * g + 8 * r) * 2) = y; }
               }
             }
@@ -910,8 +920,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int col = n * 8 + 2 * t + c;
+          for (int c = 0; c < CN; ++c) {
+            const int col = col_of(n, c);
             if (col < ncol) {
               if (r == 0) {
                 H.m[col] = m_run[n][c];
@@ -922,7 +932,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const int d = BITS == 16 ? 16 * i + 8 * h + r : 64 * (i / 4) + 8 * r + 2 * (i % 4) + h;
-                  to[col * D + entry_at<BITS>(col, d)] = o_acc[n][i][2 * h + c];
+                  to[col * D + entry_at<BITS, HALF>(col, d)] = o_acc[n][i][2 * h + c];
                 }
               }
             }
@@ -973,7 +983,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       const int i = turn * 32 + lane;  // four values of a column
       if (i >= ncol * (D / 4)) { continue; }
       const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-      const int at = col * (D / 4) + (entry_at<BITS>(col, d) >> 2);
+      const int at = col * (D / 4) + (entry_at<BITS, HALF>(col, d) >> 2);
       auto of = [&](int j) {
         return reinterpret_cast<const float4*>((j & 1) ? reinterpret_cast<const float*>(smem + (j >> 1) * A.ring_bytes)
                                                        : scratch0 + (j >> 1) * (A.cols * D))[at];
@@ -1003,8 +1013,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         add(s_f[j][col], s_fl[j][col], of(j));
       }
       if (BITS == 8) {  // entry_at exchanges values within the four
-        if (col & 2) { acc = make_float4(acc.y, acc.x, acc.w, acc.z); }
-        if (col & 4) { acc = make_float4(acc.z, acc.w, acc.x, acc.y); }
+        if (col & (HALF ? 1 : 2)) { acc = make_float4(acc.y, acc.x, acc.w, acc.z); }
+        if (col & (HALF ? 2 : 4)) { acc = make_float4(acc.z, acc.w, acc.x, acc.y); }
       }
       if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1138,7 +1148,7 @@ int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_ca
   return VPQ_OK;
 }
 
-template <int D, int BITS, int NT, int TM, int kWarps, int STAGES>
+template <int D, int BITS, int NT, bool HALF, int TM, int kWarps, int STAGES>
 int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   static_assert(kWarps <= kMaxWarps, "the workspace is sized for kMaxWarps");
   static_assert(NT * 8 * D * 4 <= STAGES * 2 * 16 * TM * (D * BITS / 8), "a warp's partial result fits its ring");
@@ -1148,7 +1158,7 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   a.stage_bytes = kStage + ((s.cols * D * 2 + 127) & ~127);
   a.ring_bytes = a.stage_bytes * STAGES;
   static int granted[64] = {};
-  auto kern = paged_attn_kernel<D, BITS, NT, TM, kWarps, STAGES>;
+  auto kern = paged_attn_kernel<D, BITS, NT, HALF, TM, kWarps, STAGES>;
   size_t smem = (size_t)kWarps * a.ring_bytes;
   const size_t first = (size_t)kWarps * s.cols * D * 4;
   if (smem + first <= 216 * 1024) {
@@ -1261,14 +1271,22 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   const int qh = d.q_heads;
   // Tokens of a unit, warps and stages. A stage holds 8 to 16 KB, so that a warp's copies in flight cover the
   // latency; the warps' rings fill the shared memory.
+  const bool half = s.cols <= 4;
+#define VPQ_GO(D, BITS, TM, W, S)                                    \
+  if (half) { return launch<D, BITS, 1, true, TM, W, S>(a, s, qh, st); } \
+  return launch<D, BITS, 1, false, TM, W, S>(a, s, qh, st);
   switch (cache_host->head_dim) {
     case 64:
-      if (q8) { return two ? launch<64, 8, 2, 2, 8, 3>(a, s, qh, st) : launch<64, 8, 1, 2, 8, 4>(a, s, qh, st); }
-      return two ? launch<64, 16, 2, 1, 8, 3>(a, s, qh, st) : launch<64, 16, 1, 1, 8, 4>(a, s, qh, st);
+      if (two) { return q8 ? launch<64, 8, 2, false, 2, 8, 3>(a, s, qh, st) : launch<64, 16, 2, false, 1, 8, 3>(a, s, qh, st); }
+      if (q8) { VPQ_GO(64, 8, 2, 8, 4) }
+      VPQ_GO(64, 16, 1, 8, 4)
     case 128:
-      if (q8) { return two ? launch<128, 8, 2, 2, 8, 2>(a, s, qh, st) : launch<128, 8, 1, 2, 8, 2>(a, s, qh, st); }
-      return two ? launch<128, 16, 2, 1, 8, 2>(a, s, qh, st) : launch<128, 16, 1, 1, 8, 2>(a, s, qh, st);
+      if (two) { return q8 ? launch<128, 8, 2, false, 2, 8, 2>(a, s, qh, st) : launch<128, 16, 2, false, 1, 8, 2>(a, s, qh, st); }
+      if (q8) { VPQ_GO(128, 8, 2, 8, 2) }
+      VPQ_GO(128, 16, 1, 8, 2)
     default:
-      return q8 ? launch<256, 8, 1, 1, 8, 2>(a, s, qh, st) : launch<256, 16, 1, 1, 5, 2>(a, s, qh, st);
+      if (q8) { VPQ_GO(256, 8, 1, 8, 2) }
+      VPQ_GO(256, 16, 1, 5, 2)
   }
+#undef VPQ_GO
 }
