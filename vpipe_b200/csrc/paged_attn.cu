@@ -1119,7 +1119,7 @@ struct Shape {
   int group, cols, nt, blocks, ctas;
   size_t heads, ml, part, scratch, total;  // byte offsets in the workspace, and its size
 };
-constexpr int kMaxWarps = 10;  // of any instantiation: the scratch has room for them
+constexpr int kMaxWarps = 16;  // of any instantiation: the scratch has room for them
 
 int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_cache* c, Shape* s) {
   if (!d || !c) { return fail(VPQ_ERR_INVALID_ARG, "%s: null descriptor", who); }
@@ -1277,9 +1277,9 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   return launch<D, BITS, 1, false, TM, W, S>(a, s, qh, st);
   switch (cache_host->head_dim) {
     case 64:
-      if (two) { return q8 ? launch<64, 8, 2, false, 2, 8, 3>(a, s, qh, st) : launch<64, 16, 2, false, 1, 8, 3>(a, s, qh, st); }
-      if (q8) { VPQ_GO(64, 8, 2, 8, 4) }
-      VPQ_GO(64, 16, 1, 8, 4)
+      if (two) { return q8 ? launch<64, 8, 2, false, 2, 12, 2>(a, s, qh, st) : launch<64, 16, 2, false, 1, 8, 3>(a, s, qh, st); }
+      if (q8) { VPQ_GO(64, 8, 2, 16, 2) }
+      VPQ_GO(64, 16, 1, 16, 2)
     case 128:
       if (two) { return q8 ? launch<128, 8, 2, false, 2, 8, 2>(a, s, qh, st) : launch<128, 16, 2, false, 1, 8, 2>(a, s, qh, st); }
       if (q8) { VPQ_GO(128, 8, 2, 8, 2) }
