@@ -480,6 +480,28 @@ def test_attention_8_bit_scales_of_any_size(vpq, gain):
     check_attention(vpq, q, c, table, [n], scale=0.1)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_averages_many_values(vpq, bits):
+    """Equal weights over 131072 tokens, each warp adding up tens of thousands of them: what is left of the values is
+    a three-hundredth of each, and must not drown in the sums it is taken from. (All sequences share the pages.)"""
+    g = gen(12)
+    n, D, B = 131072, 128, 600
+    c = layouts(vpq, "dense", n // 64, 64, 1, D, bits)
+    t = torch.arange(n, device="cuda")
+    v = normal(g, n, 1, D).to(BF)
+    vpq.ops.kv_store(v, v, c, t)
+    q = torch.zeros(B, 1, D, dtype=BF, device="cuda")
+    table = torch.arange(n // 64, dtype=torch.int32, device="cuda").expand(B, -1).contiguous()
+    got = vpq.ops.paged_attention(q, c, table, torch.full((B,), n, dtype=torch.int32, device="cuda")).to(F64)[:, 0]
+    want = held(c)[1].reshape(n, D).mean(0)
+    # A weight is 1, exact in bf16. For 8 bits 2^15 s / 2^k is rounded to fp16: at most H, independently of the codes
+    # (128 s is at most 5.5 / 255 * 128 here), so eight standard deviations of the mean; and each unit's products and
+    # its sum are off by a few f32 steps of 255 s times its weights. bf16: a sum in f32, cut at each of 8192 steps.
+    half = 128 * 11.0 / 255
+    tol = U * want.abs() * (1 + U) + (8 * H * half / math.sqrt(n) + 16 * E * half if bits == 8 else 8192 * 2 * E * want.abs() + 16 * E * 5.5)
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
 def test_attention_nan_and_infinity_stay_with_their_sequence(vpq):
     g = gen(13)
     lens = [40, 50, 60]

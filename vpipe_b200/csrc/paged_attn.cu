@@ -23,8 +23,8 @@
 //   q . k = sum_g s_g (q . c)_g + b_g sum_g q
 //   o     = sum_t p'_tg c - 128 sum_t p'_tg + sum_t p_t (b_tg + 128 s_tg),   p'_tg = p_t s_tg rounded to fp16
 // and scales and biases act on 16 x 8 scores instead of 16 x head_dim values. The middle term of o (one
-// product with a constant operand per group) takes the codes' mean out of the rounding of p', which it
-// would amplify by about three. q is scaled by a power of two per head to fill fp16's range (exact up to 2^-39 of
+// product with a constant operand per group) takes the codes' mean out of the rounding of p' and, subtracted
+// unit by unit, out of the sums. q is scaled by a power of two per head to fill fp16's range (exact up to 2^-39 of
 // the head's largest value); p s is taken relative to a running power of two above every scale, times 2^15,
 // which keeps its rounding at 2^-11 relative down to 2^-29.
 // In a bf16 cache p is rounded to bf16 (2^-8) and the sum of weights adds the rounded p, so the
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 
   float o_acc[NT][MT][4];
   float m_run[NT][CN], l_run[NT][CN];
-  float o_mean[NT][G][4], o_bias[NT][G][CN], q_sum[NT][G][CN], q_mul[NT][CN];  // 8 bits
+  float o_bias[NT][G][CN], q_sum[NT][G][CN], q_mul[NT][CN];  // 8 bits
   uint32_t qf[NT][D / 16][2];
   int sigma = -100;      // 8 bits: exponent of the power of two above every value scale so far
   bool run_begins = false, first_run = true;
@@ -599,7 +599,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
             for (int g = 0; g < G; ++g) {
               q_sum[n][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * t + c) * 4) * A.scale_log2;
               o_bias[n][g][c] = 0.0f;
-              o_mean[n][g][0] = o_mean[n][g][1] = o_mean[n][g][2] = o_mean[n][g][3] = 0.0f;
             }
           }
         }
@@ -746,10 +745,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
           if (BITS == 8) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              o_bias[n][g][c] *= f;
-              o_mean[n][g][c] *= fo;
-            }
+            for (int g = 0; g < G; ++g) { o_bias[n][g][c] *= f; }
           }
         }
       }
@@ -768,9 +764,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     }
 
     // ---- O^T += V^T P^T
+    if (BITS == 16) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      if (BITS == 16) {
+      for (int i = 0; i < TM; ++i) {
         uint32_t b[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -790,28 +786,37 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
 #pragma unroll
           for (int n = 0; n < NT; ++n) { mma<false>(o_acc[n][k], a, b[n][0], b[n][1]); }
         }
-      } else {
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int c = 0; c < CN; ++c) { l_run[n][c] += s[i][n][c] + s[i][n][2 + c]; }
         }
+      }
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          uint32_t b[NT][2];
+      for (int g = 0; g < G; ++g) {
+        uint32_t b[TM][NT][2], x[TM][2][4];
+        float mean[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { mean[n][0] = mean[n][1] = mean[n][2] = mean[n][3] = 0.0f; }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float sc = lo16(vp[i][h][g]), f = sc * up, bb = __fmaf_rn(128.0f, sc, hi16(vp[i][h][g]));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              b[n][h] = movm(pack_f16x2(s[i][n][2 * h] * f, HALF ? 0.0f : s[i][n][2 * h + 1] * f));
+              b[i][n][h] = movm(pack_f16x2(s[i][n][2 * h] * f, HALF ? 0.0f : s[i][n][2 * h + 1] * f));
 #pragma unroll
               for (int c = 0; c < CN; ++c) { o_bias[n][g][c] = __fmaf_rn(s[i][n][2 * h + c], bb, o_bias[n][g][c]); }
             }
           }
-          const uint32_t mean[4] = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // the code 128
+          const uint32_t k128[4] = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // the code 128
 #pragma unroll
-          for (int n = 0; n < NT; ++n) { mma<true>(o_mean[n][g], mean, b[n][0], b[n][1]); }
+          for (int n = 0; n < NT; ++n) { mma<true>(mean[n], k128, b[i][n][0], b[i][n][1]); }
           // codes 64 g + 8 r + 0..7 of tokens 2t, 2t + 1, 2t + 8, 2t + 9. A row's eight lanes of equal t read 64
           // bytes; the swizzle puts the four token pairs of a half warp into different banks.
           uint2 w[4];
@@ -820,19 +825,30 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
             const int row = 2 * t + (j & 1) + (j >> 1) * 8;
             w[j] = lds64(vt + (16 * i + row) * kRow + ((4 * g + (r >> 1)) ^ swz_v<D, BITS>(row)) * 16 + (r & 1) * 8);
           }
-          uint32_t x[2][4];  // per token pair: values 0|1, 2|3, 4|5, 6|7 as bytes (even token, odd token, ...)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            x[h][0] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x5140);
-            x[h][1] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x7362);
-            x[h][2] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x5140);
-            x[h][3] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x7362);
+          for (int h = 0; h < 2; ++h) {  // per token pair: values 0|1, 2|3, 4|5, 6|7 as bytes (even token, odd token, ...)
+            x[i][h][0] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x5140);
+            x[i][h][1] = __byte_perm(w[2 * h].x, w[2 * h + 1].x, 0x7362);
+            x[i][h][2] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x5140);
+            x[i][h][3] = __byte_perm(w[2 * h].y, w[2 * h + 1].y, 0x7362);
           }
+        }
+        // The products of a unit start from zero, and what is added up is their distance from the mean's: the sums
+        // over a long sequence would otherwise be 128 times the weights, next to which the product unit cuts off
+        // what the values differ by (measured at 131072 equal weights: a third of the result).
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // rows r, r + 8 of this block: values 64 g + 8 r + 2 k, + 1
-            const uint32_t a[4] = {codes<false>(x[0][k]), codes<true>(x[0][k]), codes<false>(x[1][k]), codes<true>(x[1][k])};
+        for (int k = 0; k < 4; ++k) {  // rows r, r + 8 of this block: values 64 g + 8 r + 2 k, + 1
 #pragma unroll
-            for (int n = 0; n < NT; ++n) { mma<true>(o_acc[n][g * 4 + k], a, b[n][0], b[n][1]); }
+          for (int n = 0; n < NT; ++n) {
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              const uint32_t a[4] = {codes<false>(x[i][0][k]), codes<true>(x[i][0][k]), codes<false>(x[i][1][k]),
+                                     codes<true>(x[i][1][k])};
+              mma<true>(c, a, b[i][n][0], b[i][n][1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 3 - CN) { o_acc[n][g * 4 + k][e] += c[e] - mean[n][e & 1]; }
           }
         }
       }
@@ -860,8 +876,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           for (int i = 0; i < MT; ++i) {
 #pragma unroll
             for (int e = 0; e < 4; e += 3 - CN) {
-              o_acc[n][i][e] =
-                  __fmaf_rn((o_acc[n][i][e] - o_mean[n][i / 4][e & 1]) * 16777216.0f, o_mul, o_bias[n][i / 4][e & (CN - 1)]);
+              o_acc[n][i][e] = __fmaf_rn(o_acc[n][i][e] * 16777216.0f, o_mul, o_bias[n][i / 4][e & (CN - 1)]);
             }
           }
         }

@@ -476,6 +476,8 @@ def _elsewhere(dev, stream) -> bool:
     """Whether a call for tensors of device `dev` has to switch to it or to `stream` first."""
     if dev < 0:
         raise ValueError("vpipe_b200.ops: rows must be bfloat16 on a CUDA device (no CPU path)")
+    if stream is not None and stream.device.index != dev:
+        raise ValueError(f"vpipe_b200.ops: the stream belongs to {stream.device}, the tensors to cuda:{dev}")
     return stream is not None or dev != torch.cuda.current_device()
 
 
