@@ -414,14 +414,14 @@ bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
 
 // One head per lane group while the launch is too small to fill the machine (a decode step lives by
 // latency), four once there are waves of them.
-bool is_wide(int64_t M, int heads, int D) { return M * heads > (int64_t)num_sms() * 8 * (256 / (D / 8)) * 2; }
+bool is_wide(int64_t M, int heads, int D, int sms) { return M * heads > (int64_t)sms * 8 * (256 / (D / 8)) * 2; }
 
 struct Launch {
   dim3 grid, block;
 };
 // Deals `parts` parts of heads[] heads each. The blocks of all parts together are enough for `waves` times what the SMs
 // hold at 64 registers a thread, shared out by the parts' heads.
-void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, Deal* deals, Launch* l) {
+void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int sms, Deal* deals, Launch* l) {
   const int groups = 256 / (D / 8);
   int total = 0, threads = 32;
   for (int i = 0; i < parts; ++i) { total += heads[i]; }
@@ -433,7 +433,7 @@ void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, Dea
     d.per_block = (d.chunks + d.token_blocks - 1) / d.token_blocks;
     d.tokens = groups / d.per_block;
     // few tokens: spread them
-    if (d.token_blocks > 1 || M < num_sms()) { d.tokens = 1; }
+    if (d.token_blocks > 1 || M < sms) { d.tokens = 1; }
     d.rcp = (65536u + d.per_block - 1) / d.per_block;
     threads = std::max(threads, d.tokens * d.per_block * (D / 8));
   }
@@ -441,7 +441,7 @@ void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, Dea
   for (int i = 0; i < parts; ++i) {
     Deal& d = deals[i];
     const int64_t need = (M + d.tokens - 1) / d.tokens;
-    const int64_t cap = (int64_t)num_sms() * (1024 / threads) * waves * heads[i] / total / d.token_blocks;
+    const int64_t cap = (int64_t)sms * (1024 / threads) * waves * heads[i] / total / d.token_blocks;
     const int64_t blocks = std::min(need, std::max<int64_t>(cap, 1));
     d.first = first;
     d.step = (uint32_t)(blocks * d.tokens);
@@ -470,8 +470,9 @@ template <int MODE>
 int launch_norm(const QkArgs& a0, int D, cudaStream_t st) {
   QkArgs a = a0;
   Launch l;
-  const bool wide = is_wide(a.M, a.heads[0] + (MODE ? 2 : 1) * a.heads[1], D);
-  deal(a.M, a.heads, MODE ? 3 : 2, wide ? 4 : 1, 4, D, a.deal, &l);
+  const int sms = num_sms();
+  const bool wide = is_wide(a.M, a.heads[0] + (MODE ? 2 : 1) * a.heads[1], D, sms);
+  deal(a.M, a.heads, MODE ? 3 : 2, wide ? 4 : 1, 4, D, sms, a.deal, &l);
   if (D == 64) {
     return wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, l, st, a)
                 : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, l, st, a);
@@ -488,9 +489,10 @@ template <int BITS, bool STORE>
 int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
   CopyArgs a = a0;
   Launch l;
-  const bool wide = a.kv.kv_heads >= 4 && is_wide(a.M, 2 * a.kv.kv_heads, D);
+  const int sms = num_sms();
+  const bool wide = a.kv.kv_heads >= 4 && is_wide(a.M, 2 * a.kv.kv_heads, D, sms);
   const int heads[2] = {a.kv.kv_heads, a.kv.kv_heads};
-  deal(a.M, heads, 2, wide ? 4 : 1, 8, D, a.deal, &l);
+  deal(a.M, heads, 2, wide ? 4 : 1, 8, D, sms, a.deal, &l);
   if (D == 64) {
     return wide ? launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 1>, l, st, a);
   }

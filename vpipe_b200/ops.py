@@ -549,29 +549,33 @@ class PagedKVCache:
 
 
 def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, k_out):
-    shape = q.shape
-    if len(shape) != 3 or k.dim() != 3:
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 3 or len(kshape) != 3:
         raise ValueError("vpipe_b200.ops: q and k must be bfloat16 [rows, heads, head_dim]")
     M, hq, D = shape
-    hkv = k.shape[1]
-    kshape = (M, hkv, D)
+    hkv = kshape[1]
+    if kshape[0] != M or kshape[2] != D:
+        kshape = (M, hkv, D)  # what _heads will say
     pq, sq = _heads("q", q, dev, shape)
     pk, sk = _heads("k", k, dev, kshape)
     pv, sv = _heads("v", v, dev, kshape) if v is not None else (None, 0)
     po, so = _heads("q_out", q_out, dev, shape)
     pj, sj = _heads("k_out", k_out, dev, kshape) if k_out is not None else (None, 0)
-    wq = _index("q_norm_w", q_norm_w, dev, _BF16, (D,)) if q_norm_w is not None else None
-    wk = _index("k_norm_w", k_norm_w, dev, _BF16, (D,)) if k_norm_w is not None else None
-    pt, pp, rows, rot = None, None, 0, 0
+    wq = wk = pt = pp = None
+    rows = rot = 0
+    if q_norm_w is not None:
+        wq = _index("q_norm_w", q_norm_w, dev, _BF16, (D,))
+    if k_norm_w is not None:
+        wk = _index("k_norm_w", k_norm_w, dev, _BF16, (D,))
     if cos_sin is not None:
-        if cos_sin.dim() != 2:
+        table = cos_sin.shape
+        if len(table) != 2:
             raise ValueError("vpipe_b200.ops: cos_sin must be float32 [rows, rot_dim]")
-        rows, rot = cos_sin.shape
-        pt = _index("cos_sin", cos_sin, dev, _F32, (rows, rot))
+        rows, rot = table
+        pt = _index("cos_sin", cos_sin, dev, _F32, table)
     if positions is not None:
         pp = _index("positions", positions, dev, _I32, (M,))
-    return _lib.QkDesc(pq, pk, pv, po, pj, sq, sk, sv, so, sj, wq, wk, pt, pp, M, rows, hq, hkv, D, rot, int(interleaved),
-                       eps)
+    return _lib.QkDesc(pq, pk, pv, po, pj, sq, sk, sv, so, sj, wq, wk, pt, pp, M, rows, hq, hkv, D, rot, interleaved, eps)
 
 
 def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=None, eps=1e-6, interleaved=False,
@@ -588,7 +592,9 @@ def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=Non
     k_out = torch.empty_like(k, memory_format=_DENSE) if k_out is None else k_out
     d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, None, q_out, k_out)
     if d.M != 0:
-        check(lib().vpq_qk_norm_rope_bf16(C.byref(d), _raw_stream(dev)))
+        rc = lib().vpq_qk_norm_rope_bf16(C.byref(d), _raw_stream(dev))
+        if rc != 0:
+            check(rc)
     return q_out, k_out
 
 
