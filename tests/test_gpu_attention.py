@@ -585,6 +585,64 @@ def test_attention_in_a_graph_follows_the_lengths(vpq, bits):
             assert torch.equal(out, vpq.ops.paged_attention(q, c, table, dl)), (step, now)
 
 
+@pytest.mark.parametrize("hkv", [8, 1])
+def test_attention_workspace_contents_do_not_matter(vpq, hkv):
+    """The workspace needs no initialisation: whatever is in it, also what the call before left there, the result is
+    the same, call after call."""
+    import ctypes as C
+
+    from vpipe_b200 import _lib
+    g = gen(20)
+    lens = [3000, 0, 777, 20011]
+    c, table = filled(vpq, g, "dense", lens, 16, hkv, 128, 16)
+    q = normal(g, len(lens), 4 * hkv, 128).to(BF)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = check_attention(vpq, q, c, table, lens)
+    out = torch.empty_like(want)
+    d = _lib.PagedAttentionDesc(q.data_ptr(), out.data_ptr(), 0, 0, table.data_ptr(), dl.data_ptr(), 0, len(lens),
+                                table.shape[1], q.shape[1], 0, 0.0)
+    L = vpq.lib()
+    need = L.vpq_paged_attention_bytes(C.byref(d), c.ref)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    for fill in (0, 255, None, None, 1, "random", None, None):
+        if fill == "random":
+            ws.copy_(torch.randint(0, 256, (need,), generator=g, device="cuda", dtype=torch.uint8))
+        elif fill is not None:
+            ws.fill_(fill)
+        out.fill_(float("nan"))
+        assert L.vpq_paged_attention_bf16(C.byref(d), c.ref, ws.data_ptr(), need, st) == 0
+        assert torch.equal(out, want), fill
+
+
+def test_attention_repeats_itself(vpq):
+    """Hundreds of calls and replays over uneven batches, all CTAs of a call meeting in the joins: bit for bit the same."""
+    g = gen(22)
+    for trial in range(6):
+        B = [1, 3, 40, 200, 7, 64][trial]
+        lens = (torch.rand(B, generator=g, device="cuda") ** 3 * 3000).int()
+        lens[0] = 2999
+        c, table = filled(vpq, g, "dense", [3000], 16, [8, 2, 8, 4, 16, 3][trial], 64, 8 if trial % 2 else 16)
+        table = table.expand(B, -1).contiguous()
+        q = normal(g, B, 2 * c.kv_heads, 64).to(BF)
+        want = vpq.ops.paged_attention(q, c, table, lens)
+        ref, tol = ref_attention(q, c, table, lens.tolist(), 1 / 8, 0)
+        assert ((want.to(F64) - ref).abs() <= tol).all()
+        bad = torch.zeros((), dtype=torch.bool, device="cuda")
+        for _ in range(60):
+            bad |= (vpq.ops.paged_attention(q, c, table, lens) != want).any()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [vpq.ops.paged_attention(q, c, table, lens) for _ in range(4)]
+        for _ in range(40):
+            for o in outs:
+                o.fill_(float("nan"))
+            graph.replay()
+            for o in outs:
+                bad |= (o != want).any()
+        assert not bad.item(), trial
+
+
 def test_calls_on_another_stream(vpq):
     g = gen(21)
     lens = [500, 20]
