@@ -423,6 +423,51 @@ def test_attention_window(vpq, bits, window):
     assert indexes_reported(vpq) == 0
 
 
+def with_wide_tables(monkeypatch):
+    """From here on page tables have room for thousands of tokens more than any sequence: how a call is split goes by
+    that room, and the narrow tables of the tests above only ever give each sequence a CTA of its own."""
+    narrow = filled
+
+    def wide(*args, **kw):
+        c, table = narrow(*args, **kw)
+        return c, torch.nn.functional.pad(table, (0, 600), value=1 << 30)
+    monkeypatch.setitem(globals(), "filled", wide)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("D,hq,hkv", [(128, 32, 8), (128, 1, 1), (128, 5, 1), (128, 7, 1), (128, 18, 2), (128, 16, 1),
+                                      (128, 17, 1), (128, 71, 1), (64, 12, 12), (64, 4, 1), (64, 9, 1), (64, 40, 1),
+                                      (256, 8, 1), (256, 9, 1), (256, 16, 1), (256, 6, 3)])
+def test_attention_head_layouts_wide_table(vpq, monkeypatch, bits, D, hq, hkv):
+    with_wide_tables(monkeypatch)
+    test_attention_head_layouts(vpq, bits, D, hq, hkv)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_wide_tables(vpq, monkeypatch, bits):
+    with_wide_tables(monkeypatch)
+    for D in (64, 128, 256):
+        test_attention_lengths(vpq, D, bits)
+    test_attention_sharp_and_flat_scores(vpq, bits)
+    test_attention_bad_pages_and_lengths(vpq, bits)
+    test_attention_in_a_graph_follows_the_lengths(vpq, bits)
+    if bits == 16:
+        test_attention_nan_and_infinity_stay_with_their_sequence(vpq)
+        test_attention_strided_queries_and_outputs(vpq)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("B,hkv", [(1, 1), (3, 8), (18, 8), (19, 8), (148, 1), (149, 1)])
+def test_attention_full_tables(vpq, bits, B, hkv):
+    """Sequences as long as their tables, empty and nearly empty ones beside them, at the sizes where the split changes."""
+    g = gen(B)
+    for n in (16, 496, 512, 528, 1024):
+        lens = [n, 0, 1, n - 1, n // 2][:B] + [3] * (B - 5)
+        c, table = filled(vpq, g, "dense", lens, 16, hkv, 128, bits)
+        table = table[:, :n // 16].contiguous()
+        check_attention(vpq, normal(g, B, 4 * hkv, 128).to(BF), c, table, lens)
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_attention_long_and_uneven(vpq, bits):
     g = gen(77)

@@ -11,7 +11,8 @@
 // captured graph serves any of them. Each warp streams its run through its own ring in shared memory
 // (cp.async, no barrier in the loop). What a warp has of a (sequence, head) that it shares with others is
 // joined within the CTA through shared memory, and across CTAs by a second small kernel over partial
-// results in the workspace; both joins add in the line's order, so results do not depend on timing.
+// results in the workspace; both joins add in the line's order, so results do not depend on timing. Few short sequences go
+// without a line: a CTA each per key head ("solo").
 //
 // Matrix products are m16n8k16 with the TOKENS as the 16 rows and up to eight query heads as the eight
 // columns (a GQA group of four or eight wastes half or nothing; queries as rows would waste three quarters
@@ -32,6 +33,7 @@
 #include "vpq_kv.cuh"
 #include "vpq_sm100.cuh"
 
+#include <algorithm>
 #include <climits>
 
 namespace vpq {
@@ -68,6 +70,7 @@ struct AttnArgs {
   int blocks;        // column blocks of a key head
   int hk;            // kv_heads * blocks
   uint32_t cta_rcp;  // 2^32 / CTAs, rounded up: a quotient may come out one too large, which is as good a cut
+  bool solo;         // a CTA per (sequence, column block), and no second kernel
   bool dense;        // rows of a page's head lie back to back
   bool few;          // at most 32 sequences, and few enough units for 32-bit sums
   float scale_log2;
@@ -266,61 +269,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
   // ---- this CTA's run of the line of units. Up to 32 sequences: every warp looks at all of them; more: a
   // thread at a few neighbouring ones each.
   if (lane < 2) { s_entry[warp * 2 + lane].b = -1; }
-  if (tid == 0) { A.heads[blockIdx.x].last = -1; }
-  const int cpt = A.few ? 1 : (A.batch + kWarps * 32 - 1) / (kWarps * 32);
-  const int me = A.few ? lane : tid;
-  const int b_lo = min(me * cpt, A.batch), b_hi = min(b_lo + cpt, A.batch);
-  int64_t mine = 0;
-  int2 seen = make_int2(0, 0);  // token range of the last of them
-  for (int b = b_lo; b < b_hi; ++b) {
-    token_range(A, b, seen.x, seen.y);
-    mine += span_of<kUnit>(seen.x, seen.y);
-    if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(&g_attn_status, kBadLength); }
-  }
-  int64_t excl, total;  // places (of one head) before the first of them, and of all
-  if (A.few) {
-    int incl = (int)mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) { incl += o; }
-    }
-    excl = incl - (int)mine;
-    total = __shfl_sync(0xffffffffu, incl, 31);
-  } else {
-    int64_t incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) { incl += o; }
-    }
-    if (lane == 31) { s_wsum[warp] = incl; }
-    __syncthreads();
-    excl = incl - mine;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) { excl += s_wsum[w]; }
-      total += s_wsum[w];
-    }
-    s_excl[tid] = excl;
-    s_range[tid] = seen;
-    __syncthreads();
-  }
-  const int64_t places = total * A.hk;
-  // (32-bit numbers by the reciprocal that the host has made of the number of CTAs)
-  int64_t per_cta = (places + gridDim.x) >> 31 == 0 ? (int64_t)__umulhi((uint32_t)places + gridDim.x - 1, A.cta_rcp)
-                                                    : (places + gridDim.x - 1) / gridDim.x;
-  per_cta = per_cta > kWarps ? per_cta : kWarps;
-  const int64_t cta0 = (int64_t)blockIdx.x * per_cta;
-  if (cta0 >= places) { return; }  // the whole CTA
-  const int64_t cta1 = cta0 + per_cta < places ? cta0 + per_cta : places;
-  const int64_t per_warp = (cta1 - cta0 + kWarps - 1) / kWarps;
-  const int64_t u0 = cta0 + warp * per_warp;
-  const int64_t u1 = u0 + per_warp < cta1 ? u0 + per_warp : cta1;
-  int left = u0 < u1 ? (int)(u1 - u0) : 0;  // places of the line that this warp has yet to request
-  int todo = 0;                             // units requested and not yet computed
-
+  int left = 0;  // places of the line that this warp has yet to request
+  int todo = 0;  // units requested and not yet computed
+  int64_t cta0 = 0, cta1 = 0, per_cta = 1;
   // ---- the loader's place in the line
   int lb = 0, lh = 0, lkv = 0, lblk = 0, ltile = 0, ltile0 = 0, ltile_end = 0, lstart = 0, llen = 0;
   int pg = 0, off = 0;     // page-table column and token offset in the page
@@ -342,49 +293,127 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
       if (o == A.kv.page_size) { o = 0, ++c; }
     }
   };
-  if (left > 0) {
-    // who looked at u0's sequence: the last whose sequences begin at or before it
-    int64_t at;
-    if (A.few) {
-      lb = 31 - __clz(__ballot_sync(0xffffffffu, excl * A.hk <= u0));
-      at = __shfl_sync(0xffffffffu, excl, lb);
-      lstart = __shfl_sync(0xffffffffu, seen.x, lb), llen = __shfl_sync(0xffffffffu, seen.y, lb);
-    } else {
-      int64_t upto = 0;
-      int tw = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (upto * A.hk <= u0) { tw = w; }
-        upto += s_wsum[w];
-      }
-      const int64_t ex = s_excl[tw * 32 + lane];
-      const int tl = 31 - __clz(__ballot_sync(0xffffffffu, ex * A.hk <= u0));
-      at = __shfl_sync(0xffffffffu, ex, tl);
-      lb = (tw * 32 + tl) * cpt;
-      if (cpt == 1) {
-        lstart = s_range[tw * 32 + tl].x, llen = s_range[tw * 32 + tl].y;
-      } else {
-        for (;; ++lb) {
-          token_range(A, lb, lstart, llen);
-          const int n = span_of<kUnit>(lstart, llen);
-          if ((at + n) * A.hk > u0) { break; }
-          at += n;
-        }
-      }
-    }
-    ltile0 = lstart / kUnit;
-    ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
-    const int64_t in_seq = u0 - at * A.hk;
-    const int span = ltile_end - ltile0 + 1;
-    lh = (int)div_u(in_seq, span);
-    const int place = (int)(in_seq - (int64_t)lh * span);
-    ltile = ltile0 + (place > 0 ? place - 1 : 0);
-    if (place == 0) { --left; }
+  if (A.solo) {
+    // all of one (sequence, column block), a warp having a stretch of its units
+    lb = (int)(blockIdx.x / (uint32_t)A.hk), lh = (int)(blockIdx.x - (uint32_t)lb * (uint32_t)A.hk);
     lkv = A.blocks == 1 ? lh : lh / A.blocks;
     lblk = lh - lkv * A.blocks;
+    token_range(A, lb, lstart, llen);
+    if (tid == 0 && lh == 0 && __ldg(A.seq_lens + lb) > llen) { atomicOr(&g_attn_status, kBadLength); }
+    const int n = units_of<kUnit>(lstart, llen);
+    if (n == 0) {  // no token: zeros
+      const int h0 = lkv * A.group + lblk * A.cols, ncol = min(A.cols, A.group - lblk * A.cols);
+      uint4* row = reinterpret_cast<uint4*>(A.out + (int64_t)lb * A.out_stride + (int64_t)h0 * (D * 2));
+      for (int i = tid; i < ncol * (D / 8); i += kWarps * 32) { row[i] = make_uint4(0, 0, 0, 0); }
+      return;
+    }
+    const int per_warp = (n + kWarps - 1) / kWarps;
+    left = max(0, min(per_warp, n - warp * per_warp));
+    ltile0 = lstart / kUnit;
+    ltile_end = ltile0 + n;
+    ltile = ltile0 + warp * per_warp;
     if (left > 0) {
       enter();
       fetch_pages();
+    }
+  } else {
+    if (tid == 0) { A.heads[blockIdx.x].last = -1; }
+    const int cpt = A.few ? 1 : (A.batch + kWarps * 32 - 1) / (kWarps * 32);
+    const int me = A.few ? lane : tid;
+    const int b_lo = min(me * cpt, A.batch), b_hi = min(b_lo + cpt, A.batch);
+    int64_t mine = 0;
+    int2 seen = make_int2(0, 0);  // token range of the last of them
+    for (int b = b_lo; b < b_hi; ++b) {
+      token_range(A, b, seen.x, seen.y);
+      mine += span_of<kUnit>(seen.x, seen.y);
+      if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(&g_attn_status, kBadLength); }
+    }
+    int64_t excl, total;  // places (of one head) before the first of them, and of all
+    if (A.few) {
+      int incl = (int)mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) { incl += o; }
+      }
+      excl = incl - (int)mine;
+      total = __shfl_sync(0xffffffffu, incl, 31);
+    } else {
+      int64_t incl = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) { incl += o; }
+      }
+      if (lane == 31) { s_wsum[warp] = incl; }
+      __syncthreads();
+      excl = incl - mine;
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) { excl += s_wsum[w]; }
+        total += s_wsum[w];
+      }
+      s_excl[tid] = excl;
+      s_range[tid] = seen;
+      __syncthreads();
+    }
+    const int64_t places = total * A.hk;
+    // (32-bit numbers by the reciprocal that the host has made of the number of CTAs)
+    per_cta = (places + gridDim.x) >> 31 == 0 ? (int64_t)__umulhi((uint32_t)places + gridDim.x - 1, A.cta_rcp)
+                                                      : (places + gridDim.x - 1) / gridDim.x;
+    per_cta = per_cta > kWarps ? per_cta : kWarps;
+    cta0 = (int64_t)blockIdx.x * per_cta;
+    if (cta0 >= places) { return; }  // the whole CTA
+    cta1 = cta0 + per_cta < places ? cta0 + per_cta : places;
+    const int64_t per_warp = (cta1 - cta0 + kWarps - 1) / kWarps;
+    const int64_t u0 = cta0 + warp * per_warp;
+    const int64_t u1 = u0 + per_warp < cta1 ? u0 + per_warp : cta1;
+    left = u0 < u1 ? (int)(u1 - u0) : 0;
+    if (left > 0) {
+      // who looked at u0's sequence: the last whose sequences begin at or before it
+      int64_t at;
+      if (A.few) {
+        lb = 31 - __clz(__ballot_sync(0xffffffffu, excl * A.hk <= u0));
+        at = __shfl_sync(0xffffffffu, excl, lb);
+        lstart = __shfl_sync(0xffffffffu, seen.x, lb), llen = __shfl_sync(0xffffffffu, seen.y, lb);
+      } else {
+        int64_t upto = 0;
+        int tw = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (upto * A.hk <= u0) { tw = w; }
+          upto += s_wsum[w];
+        }
+        const int64_t ex = s_excl[tw * 32 + lane];
+        const int tl = 31 - __clz(__ballot_sync(0xffffffffu, ex * A.hk <= u0));
+        at = __shfl_sync(0xffffffffu, ex, tl);
+        lb = (tw * 32 + tl) * cpt;
+        if (cpt == 1) {
+          lstart = s_range[tw * 32 + tl].x, llen = s_range[tw * 32 + tl].y;
+        } else {
+          for (;; ++lb) {
+            token_range(A, lb, lstart, llen);
+            const int n = span_of<kUnit>(lstart, llen);
+            if ((at + n) * A.hk > u0) { break; }
+            at += n;
+          }
+        }
+      }
+      ltile0 = lstart / kUnit;
+      ltile_end = ltile0 + units_of<kUnit>(lstart, llen);
+      const int64_t in_seq = u0 - at * A.hk;
+      const int span = ltile_end - ltile0 + 1;
+      lh = (int)div_u(in_seq, span);
+      const int place = (int)(in_seq - (int64_t)lh * span);
+      ltile = ltile0 + (place > 0 ? place - 1 : 0);
+      if (place == 0) { --left; }
+      lkv = A.blocks == 1 ? lh : lh / A.blocks;
+      lblk = lh - lkv * A.blocks;
+      if (left > 0) {
+        enter();
+        fetch_pages();
+      }
     }
   }
 
@@ -1132,6 +1161,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
 // ---------------------------------------------------------------- host side
 struct Shape {
   int group, cols, nt, blocks, ctas;
+  int64_t capacity;  // tokens that a row of the page table can name
   size_t heads, ml, part, scratch, total;  // byte offsets in the workspace, and its size
 };
 constexpr int kMaxWarps = 16;  // of any instantiation: the scratch has room for them
@@ -1153,6 +1183,7 @@ int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_ca
   s->cols = s->group < 8 * s->nt ? s->group : 8 * s->nt;
   s->blocks = (s->group + s->cols - 1) / s->cols;
   s->ctas = num_sms();
+  s->capacity = (int64_t)d->max_pages * c->page_size;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t row = (size_t)s->cols * c->head_dim * 4;
   s->heads = 0;
@@ -1168,7 +1199,8 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   static_assert(kWarps <= kMaxWarps, "the workspace is sized for kMaxWarps");
   static_assert(NT * 8 * D * 4 <= STAGES * 2 * 16 * TM * (D * BITS / 8), "a warp's partial result fits its ring");
   constexpr int kStage = 2 * 16 * TM * (D * BITS / 8) + (BITS == 8 ? 2 * 16 * TM * (D / kKvGroup) * 4 : 0);
-  static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= 216 * 1024, "rings fit beside the static shared memory");
+  constexpr int kRoom = 227 * 1024 - kWarps * 1216;  // beside what the kernel declares (1126 bytes a warp)
+  static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= kRoom, "rings fit beside the static shared memory");
   AttnArgs a = a0;
   a.stage_bytes = kStage + ((s.cols * D * 2 + 127) & ~127);
   a.ring_bytes = a.stage_bytes * STAGES;
@@ -1176,13 +1208,22 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   auto kern = paged_attn_kernel<D, BITS, NT, HALF, TM, kWarps, STAGES>;
   size_t smem = (size_t)kWarps * a.ring_bytes;
   const size_t first = (size_t)kWarps * s.cols * D * 4;
-  if (smem + first <= 216 * 1024) {
+  if (smem + first <= (size_t)kRoom) {
     smem += first;
     a.scratch = nullptr;
   }
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), granted, smem)) { return rc; }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)s.ctas, 1, 1);
+  // Solo: a CTA has all of a (sequence, column block), so nothing spans CTAs and the second kernel and the line are saved
+  // (3 us), but the machine is used as far as there are such CTAs and no longer than the longest lasts. Measured, 8 warps,
+  // bf16, solo against the line: 8 CTAs of 64 / 256 / 512 / 1024 tokens 3.8 / 5.4 / 7.0 / 10.1 us against 7.1 / 7.3 / 7.4 / 7.8;
+  // 128 CTAs 4.0 / 5.7 / 7.4 / 15.2 against 7.9 / 9.2 / 10.8 / 18.2. The lengths are the device's, so the rule goes by the
+  // longest that the table or the window allows, and stops at twice what suits a few CTAs: one long
+  // sequence among short ones would hold the call up.
+  const int64_t longest = a.window > 0 ? std::min<int64_t>(a.window + 16 * TM, s.capacity) : s.capacity;
+  const int64_t solo_ctas = (int64_t)a.batch * a.hk, suits = 64 * kWarps;
+  a.solo = solo_ctas <= s.ctas && longest <= 2 * suits && longest * (s.ctas - solo_ctas) <= suits * s.ctas;
+  cfg.gridDim = dim3((unsigned)(a.solo ? solo_ctas : s.ctas), 1, 1);
   cfg.blockDim = dim3(kWarps * 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -1192,6 +1233,7 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   VPQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a));
+  if (a.solo) { return VPQ_OK; }
   cfg.gridDim = dim3((unsigned)s.ctas, (unsigned)s.cols, 1);
   cfg.blockDim = dim3(kJoinWarps * 32, 1, 1);
   cfg.dynamicSmemBytes = 0;
