@@ -97,6 +97,8 @@ def test_norm_rope_refuses(vpq, kw, code):
     (dict(token_stride=128, head_stride=0, page_stride=32768), INVALID),
     (dict(token_stride=128, head_stride=4096, page_stride=-32768), INVALID),
     (dict(token_stride=128, head_stride=4096, page_stride=1 << 60), INVALID),
+    (dict(token_stride=1 << 30, head_stride=4096, page_stride=32768), INVALID),
+    (dict(token_stride=128, head_stride=1 << 30, page_stride=32768), INVALID),
 ])
 def test_a_cache_is_checked(vpq, kw, code):
     L = vpq.lib()
@@ -192,6 +194,20 @@ def test_python_refuses_cpu_tensors_and_wrong_types(vpq):
         ops.PagedKVCache(pages.to(torch.uint8), pages.to(torch.uint8))
     with pytest.raises(ValueError, match="16 or 8"):
         ops.PagedKVCache.empty(2, 16, 2, 64, bits=4, device="cpu")
+
+
+def test_page_tables_that_may_be_parts_of_wider_ones(vpq):
+    t = torch.zeros(6, 9, dtype=torch.int32)
+    part = t[1:4, 2:7]
+    assert vpq.ops._table(part, -1, 3) == (part.data_ptr(), 9, 5)
+    assert vpq.ops._table(t[:1, :4], -1, 1)[1:] == (0, 4)
+    assert vpq.ops._table(t[:, 3].unsqueeze(1), -1, 6)[1:] == (9, 1)
+    # stride 0 means "dense" to the library: a broadcast table would be read past its end
+    for bad in (t[:1, :4].expand(3, 4), t[:, :1].expand(6, 4), t.t(), t[0], t.long(), t[:, ::2]):
+        with pytest.raises(ValueError, match="page_table"):
+            vpq.ops._table(bad, -1, bad.shape[0])
+    with pytest.raises(ValueError, match="page_table"):
+        vpq.ops._table(t, -1, 5)
 
 
 def test_status_string_of_a_bad_index(vpq):

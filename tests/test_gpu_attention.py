@@ -600,6 +600,31 @@ def test_attention_strided_queries_and_outputs(vpq):
     assert (outs[:, :4] == 5).all() and (outs[:, 12:] == 5).all()
 
 
+def test_attention_slices_of_tables_and_single_pages(vpq):
+    """A page table that is part of a wider one; a cache of one page and one head whose other strides mean nothing."""
+    g = gen(18)
+    lens = [70, 33, 130]
+    c, table = filled(vpq, g, "dense", lens, 16, 2, 64, 16)
+    q = normal(g, 3, 8, 64).to(BF)
+    want = check_attention(vpq, q, c, table, lens)
+    wide = torch.full((5, table.shape[1] + 7), -1, dtype=torch.int32, device="cuda")
+    wide[1:4, 3:3 + table.shape[1]] = table
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    assert torch.equal(vpq.ops.paged_attention(q, c, wide[1:4, 3:3 + table.shape[1]], dl), want)
+    for bits in (16, 8):
+        one = vpq.ops.PagedKVCache.empty(1, 48, 1, 64, bits)
+        odd = [None if t is None else torch.as_strided(t, t.shape, (1, 3) + t.stride()[2:]) for t in (one.k, one.v, one.k_scales, one.v_scales)]
+        two = vpq.ops.PagedKVCache(*odd)
+        x = normal(g, 40, 1, 64).to(BF)
+        slots = torch.arange(40, device="cuda")
+        vpq.ops.kv_store(x, x, two, slots)
+        for a, b in zip(vpq.ops.kv_load(one, slots), vpq.ops.kv_load(two, slots)):
+            assert torch.equal(a, b)
+        check_attention(vpq, q[:1, :4], two, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), [40])
+    with pytest.raises(ValueError, match="page_table"):
+        vpq.ops.paged_attention(q, c, table.t().contiguous().t(), dl)
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_attention_in_a_graph_follows_the_lengths(vpq, bits):
     """Captured once, replayed for other lengths, queries and page tables; two graphs on two streams at once."""

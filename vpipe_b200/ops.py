@@ -498,6 +498,18 @@ def _index(name, t, dev, dtype, shape):
     return t.data_ptr()
 
 
+def _table(t, dev, B):
+    """Pointer, row stride (entries; 0: one row) and columns of a page table. The library takes stride 0 as "dense", which
+    rows that share their memory are not."""
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 or t.shape[0] != B:
+        raise ValueError(f"vpipe_b200.ops: page_table must be int32 [{B}, max_pages] on cuda:{dev}")
+    pages = t.shape[1]
+    sb, sp = t.stride()
+    if (sp != 1 and pages > 1) or (B > 1 and sb < pages):
+        raise ValueError("vpipe_b200.ops: the rows of page_table must be contiguous and must not overlap")
+    return t.data_ptr(), sb if B > 1 else 0, pages
+
+
 class PagedKVCache:
     """The pages of a key-value cache: k, v [pages, kv_heads, page_size, head_dim], bfloat16, or uint8 codes with
     k_scales, v_scales bfloat16 [pages, kv_heads, page_size, head_dim / 64, 2] = (scale, bias). Any strides whose last
@@ -650,7 +662,8 @@ def kv_load(cache, slots, k_out=None, v_out=None, stream=None):
 
 def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=None, stream=None):
     """Attention of one new token per sequence over the cache (vpq_paged_attention_bf16): q [B, q_heads, head_dim],
-    page_table int32 [B, max_pages], seq_lens int32 [B] (the new token's own key included), window 0 = all tokens.
+    page_table int32 [B, max_pages] (rows with any stride: a slice of a wider table is fine), seq_lens int32 [B] (the new
+    token's own key included), window 0 = all tokens.
     Lengths are read on the device, so a captured call serves any. The workspace is allocated per call on the stream
     that the call runs on."""
     dev = cache._dev
@@ -658,11 +671,10 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
         with _Placed(dev, stream):
             return paged_attention(q, cache, page_table, seq_lens, scale, window, out)
     shape = q.shape
-    if len(shape) != 3 or shape[2] != cache.head_dim or page_table.dim() != 2:
-        raise ValueError(f"vpipe_b200.ops: q must be bfloat16 [batch, q_heads, {cache.head_dim}], page_table int32 "
-                         "[batch, max_pages]")
+    if len(shape) != 3 or shape[2] != cache.head_dim:
+        raise ValueError(f"vpipe_b200.ops: q must be bfloat16 [batch, q_heads, {cache.head_dim}]")
     B, hq, _ = shape
-    pages = page_table.shape[1]
+    pt, ts, pages = _table(page_table, dev, B)
     if scale is None:
         scale = 0.0
     elif not scale > 0:
@@ -670,8 +682,8 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
     out = torch.empty_like(q, memory_format=_DENSE) if out is None else out
     pq, sq = _heads("q", q, dev, shape)
     po, so = _heads("out", out, dev, shape)
-    d = _lib.PagedAttentionDesc(pq, po, sq, so, _index("page_table", page_table, dev, _I32, (B, pages)),
-                                _index("seq_lens", seq_lens, dev, _I32, (B,)), 0, B, pages, hq, window, scale)
+    d = _lib.PagedAttentionDesc(pq, po, sq, so, pt, _index("seq_lens", seq_lens, dev, _I32, (B,)), ts, B, pages, hq, window,
+                                scale)
     if B == 0:
         return out
     L, ref = lib(), C.byref(d)
