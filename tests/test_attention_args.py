@@ -196,6 +196,21 @@ def test_python_refuses_cpu_tensors_and_wrong_types(vpq):
         ops.PagedKVCache.empty(2, 16, 2, 64, bits=4, device="cpu")
 
 
+def test_broadcast_rows_are_refused(vpq):
+    """Stride 0 means "dense" to the library, so rows that share their memory would be read past its end."""
+    rows = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    assert vpq.ops._heads("q", rows, -1, rows.shape)[1] == 0
+    with pytest.raises(ValueError, match="share"):
+        vpq.ops._heads("q", rows.expand(5, 4, 64), -1, (5, 4, 64))
+    one = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16).expand(3, 2, 16, 64)
+    with pytest.raises(ValueError, match="share"):
+        vpq.ops.PagedKVCache(one, one)
+    codes = torch.zeros(3, 2, 16, 64, dtype=torch.uint8)
+    pairs = torch.zeros(1, 1, 1, 1, 2, dtype=torch.bfloat16).expand(3, 2, 16, 1, 2)
+    with pytest.raises(ValueError, match="share"):
+        vpq.ops.PagedKVCache(codes, codes, pairs, pairs)
+
+
 def test_page_tables_that_may_be_parts_of_wider_ones(vpq):
     t = torch.zeros(6, 9, dtype=torch.int32)
     part = t[1:4, 2:7]

@@ -489,7 +489,11 @@ def _heads(name, t, dev, shape):
     sm, sh, sd = t.stride()
     if sd != 1 or (sh != shape[2] and shape[1] > 1):
         raise ValueError(f"vpipe_b200.ops: the heads of a row of {name} must be contiguous")
-    return t.data_ptr(), sm if shape[0] > 1 else 0
+    if shape[0] <= 1:
+        return t.data_ptr(), 0
+    if sm == 0:  # "dense" to the library
+        raise ValueError(f"vpipe_b200.ops: the rows of {name} share their memory")
+    return t.data_ptr(), sm
 
 
 def _index(name, t, dev, dtype, shape):
@@ -521,6 +525,8 @@ class PagedKVCache:
         want = torch.uint8 if quantised else torch.bfloat16
         if (v_scales is not None) != quantised or k.dtype != want or v.dtype != want:
             raise ValueError("PagedKVCache: bfloat16 pages without scales, or uint8 codes with k_scales and v_scales")
+        if any(t is not None and t.dim() >= 4 and t.stride(2) == 0 for t in (k, v, k_scales, v_scales)):
+            raise ValueError("PagedKVCache: tokens share their memory")  # stride 0: "dense" to the library
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.device != v.device or not k.is_cuda:
             raise ValueError("PagedKVCache: k and v must be alike, [pages, kv_heads, page_size, head_dim] on a CUDA device")
         if k.stride(3) != 1:
