@@ -600,6 +600,22 @@ def test_attention_strided_queries_and_outputs(vpq):
     assert (outs[:, :4] == 5).all() and (outs[:, 12:] == 5).all()
 
 
+def test_attention_after_a_refused_call_and_with_the_widest_window(vpq):
+    """A refused call leaves nothing behind that a later one trips over; a window may be as wide as its type."""
+    g = gen(19)
+    lens = [70, 700]
+    c, table = filled(vpq, g, "dense", lens, 16, 2, 64, 16)
+    q = normal(g, 2, 8, 64).to(BF)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    with pytest.raises(vpq.VpqError):
+        vpq.ops.paged_attention(q, c, table[:, :0], dl)
+    for window in (0, 2 ** 31 - 1, 2 ** 31 - 16):
+        check_attention(vpq, q, c, table, lens, window=window)
+    for window in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="window"):
+            vpq.ops.paged_attention(q, c, table, dl, window=window)
+
+
 def test_attention_slices_of_tables_and_single_pages(vpq):
     """A page table that is part of a wider one; a cache of one page and one head whose other strides mean nothing."""
     g = gen(18)

@@ -1220,7 +1220,7 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   // 128 CTAs 4.0 / 5.7 / 7.4 / 15.2 against 7.9 / 9.2 / 10.8 / 18.2. The lengths are the device's, so the rule goes by the
   // longest that the table or the window allows, and stops at twice what suits a few CTAs: one long
   // sequence among short ones would hold the call up.
-  const int64_t longest = a.window > 0 ? std::min<int64_t>(a.window + 16 * TM, s.capacity) : s.capacity;
+  const int64_t longest = a.window > 0 ? std::min<int64_t>((int64_t)a.window + 16 * TM, s.capacity) : s.capacity;
   const int64_t solo_ctas = (int64_t)a.batch * a.hk, suits = 64 * kWarps;
   a.solo = solo_ctas <= s.ctas && longest <= 2 * suits && longest * (s.ctas - solo_ctas) <= suits * s.ctas;
   cfg.gridDim = dim3((unsigned)(a.solo ? solo_ctas : s.ctas), 1, 1);
@@ -1327,7 +1327,9 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   const bool q8 = cache_host->bits == 8, two = s.nt == 2;
   const int qh = d.q_heads;
   // Tokens of a unit, warps and stages. A stage holds 8 to 16 KB, so that a warp's copies in flight cover the
-  // latency; the warps' rings fill the shared memory.
+  // latency; the warps' rings fill the shared memory. Measured at head_dim 128, warps x stages: 16 bits, 64 sequences of 1 to
+  // 16384 tokens, 8 x 2 / 10 x 2 / 6 x 3 / 4 x 4 in 89.9 / 89.0 / 89.7 / 95.2 us, one of 333 tokens 5.7 / 6.1 / 6.2 / 6.8; 8 bits,
+  // one of 131071 tokens, 8 x 2 / 10 x 2 / 6 x 3 in 52.0 / 54.8 / 58.9, and 58.2 with units of 16 tokens and 16 x 2.
   const bool half = s.cols <= 4;
 #define VPQ_GO(D, BITS, TM, W, S)                                    \
   if (half) { return launch<D, BITS, 1, true, TM, W, S>(a, s, qh, st); } \

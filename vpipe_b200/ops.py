@@ -685,6 +685,8 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
         scale = 0.0
     elif not scale > 0:
         raise ValueError("vpipe_b200.ops: scale must be positive")
+    if not 0 <= window < 1 << 31:
+        raise ValueError("vpipe_b200.ops: window must be from 0 (all tokens) to 2^31 - 1")
     out = torch.empty_like(q, memory_format=_DENSE) if out is None else out
     pq, sq = _heads("q", q, dev, shape)
     po, so = _heads("out", out, dev, shape)
@@ -694,7 +696,7 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
         return out
     L, ref = lib(), C.byref(d)
     need = cache._workspace_bytes.get(hq)  # goes by the heads alone
-    if need is None:
+    if not need:  # unknown, or 0: the descriptor of an earlier call was refused
         need = cache._workspace_bytes[hq] = int(L.vpq_paged_attention_bytes(ref, cache.ref))
     ws = cache._rows.new_empty((need + 1) // 2)  # bfloat16: two bytes each
     check(L.vpq_paged_attention_bf16(ref, cache.ref, ws.data_ptr(), need, _raw_stream(dev)))
