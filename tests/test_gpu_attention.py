@@ -308,6 +308,32 @@ def test_store_pass_is_norm_rope_then_store(vpq, bits, M, hq, hkv, D, rot, inter
 
 
 # ------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_many_rows_as_few(vpq, D, bits):
+    """Launches that take several heads at a time give what small ones give, for head counts that do and do not divide."""
+    g = gen(31)
+    for heads, kind in ((8, "dense"), (8, "token_major"), (4, "shared"), (11, "dense")):
+        M, ps = 7003, 48
+        c = layouts(vpq, kind, 160, ps, heads, D, bits)
+        k, v = (normal(g, M, heads, D).to(BF) for _ in range(2))
+        slots = torch.randperm(160 * ps, generator=g, device="cuda")[:M].contiguous()
+        slots[5], slots[M - 1], slots[4000] = -1, -7, 160 * ps + 3
+        vpq.ops.kv_store(k, v, c, slots)
+        kl, vl = vpq.ops.kv_load(c, slots)
+        for m in range(0, M, 500):
+            few = slice(m, min(m + 500, M))
+            d = layouts(vpq, kind, 160, ps, heads, D, bits)
+            vpq.ops.kv_store(k[few], v[few], d, slots[few].contiguous())
+            a, b = vpq.ops.kv_load(d, slots[few].contiguous())
+            assert torch.equal(a, kl[few]) and torch.equal(b, vl[few])
+            a, b = vpq.ops.kv_load(c, slots[few].contiguous())
+            assert torch.equal(a, kl[few]) and torch.equal(b, vl[few])
+        for bad in (5, M - 1, 4000):
+            assert (kl[bad] == 0).all() and (vl[bad] == 0).all()
+        assert indexes_reported(vpq) == 2
+
+
 def filled(vpq, g, kind, lens, ps, heads, D, bits, gain=1.0, spare=2):
     """A cache with random tokens, NaN everywhere else, and the page table: columns past a sequence's pages hold
     numbers that must never be followed."""

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace vpq {
 
@@ -160,6 +161,9 @@ __device__ __forceinline__ void split_slot(int64_t slot, const KvView& kv, uint3
 
 // MODE 0: q and k rows out. 16 / 8: q rows out, k and v into a cache of that width. HPT: heads of a chunk, all
 // requested before the first is used; their table row, norm weights and addresses are fetched once.
+// Bound by memory where rows go out as bf16: 16320 tokens of 40 + 40 heads of 128 in 106.7 us, 6.34 TB/s or 97 % of a
+// copy's rate. Into an 8-bit cache the quantizer's instructions bound it: 8191 tokens of 32 + 8 + 8 heads of 128 in
+// 50.6 us, 4.77 TB/s or 73 %. One token: 1.84 us (3.5 us with an 8-bit store), a launch and one chain of loads.
 template <int D, int MODE, int HPT>
 __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
   constexpr int LPH = D / 8;
@@ -323,7 +327,8 @@ struct CopyArgs {
 };
 
 // Rows into the cache (STORE), or out of it: eight values a lane and head, 8 bytes of codes and their pair (or 16
-// bytes of bf16) on the cache's side, 16 bytes on the rows'.
+// bytes of bf16) on the cache's side, 16 bytes on the rows'. Bound by memory: store and load of 65536 rows of 8 heads of
+// 128 with 8 bits in 135 us, 6.09 TB/s or 93 % of a copy's rate; of 512 rows in 4.3 us, two launches.
 template <int D, int BITS, bool STORE, int HPT>
 __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ CopyArgs A) {
   constexpr int LPH = D / 8;
@@ -376,6 +381,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
         }
       }
     } else {
+      using Off = std::conditional_t<(HPT > 4), uint64_t, uint32_t>;  // four heads' offsets fit 32 bits (kv_check)
       uint32_t pair[HPT];
       const int reads = live && there ? n : 0;
 #pragma unroll
@@ -386,9 +392,9 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
           if (BITS == 16) {
             raw[i] = *reinterpret_cast<const uint4*>(cache + i * A.kv.head_bytes);
           } else {
-            const uint2 c = *reinterpret_cast<const uint2*>(cache + i * A.kv.head_bytes);
+            const uint2 c = *reinterpret_cast<const uint2*>(cache + (Off)i * A.kv.head_bytes);
             raw[i].x = c.x, raw[i].y = c.y;
-            pair[i] = *reinterpret_cast<const uint32_t*>(pairs + i * A.kv.shead_bytes);
+            pair[i] = *reinterpret_cast<const uint32_t*>(pairs + (Off)i * A.kv.shead_bytes);
           }
         }
       }
@@ -413,7 +419,9 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
 bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
 
 // One head per lane group while the launch is too small to fill the machine (a decode step lives by
-// latency), four once there are waves of them.
+// latency), four once there are waves of them. Measured, one against four: one token 1.84 against 2.35 us, with an 8-bit
+// store 3.4 against 4.6; 2048 tokens of 32 + 8 heads 20.4 against 12.4, 65536 rows through an 8-bit cache 176 against 140.
+// (Two: 13.9 and 145; eight: 14.4 and 133, of which the loads' part is taken below.)
 bool is_wide(int64_t M, int heads, int D, int sms) { return M * heads > (int64_t)sms * 8 * (256 / (D / 8)) * 2; }
 
 struct Launch {
@@ -421,6 +429,8 @@ struct Launch {
 };
 // Deals `parts` parts of heads[] heads each. The blocks of all parts together are enough for `waves` times what the SMs
 // hold at 64 registers a thread, shared out by the parts' heads.
+// Measured, half as many / this / no limit: norm and rotation of 16320 tokens (4 waves) 107.7 / 106.7 / 113.2 us, 65536 rows
+// through an 8-bit cache (8 waves) 144 / 140 / 147.
 void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int sms, Deal* deals, Launch* l) {
   const int groups = 256 / (D / 8);
   int total = 0, threads = 32;
@@ -491,15 +501,21 @@ int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
   Launch l;
   const int sms = num_sms();
   const bool wide = a.kv.kv_heads >= 4 && is_wide(a.M, 2 * a.kv.kv_heads, D, sms);
+  // Codes come in half rows, so eight heads of them are as many bytes in flight as four of bf16. Loads of 8 bits, 8 heads,
+  // eight against four at a time: D 128 65536 rows 64.3 against 68.9 us, D 64 131072 rows 64.8 against 69.7, D 256 32768 rows
+  // 64.4 against 67.2. Stores, and loads of 16 bits, gain 1 % or lose as much.
+  constexpr int kMost = BITS == 8 && !STORE ? 8 : 4;
+  const bool most = wide && a.kv.kv_heads % kMost == 0;
   const int heads[2] = {a.kv.kv_heads, a.kv.kv_heads};
-  deal(a.M, heads, 2, wide ? 4 : 1, 8, D, sms, a.deal, &l);
-  if (D == 64) {
-    return wide ? launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<64, BITS, STORE, 1>, l, st, a);
-  }
-  if (D == 128) {
-    return wide ? launch_with_pdl(kv_copy_kernel<128, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<128, BITS, STORE, 1>, l, st, a);
-  }
-  return wide ? launch_with_pdl(kv_copy_kernel<256, BITS, STORE, 4>, l, st, a) : launch_with_pdl(kv_copy_kernel<256, BITS, STORE, 1>, l, st, a);
+  deal(a.M, heads, 2, most ? kMost : (wide ? 4 : 1), 8, D, sms, a.deal, &l);
+#define VPQ_GO(DIM)                                                                                   \
+  return most   ? launch_with_pdl(kv_copy_kernel<DIM, BITS, STORE, kMost>, l, st, a)                  \
+         : wide ? launch_with_pdl(kv_copy_kernel<DIM, BITS, STORE, 4>, l, st, a)                      \
+                : launch_with_pdl(kv_copy_kernel<DIM, BITS, STORE, 1>, l, st, a);
+  if (D == 64) { VPQ_GO(64) }
+  if (D == 128) { VPQ_GO(128) }
+  VPQ_GO(256)
+#undef VPQ_GO
 }
 
 bool known_dim(int d) { return d == 64 || d == 128 || d == 256; }
