@@ -334,6 +334,42 @@ def test_many_rows_as_few(vpq, D, bits):
         assert indexes_reported(vpq) == 2
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("hq,hkv,D,rot,interleaved", [(32, 8, 128, 128, False), (14, 2, 64, 32, True),
+                                                      (16, 2, 256, 64, False), (11, 11, 128, 128, True)])
+def test_many_rows_of_the_pass_as_few(vpq, bits, hq, hkv, D, rot, interleaved):
+    """The same of the pass into the cache: how rows are dealt changes nothing."""
+    g = gen(32)
+    M, ps = 6003, 16
+    rows = normal(g, M, hq + 2 * hkv, D).to(BF)
+    q, k, v = rows[:, :hq], rows[:, hq:hq + hkv], rows[:, hq + hkv:]
+    qw, kw = normal(g, D).to(BF), (1 + 0.1 * normal(g, D)).to(BF)
+    table = angles(512, rot, g)
+    pos = torch.randint(0, 512, (M,), generator=g, device="cuda", dtype=torch.int32)
+    slots = torch.randperm(400 * ps, generator=g, device="cuda")[:M].contiguous()
+    pos[17], slots[3000], slots[M - 1] = -1, -1, -5
+    live = (pos >= 0) & (slots >= 0)
+
+    def run(take, c):
+        n = len(range(*take.indices(M)))
+        out = torch.full((n, hq, D), 7.0, dtype=BF, device="cuda")
+        vpq.ops.qkv_norm_rope_store(q[take], k[take], v[take], qw, kw, table, pos[take].contiguous(), c,
+                                    slots[take].contiguous(), interleaved=interleaved, q_out=out)
+        return out
+
+    c, d = (layouts(vpq, "dense", 400, ps, hkv, D, bits) for _ in range(2))
+    whole = run(slice(0, M), c)
+    for m in range(0, M, 300):
+        assert torch.equal(run(slice(m, min(m + 300, M)), d), whole[m:m + 300])
+    assert (whole[17] == 7).all()
+    for a, b in zip(vpq.ops.kv_load(c, slots), vpq.ops.kv_load(d, slots)):
+        assert torch.equal(a[live], b[live])
+    check_norm_rope(whole[pos >= 0], *ref_norm_rope(q[pos >= 0], qw, table, pos[pos >= 0].long(), 1e-6, interleaved))
+    for x, y in ((c.k, d.k), (c.v, d.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert indexes_reported(vpq) == 0
+
+
 def filled(vpq, g, kind, lens, ps, heads, D, bits, gain=1.0, spare=2):
     """A cache with random tokens, NaN everywhere else, and the page table: columns past a sequence's pages hold
     numbers that must never be followed."""

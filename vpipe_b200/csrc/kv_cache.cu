@@ -163,7 +163,7 @@ __device__ __forceinline__ void split_slot(int64_t slot, const KvView& kv, uint3
 // requested before the first is used; their table row, norm weights and addresses are fetched once.
 // Bound by memory where rows go out as bf16: 16320 tokens of 40 + 40 heads of 128 in 106.7 us, 6.34 TB/s or 97 % of a
 // copy's rate. Into an 8-bit cache the quantizer's instructions bound it: 8191 tokens of 32 + 8 + 8 heads of 128 in
-// 50.6 us, 4.77 TB/s or 73 %. One token: 1.84 us (3.5 us with an 8-bit store), a launch and one chain of loads.
+// 38.9 us, 74 %. One token: 1.84 us (3.5 us with an 8-bit store), a launch and one chain of loads.
 template <int D, int MODE, int HPT>
 __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
   constexpr int LPH = D / 8;
@@ -428,13 +428,15 @@ struct Launch {
   dim3 grid, block;
 };
 // Deals `parts` parts of heads[] heads each. The blocks of all parts together are enough for `waves` times what the SMs
-// hold at 64 registers a thread, shared out by the parts' heads.
-// Measured, half as many / this / no limit: norm and rotation of 16320 tokens (4 waves) 107.7 / 106.7 / 113.2 us, 65536 rows
-// through an 8-bit cache (8 waves) 144 / 140 / 147.
-void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int sms, Deal* deals, Launch* l) {
+// hold at 64 registers a thread, shared out by the parts' chunks, those of k and v counted `costly` times.
+// Measured, half as many waves / this / no limit: norm and rotation of 16320 tokens (4 waves) 107.7 / 106.7 / 113.2 us, 65536
+// rows through an 8-bit cache (8 waves) 144 / 140 / 147. Rows into a cache cost more than query rows (slot, quantizer) and
+// their blocks come last; counted once / twice: 8191 tokens of 32 + 8 + 8 heads of 128 into 16 bits 37.8 / 36.7 us, into 8 bits
+// 40.9 / 38.9 (three times: 40.8); of 16 + 2 + 2 heads of 256 into 8 bits 40.2 / 38.5 (shared out by heads, not chunks: 44.8).
+void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int sms, int costly, Deal* deals, Launch* l) {
+  auto weight = [&](int part) { return part > 0 ? costly : 1; };
   const int groups = 256 / (D / 8);
   int total = 0, threads = 32;
-  for (int i = 0; i < parts; ++i) { total += heads[i]; }
   uint32_t first = 0;
   for (int i = 0; i < parts; ++i) {
     Deal& d = deals[i];
@@ -445,13 +447,14 @@ void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int
     // few tokens: spread them
     if (d.token_blocks > 1 || M < sms) { d.tokens = 1; }
     d.rcp = (65536u + d.per_block - 1) / d.per_block;
+    total += d.chunks * weight(i);
     threads = std::max(threads, d.tokens * d.per_block * (D / 8));
   }
   threads = (threads + 31) & ~31;
   for (int i = 0; i < parts; ++i) {
     Deal& d = deals[i];
     const int64_t need = (M + d.tokens - 1) / d.tokens;
-    const int64_t cap = (int64_t)sms * (1024 / threads) * waves * heads[i] / total / d.token_blocks;
+    const int64_t cap = (int64_t)sms * (1024 / threads) * waves * (d.chunks * weight(i)) / total / d.token_blocks;
     const int64_t blocks = std::min(need, std::max<int64_t>(cap, 1));
     d.first = first;
     d.step = (uint32_t)(blocks * d.tokens);
@@ -482,7 +485,7 @@ int launch_norm(const QkArgs& a0, int D, cudaStream_t st) {
   Launch l;
   const int sms = num_sms();
   const bool wide = is_wide(a.M, a.heads[0] + (MODE ? 2 : 1) * a.heads[1], D, sms);
-  deal(a.M, a.heads, MODE ? 3 : 2, wide ? 4 : 1, 4, D, sms, a.deal, &l);
+  deal(a.M, a.heads, MODE ? 3 : 2, wide ? 4 : 1, 4, D, sms, MODE ? 2 : 1, a.deal, &l);
   if (D == 64) {
     return wide ? launch_with_pdl(norm_rope_store_kernel<64, MODE, 4>, l, st, a)
                 : launch_with_pdl(norm_rope_store_kernel<64, MODE, 1>, l, st, a);
@@ -507,7 +510,7 @@ int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
   constexpr int kMost = BITS == 8 && !STORE ? 8 : 4;
   const bool most = wide && a.kv.kv_heads % kMost == 0;
   const int heads[2] = {a.kv.kv_heads, a.kv.kv_heads};
-  deal(a.M, heads, 2, most ? kMost : (wide ? 4 : 1), 8, D, sms, a.deal, &l);
+  deal(a.M, heads, 2, most ? kMost : (wide ? 4 : 1), 8, D, sms, 1, a.deal, &l);
 #define VPQ_GO(DIM)                                                                                   \
   return most   ? launch_with_pdl(kv_copy_kernel<DIM, BITS, STORE, kMost>, l, st, a)                  \
          : wide ? launch_with_pdl(kv_copy_kernel<DIM, BITS, STORE, 4>, l, st, a)                      \
