@@ -196,6 +196,14 @@ def test_python_refuses_cpu_tensors_and_wrong_types(vpq):
         ops.PagedKVCache.empty(2, 16, 2, 64, bits=4, device="cpu")
 
 
+def test_packed_descriptors_are_the_structures(vpq):
+    for cls, fields in ((_lib.QkDesc, 22), (_lib.PagedAttentionDesc, 12)):
+        values = [2 ** 40 + 7 * i if i < 5 else 3 + i for i in range(fields - 1)] + [0.25]
+        if cls is _lib.PagedAttentionDesc:
+            values[6] = 2 ** 40
+        assert bytes(cls(*values)) == cls.pack(*values)
+
+
 def test_broadcast_rows_are_refused(vpq):
     """Stride 0 means "dense" to the library, so rows that share their memory would be read past its end."""
     rows = torch.zeros(1, 4, 64, dtype=torch.bfloat16)

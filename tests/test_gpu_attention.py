@@ -673,6 +673,8 @@ def test_attention_after_a_refused_call_and_with_the_widest_window(vpq):
         vpq.ops.paged_attention(q, c, table[:, :0], dl)
     for window in (0, 2 ** 31 - 1, 2 ** 31 - 16):
         check_attention(vpq, q, c, table, lens, window=window)
+    with pytest.raises(ValueError, match="one page"):
+        vpq.ops.PagedKVCache.empty(0, 16, 2, 64)
     for window in (-1, 2 ** 31, 2 ** 32 + 5):
         with pytest.raises(ValueError, match="window"):
             vpq.ops.paged_attention(q, c, table, dl, window=window)

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _PATH = os.path.join(_HERE, "libvpq.so")
@@ -128,6 +129,8 @@ class QkDesc(C.Structure):
                 ("k_norm_w", C.c_void_p), ("cos_sin", C.c_void_p), ("positions", C.c_void_p), ("M", C.c_int64),
                 ("table_rows", C.c_int64), ("q_heads", C.c_int32), ("kv_heads", C.c_int32),
                 ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
+    # The same bytes, a microsecond sooner than through the fields (a decode step fills one per layer).
+    pack = struct.Struct("@5P5q4P2q5if").pack
 
 
 class PagedAttentionDesc(C.Structure):
@@ -136,6 +139,7 @@ class PagedAttentionDesc(C.Structure):
                 ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("table_stride", C.c_int64),
                 ("batch", C.c_int32), ("max_pages", C.c_int32), ("q_heads", C.c_int32), ("window", C.c_int32),
                 ("scale", C.c_float)]
+    pack = struct.Struct("@2P2q2Pq4if0q").pack
 
 
 class VpqError(RuntimeError):

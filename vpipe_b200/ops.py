@@ -455,6 +455,7 @@ def qmm_grouped_down(codes, scales, biases, x_sorted, tile2e, sdst=None, y_rows=
 _BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _DENSE = torch.contiguous_format
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 class _Placed:
@@ -478,7 +479,7 @@ def _elsewhere(dev, stream) -> bool:
         raise ValueError("vpipe_b200.ops: rows must be bfloat16 on a CUDA device (no CPU path)")
     if stream is not None and stream.device.index != dev:
         raise ValueError(f"vpipe_b200.ops: the stream belongs to {stream.device}, the tensors to cuda:{dev}")
-    return stream is not None or dev != torch.cuda.current_device()
+    return stream is not None or dev != _current_device()
 
 
 def _heads(name, t, dev, shape):
@@ -486,6 +487,8 @@ def _heads(name, t, dev, shape):
     if t.dtype is not _BF16 or t.get_device() != dev or t.shape != shape:
         raise ValueError(f"vpipe_b200.ops: {name} must be bfloat16 {tuple(shape)} on cuda:{dev} (no CPU path), "
                          f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), 0
     sm, sh, sd = t.stride()
     if sd != 1 or (sh != shape[2] and shape[1] > 1):
         raise ValueError(f"vpipe_b200.ops: the heads of a row of {name} must be contiguous")
@@ -529,6 +532,8 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: tokens share their memory")  # stride 0: "dense" to the library
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.device != v.device or not k.is_cuda:
             raise ValueError("PagedKVCache: k and v must be alike, [pages, kv_heads, page_size, head_dim] on a CUDA device")
+        if k.numel() == 0:
+            raise ValueError("PagedKVCache: at least one page")
         if k.stride(3) != 1:
             raise ValueError("PagedKVCache: the last dimension must be contiguous")
         pages, heads, size, dim = k.shape
@@ -551,7 +556,7 @@ class PagedKVCache:
         self.ref = C.byref(d)
         self._dev = k.get_device()
         self._rows = k_scales if quantised else k  # a bfloat16 tensor of this device
-        self._workspace_bytes = {}
+        self._workspace = {}  # per number of query heads: a view of one element that has the workspace's size
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, bits=16, device="cuda"):
@@ -567,6 +572,8 @@ class PagedKVCache:
 
 
 def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, k_out):
+    """Checked arguments as the bytes of a vpq_qk_desc, the number of rows, q_out and k_out (made here if None; with v
+    there is no k_out)."""
     shape, kshape = q.shape, k.shape
     if len(shape) != 3 or len(kshape) != 3:
         raise ValueError("vpipe_b200.ops: q and k must be bfloat16 [rows, heads, head_dim]")
@@ -576,11 +583,13 @@ def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev
         kshape = (M, hkv, D)  # what _heads will say
     pq, sq = _heads("q", q, dev, shape)
     pk, sk = _heads("k", k, dev, kshape)
-    pv, sv = _heads("v", v, dev, kshape) if v is not None else (None, 0)
-    po, so = _heads("q_out", q_out, dev, shape)
-    pj, sj = _heads("k_out", k_out, dev, kshape) if k_out is not None else (None, 0)
-    wq = wk = pt = pp = None
-    rows = rot = 0
+    pv = so = pj = sj = sv = wq = wk = pt = pp = rows = rot = 0
+    if v is not None:
+        pv, sv = _heads("v", v, dev, kshape)
+    elif k_out is not None:
+        pj, sj = _heads("k_out", k_out, dev, kshape)
+    if q_out is not None:
+        po, so = _heads("q_out", q_out, dev, shape)
     if q_norm_w is not None:
         wq = _index("q_norm_w", q_norm_w, dev, _BF16, (D,))
     if k_norm_w is not None:
@@ -593,7 +602,14 @@ def _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev
         pt = _index("cos_sin", cos_sin, dev, _F32, table)
     if positions is not None:
         pp = _index("positions", positions, dev, _I32, (M,))
-    return _lib.QkDesc(pq, pk, pv, po, pj, sq, sk, sv, so, sj, wq, wk, pt, pp, M, rows, hq, hkv, D, rot, interleaved, eps)
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=_DENSE)
+        po = q_out.data_ptr()
+    if k_out is None and v is None:
+        k_out = torch.empty_like(k, memory_format=_DENSE)
+        pj = k_out.data_ptr()
+    return _lib.QkDesc.pack(pq, pk, pv, po, pj, sq, sk, sv, so, sj, wq, wk, pt, pp, M, rows, hq, hkv, D, rot, interleaved,
+                            eps), M, q_out, k_out
 
 
 def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=None, eps=1e-6, interleaved=False,
@@ -606,13 +622,9 @@ def qk_norm_rope(q, k, q_norm_w=None, k_norm_w=None, cos_sin=None, positions=Non
     if _elsewhere(dev, stream):
         with _Placed(dev, stream):
             return qk_norm_rope(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, q_out, k_out)
-    q_out = torch.empty_like(q, memory_format=_DENSE) if q_out is None else q_out
-    k_out = torch.empty_like(k, memory_format=_DENSE) if k_out is None else k_out
-    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, None, q_out, k_out)
-    if d.M != 0:
-        rc = lib().vpq_qk_norm_rope_bf16(C.byref(d), _raw_stream(dev))
-        if rc != 0:
-            check(rc)
+    d, M, q_out, k_out = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, None, q_out, k_out)
+    if M != 0:
+        check(lib().vpq_qk_norm_rope_bf16(d, _raw_stream(dev)))
     return q_out, k_out
 
 
@@ -625,11 +637,10 @@ def qkv_norm_rope_store(q, k, v, q_norm_w, k_norm_w, cos_sin, positions, cache, 
         with _Placed(dev, stream):
             return qkv_norm_rope_store(q, k, v, q_norm_w, k_norm_w, cos_sin, positions, cache, slots, eps, interleaved,
                                        q_out)
-    q_out = torch.empty_like(q, memory_format=_DENSE) if q_out is None else q_out
-    d = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, None)
-    s = _index("slots", slots, dev, _I64, (d.M,))
-    if d.M != 0:
-        check(lib().vpq_qkv_norm_rope_store_bf16(C.byref(d), cache.ref, s, _raw_stream(dev)))
+    d, M, q_out, _ = _qk_desc(q, k, q_norm_w, k_norm_w, cos_sin, positions, eps, interleaved, dev, v, q_out, None)
+    s = _index("slots", slots, dev, _I64, (M,))
+    if M != 0:
+        check(lib().vpq_qkv_norm_rope_store_bf16(d, cache.ref, s, _raw_stream(dev)))
     return q_out
 
 
@@ -657,10 +668,17 @@ def kv_load(cache, slots, k_out=None, v_out=None, stream=None):
     M = slots.numel()
     s = _index("slots", slots, dev, _I64, (M,))
     shape = (M, cache.kv_heads, cache.head_dim)
-    k_out = cache._rows.new_empty(shape) if k_out is None else k_out
-    v_out = cache._rows.new_empty(shape) if v_out is None else v_out
-    pk, sk = _heads("k_out", k_out, dev, shape)
-    pv, sv = _heads("v_out", v_out, dev, shape)
+    sk = sv = 0
+    if k_out is None:
+        k_out = cache._rows.new_empty(shape)
+        pk = k_out.data_ptr()
+    else:
+        pk, sk = _heads("k_out", k_out, dev, shape)
+    if v_out is None:
+        v_out = torch.empty_like(k_out, memory_format=_DENSE)
+        pv = v_out.data_ptr()
+    else:
+        pv, sv = _heads("v_out", v_out, dev, shape)
     if M != 0:
         check(lib().vpq_kv_load_bf16(cache.ref, pk, pv, sk, sv, s, M, _raw_stream(dev)))
     return k_out, v_out
@@ -683,23 +701,29 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
     pt, ts, pages = _table(page_table, dev, B)
     if scale is None:
         scale = 0.0
-    elif not scale > 0:
-        raise ValueError("vpipe_b200.ops: scale must be positive")
+    elif not 0 < scale <= 3.4e38:
+        raise ValueError("vpipe_b200.ops: scale must be positive and finite")
     if not 0 <= window < 1 << 31:
         raise ValueError("vpipe_b200.ops: window must be from 0 (all tokens) to 2^31 - 1")
-    out = torch.empty_like(q, memory_format=_DENSE) if out is None else out
     pq, sq = _heads("q", q, dev, shape)
-    po, so = _heads("out", out, dev, shape)
-    d = _lib.PagedAttentionDesc(pq, po, sq, so, pt, _index("seq_lens", seq_lens, dev, _I32, (B,)), ts, B, pages, hq, window,
-                                scale)
+    ps = _index("seq_lens", seq_lens, dev, _I32, (B,))
+    so = 0
+    if out is None:
+        out = torch.empty_like(q, memory_format=_DENSE)
+        po = out.data_ptr()
+    else:
+        po, so = _heads("out", out, dev, shape)
     if B == 0:
         return out
-    L, ref = lib(), C.byref(d)
-    need = cache._workspace_bytes.get(hq)  # goes by the heads alone
-    if not need:  # unknown, or 0: the descriptor of an earlier call was refused
-        need = cache._workspace_bytes[hq] = int(L.vpq_paged_attention_bytes(ref, cache.ref))
-    ws = cache._rows.new_empty((need + 1) // 2)  # bfloat16: two bytes each
-    check(L.vpq_paged_attention_bf16(ref, cache.ref, ws.data_ptr(), need, _raw_stream(dev)))
+    L, d = lib(), _lib.PagedAttentionDesc.pack(pq, po, sq, so, pt, ps, ts, B, pages, hq, window, scale)
+    like = cache._workspace.get(hq)  # its size goes by the heads alone
+    if like is None:
+        need = int(L.vpq_paged_attention_bytes(d, cache.ref))
+        like = cache._rows.as_strided(((need + 1) // 2,), (0,))  # bfloat16: two bytes each
+        if need:  # 0: this descriptor is refused below
+            cache._workspace[hq] = like
+    ws = torch.empty_like(like, memory_format=_DENSE)
+    check(L.vpq_paged_attention_bf16(d, cache.ref, ws.data_ptr(), 2 * like.numel(), _raw_stream(dev)))
     return out
 
 
