@@ -213,7 +213,7 @@ def prepare(case, seed):
                     c[n][a:b] = x
                 else:
                     c[n][a:b], c[n + "s"][a:b] = _quantise(x.float())
-    return s
+        return s
 
 
 # ------------------------------------------------------------------------------------------------ plain forms
