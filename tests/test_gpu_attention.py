@@ -624,6 +624,41 @@ def test_attention_nan_and_infinity_stay_with_their_sequence(vpq):
     assert got[2, 1].isnan().all() and torch.equal(got[2, [0, 2, 3]], clean[2, [0, 2, 3]])
 
 
+@pytest.mark.parametrize("room", [0, 600])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_8_bits_nan_and_infinity_stay_with_their_group(vpq, D, room):
+    """64 values with a NaN or an infinity among them are NaN as a whole; the other groups of the row, the other heads
+    and the other sequences are what they would be without. (`room`: more columns of the table, so both splits.)"""
+    g = gen(14 + D)
+    lens, ps, G = [40, 50, 700, 90], 16, D // 64
+    c, table = filled(vpq, g, "dense", lens, ps, 2, D, 8)
+    wide = torch.nn.functional.pad(table, (0, room), value=1 << 30)
+    q = normal(g, 4, 8, D).to(BF)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    clean = vpq.ops.paged_attention(q, c, wide, dl)
+    want, tol = ref_attention(q, c, table, lens, 1 / math.sqrt(D), 0)
+    at = lambda b, t: (table[b, t // ps].long(), slice(None), t % ps)  # noqa: E731
+    # (sequence, token, key head, group): the first token, one in the middle and the last
+    spoilt = [(1, 35, 0, G - 1), (2, 0, 1, 0), (2, 350, 1, 0), (2, 699, 1, 0)]
+    bad = torch.zeros(4, 2, G, dtype=torch.bool, device="cuda")
+    for i, (b, t, h, grp) in enumerate(spoilt):
+        page, _, place = at(b, t)
+        c.v_scales[page, h, place, grp] = float("nan")  # what the store makes of such a group
+        if i == 2:
+            c.v_scales[page, h, place, grp] = torch.tensor([float("inf"), 0.0], dtype=BF, device="cuda")  # another's pages
+        bad[b, h, grp] = True
+    page, _, place = at(3, 17)
+    c.k_scales[page, 0, place, 0] = float("nan")  # a key: every weight of its head is NaN
+    bad[3, 0] = True
+    got = vpq.ops.paged_attention(q, c, wide, dl)
+    dead = bad.repeat_interleave(4, 1).repeat_interleave(64, 2)
+    assert not got[dead].isfinite().any()
+    err = (got.to(F64) - want).abs()
+    assert (err <= tol)[~dead].all(), float((err / tol)[~dead].max())
+    same = (~bad.any(2)).repeat_interleave(4, 1)
+    assert torch.equal(got[same], clean[same])
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_attention_bad_pages_and_lengths(vpq, bits):
     g = gen(15)

@@ -750,7 +750,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         }
       }
       top = __reduce_max_sync(0xffffffffu, top);
-      const int e = (int)(top >> 7) - 126;  // every scale is below 2^e
+      if (top >= 0x7f80u) {  // a NaN or an infinity spoils its own group's values; the others' rounding does not go by it
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const uint32_t x = vp[i][h][g] & 0x7fffu;
+              top = max(top, x < 0x7f80u ? x : 0u);
+            }
+          }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+      }
+      const int e = (int)(top >> 7) - 126;  // every scale that is a number is below 2^e
       if (e > sigma) {
         grows = true;
         rescale = ex2((float)(sigma - e));
