@@ -122,6 +122,26 @@ def test_an_8_bit_cache_is_checked(vpq, kw, code):
     assert attend(L, attn(), c) == code
 
 
+def test_an_8_bit_cache_with_scale_strides_out_of_range_is_refused(vpq):
+    """The pairs of up to four heads are addressed with 32 bits, so a scale's strides, two bytes an element, end where those
+    of bf16 pages do: below 2^30 bytes."""
+    L = vpq.lib()
+    far, last = 1 << 29, (1 << 29) - 4  # elements of two bytes
+
+    def calls(c):
+        yield L.vpq_kv_store_bf16(C.byref(c), P, P, 0, 0, P, 5, None)
+        yield L.vpq_kv_load_bf16(C.byref(c), P, P, 0, 0, P, 5, None)
+        yield store_pass(L, qk(), c)
+        yield attend(L, attn(), c)
+
+    for token, head in ((4, far), (far, 128), (4, far + 1024), (4, (1 << 30) - 4), ((1 << 30) - 4, 128)):
+        c = cache8(scale_token_stride=token, scale_head_stride=head, scale_page_stride=1 << 33)
+        assert set(calls(c)) == {INVALID}, (token, head)
+    for token, head in ((4, last), (last, 128)):
+        c = cache8(scale_token_stride=token, scale_head_stride=head, scale_page_stride=1 << 33)
+        assert set(calls(c)) == {CUDA}, (token, head)
+
+
 def test_store_pass_refuses(vpq):
     L = vpq.lib()
     assert store_pass(L, qk(v=None), cache()) == INVALID

@@ -635,8 +635,8 @@ int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
   // the stride of the only head or page does not matter
   if (c->kv_heads == 1) { hs = shs = 0; }
   if (c->num_pages == 1) { ps = sps = 0; }
-  const int64_t lim = INT_MAX / 2 / elt;  // four heads' offsets fit 32 bits
-  if (ts > lim || hs > lim || sts > lim || shs > lim || ps > ((int64_t)1 << 46) / c->num_pages ||
+  const int64_t lim = INT_MAX / 2 / elt, slim = INT_MAX / 2 / 2;  // four heads' offsets in bytes fit 32 bits
+  if (ts > lim || hs > lim || sts > slim || shs > slim || ps > ((int64_t)1 << 46) / c->num_pages ||
       sps > ((int64_t)1 << 46) / c->num_pages) {
     return fail(VPQ_ERR_INVALID_ARG, "%s: a stride is out of range (token and head strides stay below 2^30 bytes)", who);
   }
