@@ -518,7 +518,8 @@ int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, i
  * workspace: device memory of vpq_paged_attention_bytes, 16-byte aligned, scratch of this call (calls
  * that may overlap on the GPU need one each); it needs no initialisation and holds nothing afterwards.
  * q and out rows: stride in elements, 0 = q_heads * head_dim, 16-byte multiples. q_heads is a multiple of the
- * cache's kv_heads. scale 0: 1 / sqrt(head_dim). With an 8-bit cache scale * |q| must stay below 2^116. */
+ * cache's kv_heads. scale 0: 1 / sqrt(head_dim); else from 2^-126 to 2.3586e38 (times log2(e) it is an f32
+ * number). With an 8-bit cache scale * |q| must stay below 2^116. */
 typedef struct vpq_paged_attention_desc {
   const void* q;
   void* out;

@@ -186,6 +186,30 @@ def test_paged_attention_refuses(vpq, kw, code):
     assert vpq.lib().vpq_last_error()
 
 
+# f32 numbers around the ends of what a scale may be: 2^-126, and the largest whose product with log2(e) is a number.
+SMALLEST, LARGEST = 2.0 ** -126, 2.3586e38
+
+
+@pytest.mark.parametrize("scale,code", [
+    (2.0 ** -149, INVALID), (1e-40, INVALID), (1.17e-38, INVALID), (2.37e38, INVALID), (3.3e38, INVALID), (3.4e38, INVALID),
+    (SMALLEST, CUDA), (1e-30, CUDA), (1.0, CUDA), (2.35e38, CUDA), (LARGEST, CUDA), (0.0, CUDA),
+])
+def test_paged_attention_scales_at_the_ends_of_their_range(vpq, scale, code):
+    """A scale below the normal numbers, or one whose product with log2(e) is not a number, does not weigh as it says."""
+    for c in (cache(), cache8()):
+        assert attend(vpq.lib(), attn(scale=scale), c) == code
+
+
+def test_python_refuses_scales_that_f32_does_not_hold(vpq):
+    """1e-46 is positive and becomes 0 in f32, which means 1 / sqrt(head_dim) to the library."""
+    for scale in (1e-46, 1e-300, 1e-40, 0.0, -1.0, 2.37e38, 1e39, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            vpq.ops._scale(scale)
+    for scale in (SMALLEST, 1e-30, 0.125, 1, LARGEST):
+        assert vpq.ops._scale(scale) == scale
+    assert vpq.ops._scale(None) == 0.0
+
+
 def test_paged_attention_workspace(vpq):
     L = vpq.lib()
     need = L.vpq_paged_attention_bytes(C.byref(attn()), C.byref(cache()))

@@ -34,6 +34,7 @@
 #include "vpq_sm100.cuh"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 namespace vpq {
@@ -1304,7 +1305,11 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   if ((int64_t)d.max_pages * cache_host->page_size > INT_MAX - 64) {
     return fail(VPQ_ERR_UNSUPPORTED, "%s: max_pages * page_size must stay below 2^31", who);
   }
-  if (!(d.scale >= 0.0f) || d.scale > 3.4e38f) { return fail(VPQ_ERR_INVALID_ARG, "%s: scale must be finite and not negative", who); }
+  const float scale = d.scale != 0.0f ? d.scale : 1.0f / sqrtf((float)cache_host->head_dim);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale >= FLT_MIN) || !(scale_log2 <= FLT_MAX)) {
+    return fail(VPQ_ERR_INVALID_ARG, "%s: scale must be 0 (1 / sqrt(head_dim)) or from 2^-126 to 2.3586e38 (got %g)", who, (double)d.scale);
+  }
   if (!aligned16(d.q) || !aligned16(d.out) || (qs & 7) || (os & 7) || !aligned16(workspace) ||
       (reinterpret_cast<uintptr_t>(d.page_table) & 3) || (reinterpret_cast<uintptr_t>(d.seq_lens) & 3)) {
     return fail(VPQ_ERR_ALIGNMENT, "%s: q, out, their row strides and the workspace must be multiples of 16 bytes", who);
@@ -1336,8 +1341,7 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
             (cache_host->bits == 16 || a.kv.stoken_bytes == (uint32_t)(cache_host->head_dim / kKvGroup * 4));
   a.cta_rcp = (uint32_t)((((uint64_t)1 << 32) + s.ctas - 1) / s.ctas);
   a.few = d.batch <= 32 && (int64_t)d.max_pages * cache_host->page_size <= INT_MAX / 4;
-  const float scale = d.scale != 0.0f ? d.scale : 1.0f / sqrtf((float)cache_host->head_dim);
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool q8 = cache_host->bits == 8, two = s.nt == 2;
   const int qh = d.q_heads;

@@ -517,6 +517,15 @@ def _table(t, dev, B):
     return t.data_ptr(), sb if B > 1 else 0, pages
 
 
+def _scale(scale):
+    """The descriptor's scale, an f32 number: 0 says 1 / sqrt(head_dim), which what f32 has no number for must not become."""
+    if scale is None:
+        return 0.0
+    if not 2.0 ** -126 <= scale <= 2.3586e38:
+        raise ValueError("vpipe_b200.ops: scale must be from 2^-126 to 2.3586e38 (None: 1 / sqrt(head_dim))")
+    return scale
+
+
 class PagedKVCache:
     """The pages of a key-value cache: k, v [pages, kv_heads, page_size, head_dim], bfloat16, or uint8 codes with
     k_scales, v_scales bfloat16 [pages, kv_heads, page_size, head_dim / 64, 2] = (scale, bias). Any strides whose last
@@ -699,10 +708,7 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
         raise ValueError(f"vpipe_b200.ops: q must be bfloat16 [batch, q_heads, {cache.head_dim}]")
     B, hq, _ = shape
     pt, ts, pages = _table(page_table, dev, B)
-    if scale is None:
-        scale = 0.0
-    elif not 0 < scale <= 3.4e38:
-        raise ValueError("vpipe_b200.ops: scale must be positive and finite")
+    scale = _scale(scale)
     if not 0 <= window < 1 << 31:
         raise ValueError("vpipe_b200.ops: window must be from 0 (all tokens) to 2^31 - 1")
     pq, sq = _heads("q", q, dev, shape)
