@@ -588,6 +588,18 @@ def test_attention_8_bit_scales_of_any_size(vpq, gain):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("power", [120, 103, 60, -60, -112, -120])
+def test_attention_large_scales_of_small_queries(vpq, bits, power):
+    """Scores of ordinary size from a scale and queries that are not: only their product may bound the call."""
+    g = gen(16)
+    lens, D = [333, 40], 128
+    c, table = filled(vpq, g, "dense", lens, 16, 2, D, bits)
+    q = (normal(g, 2, 8, D) * 2.0 ** -power).to(BF)
+    assert (q.abs() > 2.0 ** -126).float().mean() > 0.9
+    check_attention(vpq, q, c, table, lens, scale=0.1 * 2.0 ** power)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 def test_attention_averages_many_values(vpq, bits):
     """Equal weights over 131072 tokens, each warp adding up tens of thousands of them: what is left of the values is
     a three-hundredth of each, and must not drown in the sums it is taken from. (All sequences share the pages.)"""

@@ -617,6 +617,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           e = min(max(e, -100), 127);
           const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
           const float down = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+          // a code's 2^24, the power of two and the scale in an order in which nothing but their product can overflow
+          const float mul = e > 100 ? down * A.scale_log2 * 16777216.0f : down * 16777216.0f * A.scale_log2;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
 #pragma unroll
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
           }
 #pragma unroll
           for (int c = 0; c < CN; ++c) {  // the same for the columns of this lane's scores
-            q_mul[n][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * (A.scale_log2 * 16777216.0f);  // codes' 2^24
+            q_mul[n][c] = __shfl_sync(0xffffffffu, mul, (2 * t + c) * 4);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               q_sum[n][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * t + c) * 4) * A.scale_log2;
