@@ -454,8 +454,9 @@ def qmm_grouped_down(codes, scales, biases, x_sorted, tile2e, sdst=None, y_rows=
 # A decode step makes these calls once a layer, so the checks below are written for a short way through Python.
 _BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _DENSE = torch.contiguous_format
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# torch's own short ways to the current stream and device; builds without CUDA do not bind them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class _Placed:
