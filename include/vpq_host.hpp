@@ -100,7 +100,8 @@ class Fence {
  public:
   Fence(cudaStream_t st, int enqueue_status) : _st(st), _status(enqueue_status) {}
   void wait() { wait_ok(nullptr); }
-  // false if an enqueue failed, the stream faulted, or a bounded device-side wait gave up
+  // false if an enqueue failed, the stream faulted, a bounded device-side wait gave up, or the attention block met an
+  // index outside of its table
   bool wait_ok(std::string* reason) {
     if (_status != VPQ_OK) {
       if (reason) { *reason = vpq_last_error(); }

@@ -9,8 +9,6 @@
 
 namespace vpq {
 
-__device__ uint32_t g_kv_status = 0;
-
 namespace {
 
 // How rows are dealt: a block belongs to one part (q, k or v; so what goes by the part is the same for all its
@@ -62,6 +60,7 @@ struct QkArgs {
   int rot, interleaved;
   float eps, inv_d;
   KvView kv;
+  uint32_t* status;  // index reports
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
     uint32_t row = mm;
     if (by_position) {
       turn = live && p >= 0 && (uint32_t)p < A.table_rows;
-      if (live && p >= 0 && !turn && l == 0) { atomicOr(&g_kv_status, kBadPosition); }
+      if (live && p >= 0 && !turn && l == 0) { atomicOr(A.status, kBadPosition); }
       row = turn ? (uint32_t)p : 0;
       if (m + deal.step < A.M) { p = __ldg(A.positions + m + deal.step); }
     }
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(c
     uint8_t* pairs = nullptr;
     if (to_cache) {
       const int64_t s = __ldg(A.slots + mm);
-      if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+      if (live && s >= A.num_slots && l == 0) { atomicOr(A.status, kBadSlot); }
       turn = turn && s >= 0 && s < A.num_slots;
       uint32_t page = 0, place = 0;
       if (turn) { split_slot(s, A.kv, page, place); }
@@ -323,6 +322,7 @@ struct CopyArgs {
   uint32_t M;
   const int64_t* slots;
   int64_t num_slots;
+  uint32_t* status;  // index reports
   Deal deal[2];
 };
 
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
       }
     }
     const bool there = s >= 0 && s < A.num_slots;
-    if (live && s >= A.num_slots && l == 0) { atomicOr(&g_kv_status, kBadSlot); }
+    if (live && s >= A.num_slots && l == 0) { atomicOr(A.status, kBadSlot); }
     uint32_t page = 0, place = 0;
     if (there) { split_slot(s, A.kv, page, place); }
     s = m + deal.step < A.M ? __ldg(A.slots + m + deal.step) : -1;  // of the next token
@@ -665,19 +665,6 @@ int kv_check(const char* who, const vpq_kv_cache* c, KvView* view) {
   return VPQ_OK;
 }
 
-int kv_status_read(cudaStream_t st, uint32_t* out) {
-  uint32_t v = 0;
-  VPQ_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, g_kv_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st));
-  VPQ_CUDA_OK(cudaStreamSynchronize(st));
-  if (v != 0) {
-    const uint32_t zero = 0;
-    VPQ_CUDA_OK(cudaMemcpyToSymbolAsync(g_kv_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
-    VPQ_CUDA_OK(cudaStreamSynchronize(st));
-  }
-  *out = v;
-  return VPQ_OK;
-}
-
 }  // namespace vpq
 
 using namespace vpq;
@@ -696,6 +683,7 @@ extern "C" int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream)
     return fail(VPQ_ERR_INVALID_ARG, "%s: k_out is k with another row stride", who);
   }
   if (int rc = require_sm100()) { return rc; }
+  if (int rc = index_status_word(&a.status)) { return rc; }
   return launch_norm<0>(a, desc_host->head_dim, static_cast<cudaStream_t>(stream));
 }
 
@@ -719,6 +707,7 @@ extern "C" int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const 
   a.slots = slots;
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
+  if (int rc = index_status_word(&a.status)) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return cache_host->bits == 8 ? launch_norm<8>(a, desc_host->head_dim, st)
                                : launch_norm<16>(a, desc_host->head_dim, st);
@@ -743,6 +732,7 @@ int copy_rows(const char* who, const vpq_kv_cache* c, const void* k, const void*
   a.M = (uint32_t)M;
   a.num_slots = a.kv.num_pages * a.kv.page_size;
   if (int rc = require_sm100()) { return rc; }
+  if (int rc = index_status_word(&a.status)) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return c->bits == 8 ? launch_copy<8, STORE>(a, D, st) : launch_copy<16, STORE>(a, D, st);
 }

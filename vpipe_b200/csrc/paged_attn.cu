@@ -39,8 +39,6 @@
 
 namespace vpq {
 
-__device__ uint32_t g_attn_status = 0;
-
 namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -56,6 +54,7 @@ struct AttnArgs {
   KvView kv;
   const uint8_t* q;
   uint8_t* out;
+  uint32_t* status;              // index reports
   int64_t q_stride, out_stride;  // bytes
   const int32_t* page_table;
   const int32_t* seq_lens;
@@ -300,7 +299,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     lkv = A.blocks == 1 ? lh : lh / A.blocks;
     lblk = lh - lkv * A.blocks;
     token_range(A, lb, lstart, llen);
-    if (tid == 0 && lh == 0 && __ldg(A.seq_lens + lb) > llen) { atomicOr(&g_attn_status, kBadLength); }
+    if (tid == 0 && lh == 0 && __ldg(A.seq_lens + lb) > llen) { atomicOr(A.status, kBadLength); }
     const int n = units_of<kUnit>(lstart, llen);
     if (n == 0) {  // no token: zeros
       const int h0 = lkv * A.group + lblk * A.cols, ncol = min(A.cols, A.group - lblk * A.cols);
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
     for (int b = b_lo; b < b_hi; ++b) {
       token_range(A, b, seen.x, seen.y);
       mine += span_of<kUnit>(seen.x, seen.y);
-      if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(&g_attn_status, kBadLength); }
+      if (blockIdx.x == 0 && __ldg(A.seq_lens + b) > seen.y) { atomicOr(A.status, kBadLength); }
     }
     int64_t excl, total;  // places (of one head) before the first of them, and of all
     if (A.few) {
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const AttnAr
         }
       }
       if (bad) {  // a page outside the cache holds no tokens: the live rows shrink to what is left
-        if (lane == 0) { atomicOr(&g_attn_status, kBadPage); }
+        if (lane == 0) { atomicOr(A.status, kBadPage); }
         if (TM == 1 || bad == 3) {
           lo = hi = 0;
         } else if (bad == 1) {
@@ -1261,19 +1260,6 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
 
 }  // namespace
 
-int attn_status_read(cudaStream_t st, uint32_t* out) {
-  uint32_t v = 0;
-  VPQ_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, g_attn_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st));
-  VPQ_CUDA_OK(cudaStreamSynchronize(st));
-  if (v != 0) {
-    const uint32_t zero = 0;
-    VPQ_CUDA_OK(cudaMemcpyToSymbolAsync(g_attn_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
-    VPQ_CUDA_OK(cudaStreamSynchronize(st));
-  }
-  *out = v;
-  return VPQ_OK;
-}
-
 }  // namespace vpq
 
 using namespace vpq;
@@ -1320,6 +1306,7 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
     return fail(VPQ_ERR_INVALID_ARG, "%s: workspace of %zu bytes, %zu are needed", who, bytes, s.total);
   }
   if (int rc = require_sm100()) { return rc; }
+  if (int rc = index_status_word(&a.status)) { return rc; }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.q = static_cast<const uint8_t*>(d.q);
   a.out = static_cast<uint8_t*>(d.out);

@@ -31,13 +31,15 @@
 #include "vpq_sm100.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 
 namespace vpq {
 
 // Status word of the tensor-core kernels: 0, or (site << 8) | role of the
-// first bounded wait that gave up.
-__device__ uint32_t g_qmm_status;
+// first bounded wait that gave up. Behind it the attention block's: the kinds of index that lay
+// outside of their tables. One read-back gets both.
+__device__ uint32_t g_qmm_status[2];
 
 namespace {
 
@@ -363,7 +365,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
           const int s = it % kStages;
           const uint32_t ph = (it / kStages) & 1u;
-          if (!mbar_wait(bar_empty(s), ph ^ 1u, (1u << 8) | kRoleTma, abort_flag, &g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait(bar_empty(s), ph ^ 1u, (1u << 8) | kRoleTma, abort_flag, g_qmm_status)) { ok = false; break; }
           mbar_expect_tx(bar_full(s), L::kXBytes + L::kCodeBytes);
           tma_load_2d(base + L::kOffX + s * L::kXBytes, &tmap_x, bar_full(s), kb * BK, m0);
           tma_load_2d(base + L::kOffCode + s * L::kCodeBytes, &tmap_w, bar_full(s), kb * (BK * BITS / 32), w_row0);
@@ -375,7 +377,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
         // index of the last iteration that used stage s, if any
         if (issued > (uint32_t)s) {
           const uint32_t last = ((issued - 1 - s) / kStages) * kStages + s;
-          mbar_wait(bar_full(s), (last / kStages) & 1u, (2u << 8) | kRoleTma, abort_flag, &g_qmm_status);
+          mbar_wait(bar_full(s), (last / kStages) & 1u, (2u << 8) | kRoleTma, abort_flag, g_qmm_status);
         }
       }
     }
@@ -390,7 +392,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
         const int a = ti & 1;
         const uint32_t aph = (ti >> 1) & 1u;
         ++ti;
-        if (!mbar_wait(bar_accempty(a), aph ^ 1u, (1u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!mbar_wait(bar_accempty(a), aph ^ 1u, (1u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(a * BN);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
@@ -398,8 +400,8 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
           const uint32_t ph = (it / kStages) & 1u;
           const int t = it % kBStages;
           const uint32_t bph = (it / kBStages) & 1u;
-          if (!mbar_wait(bar_full(s), ph, (2u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
-          if (!mbar_wait(bar_bfull(t), bph, (3u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait(bar_full(s), ph, (2u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait(bar_bfull(t), bph, (3u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
           tc_fence_after();
           const uint64_t a_desc = make_sw128_desc(base + L::kOffX + s * L::kXBytes);
           const uint64_t b_desc = make_sw128_desc(base + L::kOffB + t * L::kBBytes);
@@ -439,7 +441,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
         const uint32_t bph = (it / kBStages) & 1u;
         float sc, bi;
         sst.get(kb, sc, bi);
-        if (!warp_wait(bar_full(s), ph, (1u << 8) | kRoleDq, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!warp_wait(bar_full(s), ph, (1u << 8) | kRoleDq, abort_flag, g_qmm_status)) { ok = false; break; }
         const uint4* cp = reinterpret_cast<const uint4*>(base_ptr + L::kOffCode + s * L::kCodeBytes +
                                                          t_row * (BK * BITS / 8));
         uint32_t o[32];
@@ -473,7 +475,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
           }
         }
 
-        if (!warp_wait(bar_bempty(t), bph ^ 1u, (2u << 8) | kRoleDq, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!warp_wait(bar_bempty(t), bph ^ 1u, (2u << 8) | kRoleDq, abort_flag, g_qmm_status)) { ok = false; break; }
         unsigned char* bt = base_ptr + L::kOffB + t * L::kBBytes + row_off;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {  // 16-byte chunk c of the row lands at chunk (c ^ row%8)
@@ -498,7 +500,7 @@ affine_qmm_w4g64_kernel(const __grid_constant__ CUtensorMap tmap_x,
       const int a = ti & 1;
       const uint32_t aph = (ti >> 1) & 1u;
       ++ti;
-      if (!warp_wait(bar_accfull(a), aph, (1u << 8) | kRoleEpi, abort_flag, &g_qmm_status)) { ok = false; break; }
+      if (!warp_wait(bar_accfull(a), aph, (1u << 8) | kRoleEpi, abort_flag, g_qmm_status)) { ok = false; break; }
       tc_fence_after();
       const int m = m0 + warp * 32 + lane;  // warp w reads tensor-memory lanes 32w .. 32w+31
       const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)(a * BN);
@@ -1081,10 +1083,25 @@ __global__ void wait_probe_kernel(uint32_t polls, uint32_t hint_ns) {
     mbar_init(smem_u32(&bar), 1);
     abort_flag = 0;
     fence_mbar_init();
-    mbar_wait_limited(smem_u32(&bar), 0u, (0x7fu << 8) | 0x7fu, &abort_flag, &g_qmm_status, polls, hint_ns);
+    mbar_wait_limited(smem_u32(&bar), 0u, (0x7fu << 8) | 0x7fu, &abort_flag, g_qmm_status, polls, hint_ns);
   }
 }
+
+__global__ void clear_index_kernel(uint32_t seen) { atomicAnd(g_qmm_status + 1, ~seen); }
 }  // namespace
+
+int index_status_word(uint32_t** word) {
+  static std::atomic<uint32_t*> known[64] = {};  // per device
+  int dev = 0;
+  VPQ_CUDA_OK(cudaGetDevice(&dev));
+  uint32_t* p = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (!p) {
+    VPQ_CUDA_OK(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_qmm_status));
+    if (dev < 64) { known[dev].store(p, std::memory_order_relaxed); }
+  }
+  *word = p + 1;
+  return VPQ_OK;
+}
 }  // namespace vpq
 
 extern "C" int vpq_wait_probe(uint32_t polls, uint32_t hint_ns, void* stream) {
@@ -1102,9 +1119,10 @@ extern "C" int vpq_device_status(void* stream, uint32_t* detail) {
   clear_error();
   if (int rc = require_sm100()) { return rc; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  uint32_t v = 0;
-  VPQ_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, g_qmm_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st));
+  uint32_t words[2] = {0, 0};
+  VPQ_CUDA_OK(cudaMemcpyFromSymbolAsync(words, g_qmm_status, sizeof(words), 0, cudaMemcpyDeviceToHost, st));
   VPQ_CUDA_OK(cudaStreamSynchronize(st));
+  const uint32_t v = words[0], index = words[1];
   uint32_t vq = 0;
   if (int rc = qmv_status_read(st, &vq)) { return rc; }
   if (vq == 0) {
@@ -1130,14 +1148,14 @@ extern "C" int vpq_device_status(void* stream, uint32_t* detail) {
     VPQ_CUDA_OK(cudaStreamSynchronize(st));
     return fail(VPQ_ERR_TIMEOUT, "a bounded device-side wait gave up (site %u, role %u)", v >> 8, v & 0xffu);
   }
-  uint32_t ik = 0, ia = 0;
-  if (int rc = kv_status_read(st, &ik)) { return rc; }
-  if (int rc = attn_status_read(st, &ia)) { return rc; }
-  if ((ik | ia) != 0) {
-    ik |= ia;
-    if (detail) { *detail = ik | 0x40000u; }
-    return fail(VPQ_ERR_INDEX, "the attention block met an index outside of its table:%s%s%s%s", (ik & kBadPage) ? " page" : "",
-                (ik & kBadSlot) ? " slot" : "", (ik & kBadPosition) ? " position" : "", (ik & kBadLength) ? " length" : "");
+  if (index != 0) {
+    // Only what has been read is cleared: kernels of other streams may report something else meanwhile.
+    clear_index_kernel<<<1, 1, 0, st>>>(index);
+    VPQ_LAUNCH_OK("clear_index");
+    VPQ_CUDA_OK(cudaStreamSynchronize(st));
+    if (detail) { *detail = index | 0x40000u; }
+    return fail(VPQ_ERR_INDEX, "the attention block met an index outside of its table:%s%s%s%s", (index & kBadPage) ? " page" : "",
+                (index & kBadSlot) ? " slot" : "", (index & kBadPosition) ? " position" : "", (index & kBadLength) ? " length" : "");
   }
   return VPQ_OK;
 }

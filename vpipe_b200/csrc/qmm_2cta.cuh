@@ -232,7 +232,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
       }
       if (!seen) {
         comm_ok = 0;
-        atomicCAS(&g_qmm_status, 0u, (2u << 8) | kRoleSend);
+        atomicCAS(g_qmm_status, 0u, (2u << 8) | kRoleSend);
       }
     }
     __threadfence_system();
@@ -297,7 +297,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
           const bool must = loaded == q;
           if (!tile_ready(loaded / kChunksPerTile, must)) {
             if (must) {
-              atomicCAS(&g_qmm_status, 0u, (1u << 8) | kRoleSend);
+              atomicCAS(g_qmm_status, 0u, (1u << 8) | kRoleSend);
               ok = false;
             }
             break;
@@ -307,7 +307,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
         }
         if (!ok) { break; }
         const int slot = q % kSlots;
-        if (!mbar_wait(sbar + 8u * slot, (uint32_t)(q / kSlots) & 1u, (3u << 8) | kRoleSend, &comm_abort, &g_qmm_status)) {
+        if (!mbar_wait(sbar + 8u * slot, (uint32_t)(q / kSlots) & 1u, (3u << 8) | kRoleSend, &comm_abort, g_qmm_status)) {
           ok = false;
           break;
         }
@@ -388,7 +388,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
           const int s = it % kXStages;
           const uint32_t ph = (it / kXStages) & 1u;
-          if (!mbar_wait(bar_empty(s), ph ^ 1u, (1u << 8) | kRoleTma, abort_flag, &g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait(bar_empty(s), ph ^ 1u, (1u << 8) | kRoleTma, abort_flag, g_qmm_status)) { ok = false; break; }
           // the leader expects the x bytes of both CTAs; each CTA expects its own codes
           if (rank == 0) { mbar_expect_tx(bar_xfull(s), 2 * L::kXBytes); }
           mbar_expect_tx(bar_cfull(s), L::kCodeBytes);
@@ -402,9 +402,9 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
       for (int s = 0; s < kXStages; ++s) {
         if (it > (uint32_t)s) {
           const uint32_t last = ((it - 1 - s) / kXStages) * kXStages + s;
-          mbar_wait(bar_cfull(s), (last / kXStages) & 1u, (2u << 8) | kRoleTma, abort_flag, &g_qmm_status);
+          mbar_wait(bar_cfull(s), (last / kXStages) & 1u, (2u << 8) | kRoleTma, abort_flag, g_qmm_status);
           if (rank == 0) {
-            mbar_wait(bar_xfull(s), (last / kXStages) & 1u, (3u << 8) | kRoleTma, abort_flag, &g_qmm_status);
+            mbar_wait(bar_xfull(s), (last / kXStages) & 1u, (3u << 8) | kRoleTma, abort_flag, g_qmm_status);
           }
         }
       }
@@ -418,7 +418,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
       for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters, ++ti) {
         const int a = ti & 1;
         const uint32_t aph = (ti >> 1) & 1u;
-        if (!mbar_wait_cluster(bar_accempty(a), aph ^ 1u, (1u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!mbar_wait_cluster(bar_accempty(a), aph ^ 1u, (1u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(a * TN);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
@@ -426,8 +426,8 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
           const uint32_t ph = (it / kXStages) & 1u;
           const int t = it % kBTiles;
           const uint32_t bph = (it / kBTiles) & 1u;
-          if (!mbar_wait_cluster(bar_xfull(s), ph, (2u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
-          if (!mbar_wait_cluster(bar_bfull(t), bph, (3u << 8) | kRoleMma, abort_flag, &g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait_cluster(bar_xfull(s), ph, (2u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
+          if (!mbar_wait_cluster(bar_bfull(t), bph, (3u << 8) | kRoleMma, abort_flag, g_qmm_status)) { ok = false; break; }
           tc_fence_after();
           const uint64_t a_desc = make_sw128_desc(base + L::kOffX + s * L::kXBytes);
           const uint64_t b_desc = make_sw128_desc(base + L::kOffB + t * L::kBBytes);
@@ -475,7 +475,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
           sst.get(2 * kb, sc, bi);
           sst.get(2 * kb + 1, sc_hi, bi_hi);
         }
-        if (!warp_wait(bar_cfull(s), ph, (1u << 8) | kRoleDq, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!warp_wait(bar_cfull(s), ph, (1u << 8) | kRoleDq, abort_flag, g_qmm_status)) { ok = false; break; }
         const uint4* cp = reinterpret_cast<const uint4*>(base_ptr + L::kOffCode + s * L::kCodeBytes +
                                                          t_row * (BK * BITS / 8));
         uint32_t o[32];
@@ -525,7 +525,7 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
           }
         }
 
-        if (!warp_wait(bar_bempty(t), bph ^ 1u, (2u << 8) | kRoleDq, abort_flag, &g_qmm_status)) { ok = false; break; }
+        if (!warp_wait(bar_bempty(t), bph ^ 1u, (2u << 8) | kRoleDq, abort_flag, g_qmm_status)) { ok = false; break; }
         unsigned char* bt = base_ptr + L::kOffB + t * L::kBBytes + row_off;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {  // 16-byte chunk c of the row lands at chunk (c ^ row%8)
@@ -579,12 +579,12 @@ affine_qmm_w4g64_2cta_kernel(const __grid_constant__ CUtensorMap tmap_x,
           }
         }
         if (!__all_sync(0xffffffffu, seen)) {
-          if (lane == 0) { atomicCAS(&g_qmm_status, 0u, (4u << 8) | kRoleSend); }
+          if (lane == 0) { atomicCAS(g_qmm_status, 0u, (4u << 8) | kRoleSend); }
           direct = false;  // this GPU's y is still written; the peers' stay untouched
         }
         __threadfence_system();
       }
-      if (!warp_wait(bar_accfull(a), aph, (1u << 8) | kRoleEpi, abort_flag, &g_qmm_status)) { ok = false; break; }
+      if (!warp_wait(bar_accfull(a), aph, (1u << 8) | kRoleEpi, abort_flag, g_qmm_status)) { ok = false; break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)(a * TN);
       // The accumulator comes out of tensor memory one row per lane; it is transposed through a

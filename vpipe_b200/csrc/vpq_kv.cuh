@@ -26,8 +26,7 @@ struct KvView {
 
 // Checks a cache descriptor and fills `view`; kv_cache.cu.
 int kv_check(const char* who, const vpq_kv_cache* c, KvView* view);
-// Reads and clears the index reports of the two sources; kv_cache.cu, paged_attn.cu.
-int kv_status_read(cudaStream_t st, uint32_t* out);
-int attn_status_read(cudaStream_t st, uint32_t* out);
+// The current device's word that the kernels report indices in; qmm.cu, beside the word of vpq_device_status.
+int index_status_word(uint32_t** word);
 
 }  // namespace vpq
