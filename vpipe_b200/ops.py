@@ -709,7 +709,7 @@ def paged_attention(q, cache, page_table, seq_lens, scale=None, window=0, out=No
         raise ValueError(f"vpipe_b200.ops: q must be bfloat16 [batch, q_heads, {cache.head_dim}]")
     B, hq, _ = shape
     pt, ts, pages = _table(page_table, dev, B)
-    scale = _scale(scale)
+    scale = 0.0 if scale is None else _scale(scale)
     if not 0 <= window < 1 << 31:
         raise ValueError("vpipe_b200.ops: window must be from 0 (all tokens) to 2^31 - 1")
     pq, sq = _heads("q", q, dev, shape)
