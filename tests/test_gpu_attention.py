@@ -118,6 +118,36 @@ def test_norm_rope_without_norm_without_positions_and_in_place(vpq):
     assert a.shape == (0, 3, 64)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,hq,hkv", [(64, 32, 8), (64, 38, 3), (128, 32, 8), (128, 17, 5), (256, 14, 2)])
+def test_norm_rope_of_a_prompt(vpq, D, hq, hkv, interleaved):
+    """Rows of a prompt, out of place and in place: launches that take several heads at a time (2049 rows are enough for
+    that at each of these head sizes) against the formula, and against the same rows a few at a time."""
+    g = gen(D + hq)
+    M = 2049
+    assert M * (hq + hkv) > 148 * 8 * (256 // (D // 8)) * 2
+    rows = normal(g, M, hq + 2 * hkv, D).to(BF)
+    q, k = rows[:, :hq], rows[:, hq:hq + hkv]
+    qw, kw = normal(g, D).to(BF), (1 + 0.1 * normal(g, D)).to(BF)
+    for rot, by_position in ((D, True), (D // 2, True), (D, False)):
+        table = angles(5000, rot, g)
+        pos = torch.randint(0, 5000, (M,), generator=g, device="cuda", dtype=torch.int32) if by_position else None
+        at = pos.long() if by_position else torch.arange(M, device="cuda")
+        qo, ko = vpq.ops.qk_norm_rope(q, k, qw, kw, table, pos, interleaved=interleaved)
+        check_norm_rope(qo, *ref_norm_rope(q, qw, table, at, 1e-6, interleaved))
+        check_norm_rope(ko, *ref_norm_rope(k, kw, table, at, 1e-6, interleaved))
+        for m in (0, 1000, M - 5):
+            few = slice(m, m + 5)
+            a, b = vpq.ops.qk_norm_rope(q[few], k[few], qw, kw, table if by_position else table[few].contiguous(),
+                                        pos[few].contiguous() if by_position else None, interleaved=interleaved)
+            assert torch.equal(a, qo[few]) and torch.equal(b, ko[few])
+        here = rows.clone()
+        vpq.ops.qk_norm_rope(here[:, :hq], here[:, hq:hq + hkv], qw, kw, table, pos, interleaved=interleaved,
+                             q_out=here[:, :hq], k_out=here[:, hq:hq + hkv])
+        assert torch.equal(here[:, :hq], qo) and torch.equal(here[:, hq:hq + hkv], ko)
+        assert torch.equal(here[:, hq + hkv:], rows[:, hq + hkv:])
+
+
 def test_rows_with_a_position_outside_are_left_as_they_were(vpq):
     g = gen(6)
     M, D = 9, 64
@@ -505,6 +535,95 @@ def test_attention_window(vpq, bits, window):
     want, tol = ref_attention(q, c, want_table, lens, 1 / math.sqrt(128), window)
     assert ((got.to(F64) - want).abs() <= tol).all()
     assert indexes_reported(vpq) == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("window", [1, 17, 1000])
+def test_attention_window_that_cuts_many_sequences(vpq, bits, D, window):
+    """Windows that begin inside of sequences, with more (sequence, key head) pairs than SMs: one line of units from window
+    to window, whose runs begin and end anywhere in them."""
+    g = gen(window + D)
+    lens = [0, 1, 2, 16, 17, 999, 1000, 1001, 1016, 1017, 2500, 3000]
+    lens += torch.randint(0, 2000, (28,), generator=g, device="cuda").tolist()
+    hkv, ps = 4, 48
+    assert len(lens) * hkv > 148
+    c, table = filled(vpq, g, "dense", lens, ps, hkv, D, bits)
+    want_table = table.clone()
+    for b, n in enumerate(lens):  # pages that lie wholly before the window may be gone
+        table[b, :max(0, n - window) // ps] = -9
+    q = normal(g, len(lens), 2 * hkv, D).to(BF)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = vpq.ops.paged_attention(q, c, table, dl, window=window)
+    want, tol = ref_attention(q, c, want_table, lens, 1 / math.sqrt(D), window)
+    err = (got.to(F64) - want).abs()
+    assert (err <= tol).all(), float((err / tol.clamp(min=1e-300)).max())
+    assert indexes_reported(vpq) == 0
+
+
+def count_tokens(vpq, g, bits, D, hkv, per, lens, window, first=0):
+    """Attention that counts: queries of 0 give every token the weight 1, and key head h has a 1 only in tokens 16 i + r,
+    r = (first + h) % 16, there in column i % D. Every output is a small number of tokens over the window's length, so one
+    token that is lost or taken twice shows."""
+    ps, B = 48, len(lens)
+    need = [-(-n // ps) for n in lens]
+    pages = sum(need)
+    c = layouts(vpq, "dense", pages, ps, hkv, D, bits)
+    place = torch.randperm(pages, generator=g, device="cuda").int()
+    table = torch.full((B, max(need)), 1 << 30, dtype=torch.int32, device="cuda")
+    want = torch.zeros(B, hkv, D, dtype=F64, device="cuda")
+    used = 0
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = place[used:used + need[b]]
+        used += need[b]
+        t = torch.arange(n, device="cuda")
+        r = (first + torch.arange(hkv, device="cuda")) % 16
+        v = torch.zeros(n, hkv, D, dtype=BF, device="cuda")
+        v[t[:, None], torch.arange(hkv, device="cuda")[None], (t // 16 % D)[:, None]] = (t[:, None] % 16 == r[None]).to(BF)
+        vpq.ops.kv_store(normal(g, n, hkv, D).to(BF), v, c, table[b, t // ps].long() * ps + t % ps)
+        lo = max(0, n - window) if window else 0
+        # what a 1 reads back as: 254 times 1 / 255 rounded up to bf16, if the cache has 8 bits
+        one = 254 * 0.00393676757812 if bits == 8 else 1.0
+        want[b] = v[lo:].to(F64).sum(0) * one / (n - lo)
+    got = vpq.ops.paged_attention(torch.zeros(B, hkv * per, D, dtype=BF, device="cuda"), c, table,
+                                  torch.tensor(lens, dtype=torch.int32, device="cuda"), window=window)
+    # One rounding to bf16; in f32 the sum of weights is exact and its reciprocal and a product are two roundings. 8 bits: the
+    # two sums of 128 s (at most 0.51) over a sixteenth of the tokens differ by the roundings of at most 200 additions of
+    # two steps each, 200 * 2 E * 0.51 / 16 of the average.
+    want = want.repeat_interleave(per, 1)
+    tol = (U + 64 * E) * want + (16 * E if bits == 8 else 0)
+    # a token more or less is more than that
+    n = torch.tensor([min(n, window) if window else n for n in lens], device="cuda")
+    assert (tol.amax((1, 2)) < 0.99 / n).all()
+    err = (got.to(F64) - want).abs()
+    assert (err <= tol).all(), (int((err > tol).sum()), float((err * n[:, None, None]).max()))
+
+
+@pytest.mark.parametrize("per", [1, 5, 12])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_counts_every_token_once(vpq, bits, D, per):
+    """One key head over all CTAs, joined across all of them, for each place in sixteen; all sixteen at once; two sequences; a
+    window that begins inside of a unit and a page."""
+    g = gen(24 + D)
+    for r in range(16):
+        count_tokens(vpq, g, bits, D, 1, per, [40000 - 7 * r], 0, first=r)
+    count_tokens(vpq, g, bits, D, 16, per, [40003], 0)
+    count_tokens(vpq, g, bits, D, 16, per, [20011, 33333], 0)
+    for window in (9001, 19990):
+        count_tokens(vpq, g, bits, D, 1, per, [40000], window, first=window % 16)
+        count_tokens(vpq, g, bits, D, 16, per, [20011, 33333], window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_counts_every_token_of_short_sequences_once(vpq, bits, D):
+    """The same where a CTA has a whole sequence and key head, and where it has parts of several."""
+    g = gen(25 + D)
+    for n in (1, 15, 31, 32, 33, 47, 100, 333, 512):
+        count_tokens(vpq, g, bits, D, 16, 4, [n, 1, n], 0)
+    count_tokens(vpq, g, bits, D, 16, 4, [700 + 13 * i for i in range(20)], 0)
+    count_tokens(vpq, g, bits, D, 16, 4, [700 + 13 * i for i in range(20)], 333)
 
 
 def with_wide_tables(monkeypatch):
