@@ -493,16 +493,18 @@ int vpq_qk_norm_rope_bf16(const vpq_qk_desc* desc_host, void* stream);
 
 /* The same pass with the keys, and the values as they are, going straight to slot slots[m] of the
  * cache (slot = page * page_size + place in the page; 8-bit codes are made from the unrounded f32
- * keys). q_out is written for every row whose position is in the table, slot or not; a negative slot
- * stores nothing. Two rows must not name the same slot. */
+ * keys). q_out is written for every row whose position is in the table, slot or not; a negative slot, or a
+ * position that is not in the table, stores nothing. Two rows must not name the same slot. */
 int vpq_qkv_norm_rope_store_bf16(const vpq_qk_desc* desc_host, const vpq_kv_cache* cache_host,
                                  const int64_t* slots, void* stream);
 
 /* Rows k, v [M, kv_heads, head_dim] (row strides in elements, 0 = dense) into and out of the cache.
  * The 8-bit quantizer, per 64 values: bias = min rounded down to bf16, scale = (max - bias) / 255
- * rounded up to bf16 (at least 2^-126), code = rint((x - bias) / scale), so no value is clipped and each
- * reads back within scale / 2 (before load's rounding to bf16). 64 values with a NaN or infinity among them, or farther
- * apart than the largest float, read back as NaN. vpq_kv_load_bf16 gives zeros for a slot outside. */
+ * rounded up to bf16 (at least 2^-126), code = (x - bias) / scale rounded, so no value is clipped. The quotient is
+ * a product with an approximate reciprocal, so that one next to the middle between two codes may go to either;
+ * each value reads back within (1/2 + 2^-14) scale (before load's rounding to bf16). 64 values with a NaN or
+ * infinity among them, or farther apart than the largest float, read back as NaN. vpq_kv_load_bf16 gives zeros
+ * for a slot outside. */
 int vpq_kv_store_bf16(const vpq_kv_cache* cache_host, const void* k, const void* v, int64_t k_stride,
                       int64_t v_stride, const int64_t* slots, int64_t M, void* stream);
 int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, int64_t k_stride,
@@ -514,7 +516,9 @@ int vpq_kv_load_bf16(const vpq_kv_cache* cache_host, void* k_out, void* v_out, i
  * length 0 (or less) gives zeros. Token t lies in page page_table[b * table_stride + t / page_size];
  * entries of pages outside the token range are not read. A length above max_pages * page_size is cut to it and
  * reported, a page outside the cache holds no tokens and is reported. Scores, weights' sums and
- * products accumulate in f32; the result does not depend on timing.
+ * products accumulate in f32; the result does not depend on timing. Before their product with the values the weights
+ * are rounded: to bf16 with a 16-bit cache (2^-8 of each); times the values' scale to fp16 with an 8-bit one (2^-11 of
+ * each, or 2^-39 of the largest value scale of the sequence and key head, or of 2^-100, if those are more).
  * workspace: device memory of vpq_paged_attention_bytes, 16-byte aligned, scratch of this call (calls
  * that may overlap on the GPU need one each); it needs no initialisation and holds nothing afterwards.
  * q and out rows: stride in elements, 0 = q_heads * head_dim, 16-byte multiples. q_heads is a multiple of the
