@@ -162,7 +162,7 @@ __device__ __forceinline__ void split_slot(int64_t slot, const KvView& kv, uint3
 // requested before the first is used; their table row, norm weights and addresses are fetched once.
 // Bound by memory where rows go out as bf16: 16320 tokens of 40 + 40 heads of 128 in 106.7 us, 6.34 TB/s or 97 % of a
 // copy's rate. Into an 8-bit cache the quantizer's instructions bound it: 8191 tokens of 32 + 8 + 8 heads of 128 in
-// 38.9 us, 74 %. One token: 1.84 us (3.5 us with an 8-bit store), a launch and one chain of loads.
+// 39.4 us, 74 %. One token: 1.8 us (2.3 us with an 8-bit store), a launch and one chain of loads.
 template <int D, int MODE, int HPT>
 __global__ void __launch_bounds__(256, HPT > 1 ? 4 : 3) norm_rope_store_kernel(const __grid_constant__ QkArgs A) {
   constexpr int LPH = D / 8;
@@ -419,9 +419,9 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Co
 bool strides_ok(int64_t s, int64_t mult) { return s >= 0 && s % mult == 0; }
 
 // One head per lane group while the launch is too small to fill the machine (a decode step lives by
-// latency), four once there are waves of them. Measured, one against four: one token 1.84 against 2.35 us, with an 8-bit
-// store 3.4 against 4.6; 2048 tokens of 32 + 8 heads 20.4 against 12.4, 65536 rows through an 8-bit cache 176 against 140.
-// (Two: 13.9 and 145; eight: 14.4 and 133, of which the loads' part is taken below.)
+// latency), four once there are waves of them. Measured, one against four: one token 1.8 against 2.3 us, with an 8-bit
+// store 2.3 against 3.3; 2048 tokens of 32 + 8 heads 20.4 against 12.4, 65536 rows through an 8-bit cache 176 against 135.
+// (Two: 13.9 and 144; eight: 14.4 and 133, of which the loads' part is taken below.)
 bool is_wide(int64_t M, int heads, int D, int sms) { return M * heads > (int64_t)sms * 8 * (256 / (D / 8)) * 2; }
 
 struct Launch {
@@ -429,10 +429,10 @@ struct Launch {
 };
 // Deals `parts` parts of heads[] heads each. The blocks of all parts together are enough for `waves` times what the SMs
 // hold at 64 registers a thread, shared out by the parts' chunks, those of k and v counted `costly` times.
-// Measured, half as many waves / this / no limit: norm and rotation of 16320 tokens (4 waves) 107.7 / 106.7 / 113.2 us, 65536
-// rows through an 8-bit cache (8 waves) 144 / 140 / 147. Rows into a cache cost more than query rows (slot, quantizer) and
-// their blocks come last; counted once / twice: 8191 tokens of 32 + 8 + 8 heads of 128 into 16 bits 37.8 / 36.7 us, into 8 bits
-// 40.9 / 38.9 (three times: 40.8); of 16 + 2 + 2 heads of 256 into 8 bits 40.2 / 38.5 (shared out by heads, not chunks: 44.8).
+// Measured, half as many waves / this / no limit: norm and rotation of 16320 tokens (4 waves) 108.5 / 106.7 / 113.3 us, 65536
+// rows through an 8-bit cache (8 waves) 139 / 135 / 140. Rows into a cache cost more than query rows (slot, quantizer) and
+// their blocks come last; counted once / twice: 8191 tokens of 32 + 8 + 8 heads of 128 into 16 bits 38.1 / 36.3 us, into 8 bits
+// 41.6 / 39.4 (three times: 39.5); of 16 + 2 + 2 heads of 256 into 8 bits 39.6 / 37.9 (shared out by heads, not chunks: 44.8).
 void deal(int64_t M, const int* heads, int parts, int hpt, int waves, int D, int sms, int costly, Deal* deals, Launch* l) {
   auto weight = [&](int part) { return part > 0 ? costly : 1; };
   const int groups = 256 / (D / 8);
@@ -505,8 +505,8 @@ int launch_copy(const CopyArgs& a0, int D, cudaStream_t st) {
   const int sms = num_sms();
   const bool wide = a.kv.kv_heads >= 4 && is_wide(a.M, 2 * a.kv.kv_heads, D, sms);
   // Codes come in half rows, so eight heads of them are as many bytes in flight as four of bf16. Loads of 8 bits, 8 heads,
-  // eight against four at a time: D 128 65536 rows 64.3 against 68.9 us, D 64 131072 rows 64.8 against 69.7, D 256 32768 rows
-  // 64.4 against 67.2. Stores, and loads of 16 bits, gain 1 % or lose as much.
+  // eight against four at a time: D 128 65536 rows 63.4 against 69.2 us, D 64 131072 rows 63.7 against 69.4, D 256 32768 rows
+  // 63.4 against 66.7. Stores, and loads of 16 bits, gain 1 % or lose as much.
   constexpr int kMost = BITS == 8 && !STORE ? 8 : 4;
   const bool most = wide && a.kv.kv_heads % kMost == 0;
   const int heads[2] = {a.kv.kv_heads, a.kv.kv_heads};

@@ -1195,7 +1195,9 @@ int shape_of(const char* who, const vpq_paged_attention_desc* d, const vpq_kv_ca
   if (d->q_heads > 65536) { return fail(VPQ_ERR_UNSUPPORTED, "%s: at most 65536 query heads", who); }
   s->group = d->q_heads / c->kv_heads;
   // Two column blocks of eight share a read of the cache where the accumulators leave room (head_dim
-  // 256 has 64 of them per block); wider groups read it again, from L2 for the most part.
+  // 256 has 64 of them per block). Wider groups read it again, from HBM where a sequence is long: 64 sequences of 4096 tokens,
+  // four key heads, 16 bits, 8 / 16 query heads a key head at head_dim 256 1.08 / 2.15 GB and 172 / 329 us, 16 / 32 at
+  // head_dim 128 0.54 / 1.08 GB and 97.5 / 178 us.
   s->nt = (s->group > 8 && c->head_dim <= 128) ? 2 : 1;
   s->cols = s->group < 8 * s->nt ? s->group : 8 * s->nt;
   s->blocks = (s->group + s->cols - 1) / s->cols;
@@ -1216,7 +1218,7 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   static_assert(kWarps <= kMaxWarps, "the workspace is sized for kMaxWarps");
   static_assert(NT * 8 * D * 4 <= STAGES * 2 * 16 * TM * (D * BITS / 8), "a warp's partial result fits its ring");
   constexpr int kStage = 2 * 16 * TM * (D * BITS / 8) + (BITS == 8 ? 2 * 16 * TM * (D / kKvGroup) * 4 : 0);
-  constexpr int kRoom = 227 * 1024 - kWarps * 1216;  // beside what the kernel declares (1126 bytes a warp)
+  constexpr int kRoom = 227 * 1024 - kWarps * 1216;  // beside what the kernel declares (at most 1136 bytes a warp)
   static_assert(kWarps * STAGES * (kStage + NT * 8 * D * 2) <= kRoom, "rings fit beside the static shared memory");
   AttnArgs a = a0;
   a.stage_bytes = kStage + ((s.cols * D * 2 + 127) & ~127);
@@ -1232,11 +1234,17 @@ int launch(const AttnArgs& a0, const Shape& s, int q_heads, cudaStream_t st) {
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), granted, smem)) { return rc; }
   cudaLaunchConfig_t cfg = {};
   // Solo: a CTA has all of a (sequence, column block), so nothing spans CTAs and the second kernel and the line are saved
-  // (3 us), but the machine is used as far as there are such CTAs and no longer than the longest lasts. Measured, 8 warps,
-  // bf16, solo against the line: 8 CTAs of 64 / 256 / 512 / 1024 tokens 3.8 / 5.4 / 7.0 / 10.1 us against 7.1 / 7.3 / 7.4 / 7.8;
-  // 128 CTAs 4.0 / 5.7 / 7.4 / 15.2 against 7.9 / 9.2 / 10.8 / 18.2. The lengths are the device's, so the rule goes by the
-  // longest that the table or the window allows, and stops at twice what suits a few CTAs: one long
-  // sequence among short ones would hold the call up.
+  // (3 us), but the machine is used as far as there are such CTAs and no longer than the longest lasts. Measured, solo against
+  // the line, four query heads a key head unless said, a table as wide as the sequences:
+  //   8 warps (128, bf16), 8 CTAs of 64 / 256 / 512 / 1024 tokens 3.7 / 5.3 / 6.9 / 10.0 us against 7.0 / 7.2 / 7.3 / 7.8, 128 CTAs
+  //     3.9 / 5.5 / 7.2 / 10.5 against 7.5 / 9.1 / 10.7 / 13.9; (128, 8 bits), 8 CTAs of 512 / 1024 6.7 / 9.6 against 7.8 / 7.9;
+  //     (256, 8 bits), 8 CTAs of 256 / 512 7.3 / 10.1 against 9.2 / 9.0, 128 CTAs of 512 / 1024 10.6 / 16.0 against 14.7 / 20.2;
+  //   16 warps (64, bf16), 8 CTAs of 1024 / 2048 7.3 / 10.4 against 7.8 / 8.5, 128 CTAs 7.7 / 11.4 against 11.0 / 13.8; 8 bits alike;
+  //   12 warps (64, 8 bits, 12 heads), 8 CTAs of 512 / 1024 7.5 / 10.5 against 10.1 / 10.0, 128 CTAs of 1024 11.1 against 15.2;
+  //   5 warps (256, bf16), 8 CTAs of 256 / 512 7.9 / 11.2 against 8.5 / 8.7, 128 CTAs of 512 / 1024 11.7 / 24.6 against 15.7 / 29.8.
+  // The lengths are the device's, so the rule goes by the longest that the table or the window allows, and stops at twice
+  // what suits a few CTAs: one long sequence among short ones would hold the call up. (Of all these it takes the slower
+  // side for 512 tokens of (256, 8 bits), by 1 us, and for 1024 of (256, bf16) in 128 CTAs.)
   const int64_t longest = a.window > 0 ? std::min<int64_t>((int64_t)a.window + 16 * TM, s.capacity) : s.capacity;
   const int64_t solo_ctas = (int64_t)a.batch * a.hk, suits = 64 * kWarps;
   a.solo = solo_ctas <= s.ctas && longest <= 2 * suits && longest * (s.ctas - solo_ctas) <= suits * s.ctas;
@@ -1337,7 +1345,11 @@ extern "C" int vpq_paged_attention_bf16(const vpq_paged_attention_desc* desc_hos
   // Tokens of a unit, warps and stages. A stage holds 8 to 16 KB, so that a warp's copies in flight cover the
   // latency; the warps' rings fill the shared memory. Measured at head_dim 128, warps x stages: 16 bits, 64 sequences of 1 to
   // 16384 tokens, 8 x 2 / 10 x 2 / 6 x 3 / 4 x 4 in 89.9 / 89.0 / 89.7 / 95.2 us, one of 333 tokens 5.7 / 6.1 / 6.2 / 6.8; 8 bits,
-  // one of 131071 tokens, 8 x 2 / 10 x 2 / 6 x 3 in 52.0 / 54.8 / 58.9, and 58.2 with units of 16 tokens and 16 x 2.
+  // one of 131071 tokens, 8 x 2 / 10 x 2 / 6 x 3 in 52.0 / 54.8 / 58.9, and 58.2 with units of 16 tokens and 16 x 2. 64 sequences of
+  // 4096 tokens, eight key heads with four query heads each (head_dim 256: four) unless said: head_dim 64, 16 bits, 16 x 2 / 12 x 2 /
+  // 8 x 3 86.9 / 88.7 / 88.3; 8 bits, 16 x 2 / 12 x 2 / 8 x 2 54.0 / 55.0 / 64.3; twelve query heads, 16 bits, 8 x 3 / 8 x 2 / 12 x 2 /
+  // 16 x 2 101 / 104.5 / 92.5 / 93.3, 8 bits, 12 x 2 / 8 x 2 / 16 x 2 82.6 / 88.0 / 109.4; head_dim 256, 16 bits, 5 x 2 / 4 x 2 / 3 x 2
+  // 163.9 / 167.1 / 178.7, 8 bits, 8 x 2 / 6 x 2 / 5 x 3 95.3 / 110.7 / 129.4.
   const bool half = s.cols <= 4;
 #define VPQ_GO(D, BITS, TM, W, S)                                    \
   if (half) { return launch<D, BITS, 1, true, TM, W, S>(a, s, qh, st); } \
