@@ -728,6 +728,21 @@ def test_attention_8_bit_scales_of_any_size(vpq, gain):
     check_attention(vpq, q, c, table, [n], scale=0.1)
 
 
+@pytest.mark.parametrize("D,per", [(64, 4), (128, 4), (128, 12), (256, 6)])
+def test_attention_scales_of_either_sign(vpq, D, per):
+    """Pages that another quantizer has filled: scales of either sign, zeros among them, any codes."""
+    g = gen(26)
+    lens = [200, 33, 1000]
+    c, table = filled(vpq, g, "dense", lens, 16, 2, D, 8)
+    for pairs in (c.k_scales, c.v_scales):
+        s = normal(g, *pairs.shape[:-1]) * 0.01
+        pairs[..., 0] = torch.where(torch.rand(s.shape, generator=g, device="cuda") < 0.1, torch.zeros_like(s), s).to(BF)
+        pairs[..., 1] = normal(g, *pairs.shape[:-1]).to(BF)
+    for pages in (c.k, c.v):
+        pages.copy_(torch.randint(0, 256, pages.shape, generator=g, device="cuda", dtype=torch.uint8))
+    check_attention(vpq, normal(g, 3, 2 * per, D).to(BF), c, table, lens)
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("power", [120, 103, 60, -60, -112, -120])
 def test_attention_large_scales_of_small_queries(vpq, bits, power):
@@ -778,15 +793,16 @@ def test_attention_nan_and_infinity_stay_with_their_sequence(vpq):
 
 
 @pytest.mark.parametrize("room", [0, 600])
+@pytest.mark.parametrize("per", [4, 7, 12])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_attention_8_bits_nan_and_infinity_stay_with_their_group(vpq, D, room):
+def test_attention_8_bits_nan_and_infinity_stay_with_their_group(vpq, D, per, room):
     """64 values with a NaN or an infinity among them are NaN as a whole; the other groups of the row, the other heads
     and the other sequences are what they would be without. (`room`: more columns of the table, so both splits.)"""
     g = gen(14 + D)
     lens, ps, G = [40, 50, 700, 90], 16, D // 64
     c, table = filled(vpq, g, "dense", lens, ps, 2, D, 8)
     wide = torch.nn.functional.pad(table, (0, room), value=1 << 30)
-    q = normal(g, 4, 8, D).to(BF)
+    q = normal(g, 4, 2 * per, D).to(BF)
     dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
     clean = vpq.ops.paged_attention(q, c, wide, dl)
     want, tol = ref_attention(q, c, table, lens, 1 / math.sqrt(D), 0)
@@ -804,11 +820,11 @@ def test_attention_8_bits_nan_and_infinity_stay_with_their_group(vpq, D, room):
     c.k_scales[page, 0, place, 0] = float("nan")  # a key: every weight of its head is NaN
     bad[3, 0] = True
     got = vpq.ops.paged_attention(q, c, wide, dl)
-    dead = bad.repeat_interleave(4, 1).repeat_interleave(64, 2)
+    dead = bad.repeat_interleave(per, 1).repeat_interleave(64, 2)
     assert not got[dead].isfinite().any()
     err = (got.to(F64) - want).abs()
     assert (err <= tol)[~dead].all(), float((err / tol)[~dead].max())
-    same = (~bad.any(2)).repeat_interleave(4, 1)
+    same = (~bad.any(2)).repeat_interleave(per, 1)
     assert torch.equal(got[same], clean[same])
 
 
@@ -921,6 +937,47 @@ def test_attention_in_a_graph_follows_the_lengths(vpq, bits):
         torch.cuda.synchronize()
         for graph, q, dl, out, s in made:
             assert torch.equal(out, vpq.ops.paged_attention(q, c, table, dl)), (step, now)
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """What a call looks up once per device (kernels, the status word) may be looked up while a graph is captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, vpipe_b200
+ops = vpipe_b200.ops
+c = ops.PagedKVCache.empty(8, 16, 2, 64, 8)
+q, k = torch.randn(1, 4, 64, device="cuda").bfloat16(), torch.randn(1, 2, 64, device="cuda").bfloat16()
+slot, lens = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+table = torch.zeros(1, 8, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a, b = ops.qk_norm_rope(q, k)
+    ops.kv_store(k, k, c, slot)
+    o = ops.paged_attention(a, c, table, lens)
+    x, _ = ops.kv_load(c, slot)
+slot.fill_(999)
+g.replay()
+torch.cuda.synchronize()
+try:
+    ops.device_status()
+except vpipe_b200.VpqError as e:
+    assert e.status == 8
+else:
+    raise AssertionError("a slot outside was not reported")
+slot.fill_(5)
+lens.fill_(6)
+g.replay()
+torch.cuda.synchronize()
+assert ops.device_status() == 0 and torch.equal(a, q)
+assert (x.float() - k.float()).abs().max() < 0.02
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("hkv", [8, 1])
